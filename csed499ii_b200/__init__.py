@@ -11,7 +11,10 @@ Python surface mirrors the reference's ``marlin`` package
   ``matmul``);
 * :class:`Layer_2_4` / :func:`replace_linear` -- the torch module surface
   (``__init__.py:274-415``), packing on the GPU;
-* :mod:`csed499ii_b200.shard` -- column-parallel execution across GPUs.
+* :mod:`csed499ii_b200.shard` -- column-parallel execution across GPUs;
+* :mod:`csed499ii_b200.kv4` -- a 4-bit paged key/value cache for serving:
+  block tables and slots, quantising writes, attention (no counterpart in the
+  reference).
 
 All compute runs in the in-tree CUDA library through its C ABI
 (``include/sm100_marlin.h``); nothing here computes on the CPU.
@@ -23,7 +26,8 @@ import torch
 from . import _ext
 
 __all__ = ["mul_2_4", "mul_2_4_epilogue", "ACTIVATIONS", "scratch_bytes", "device_status",
-           "Layer_2_4", "replace_linear"]
+           "Layer_2_4", "replace_linear", "kv4_cache", "kv4_schedule", "kv4_append", "kv4_read",
+           "kv4_attention", "kv4_workspace", "KV4Step", "KV4_FATES"]
 
 # fused-epilogue activations (SM100_MARLIN_ACT_* of the C header)
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
@@ -166,3 +170,5 @@ def device_status(dev: int = 0) -> int:
 
 
 from .layer import Layer_2_4, replace_linear  # noqa: E402  (needs mul_2_4 above)
+from .kv4 import (KV4_FATES, KV4Step, kv4_append, kv4_attention, kv4_cache, kv4_read,  # noqa: E402
+                  kv4_schedule, kv4_workspace)

@@ -58,6 +58,18 @@ SIGNATURES = {
     "sm100_marlin_ipc_get_handle": (_c_int, [_vp, _c_int, _vp]),
     "sm100_marlin_ipc_open": (_c_int, [_vp, _c_int, ctypes.POINTER(_vp)]),
     "sm100_marlin_ipc_close": (_c_int, [_vp, _c_int]),
+    "sm100_marlin_kv4_schedule": (_c_int, [_vp, _vp, _vp, _i64, _c_int, _c_int, _vp, _c_int, _vp,
+                                           _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _c_int,
+                                           _vp]),
+    "sm100_marlin_kv4_append": (_c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _c_int, _c_int,
+                                         _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _vp]),
+    "sm100_marlin_kv4_read": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int,
+                                       _vp, _vp, _c_int, _vp]),
+    "sm100_marlin_kv4_attention": (_c_int, [_vp, _i64, _i64, _vp, _c_int, _c_int, _c_int, _c_int,
+                                            _c_int, _vp, _i64, _c_int, _vp, _vp, _c_int, _c_int,
+                                            _c_int, _c_int, _c_int, ctypes.c_float, _vp, _vp,
+                                            _size, _c_int, _vp]),
+    "sm100_marlin_kv4_workspace_bytes": (_size, [_c_int]),
 }
 
 OK = 0

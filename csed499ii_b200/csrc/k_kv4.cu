@@ -1,0 +1,180 @@
+// C ABI and launches of the 4-bit paged key/value cache (kv4_*.cuh).
+#include <cuda_runtime.h>
+
+#include "../../include/sm100_marlin.h"
+#include "kv4_attention.cuh"
+#include "kv4_cache.cuh"
+#include "kv4_schedule.cuh"
+
+namespace sm100 {
+
+int cuda_fail(cudaError_t e);  // sm100_marlin.cu
+
+namespace {
+
+using namespace kv4;
+
+// Makes `dev` current for a launch; the caller's device comes back on scope exit.
+struct OnDevice {
+  int prev = -1;
+  cudaError_t error;
+  explicit OnDevice(int dev) : error(cudaGetDevice(&prev)) {
+    if (error == cudaSuccess && prev != dev) {
+      error = cudaSetDevice(dev);
+    } else {
+      prev = -1;
+    }
+  }
+  ~OnDevice() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? SM100_MARLIN_OK : cuda_fail(e);
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int check_cache(const void* cache, int pages, int heads, int page_size, int dim, int dtype) {
+  if (dim != 64 && dim != 128) return SM100_MARLIN_ERR_KERN_SHAPE;
+  if (dtype != SM100_MARLIN_FP16 && dtype != SM100_MARLIN_BF16) return SM100_MARLIN_ERR_ARGUMENT;
+  if (pages < 0 || heads <= 0 || page_size <= 0 || page_size % kTile != 0)
+    return SM100_MARLIN_ERR_PROB_SHAPE;
+  if (static_cast<int64_t>(pages) * page_size > 0x7fffffffll) return SM100_MARLIN_ERR_PROB_SHAPE;
+  if (!cache && pages > 0) return SM100_MARLIN_ERR_ARGUMENT;
+  return aligned(cache, 16) ? SM100_MARLIN_OK : SM100_MARLIN_ERR_ALIGNMENT;
+}
+
+// f(T{}, std::integral_constant-like D) for the cache's type and head size.
+template <int D>
+struct Dim {
+  static constexpr int value = D;
+};
+template <class F>
+int dispatch(int dtype, int dim, F&& f) {
+  if (dtype == SM100_MARLIN_FP16) return dim == 64 ? f(Half{}, Dim<64>{}) : f(Half{}, Dim<128>{});
+  return dim == 64 ? f(Bf16{}, Dim<64>{}) : f(Bf16{}, Dim<128>{});
+}
+
+}  // namespace
+}  // namespace sm100
+
+using namespace sm100;
+using namespace sm100::kv4;
+
+extern "C" {
+
+int sm100_marlin_kv4_schedule(const int* new_lens, const int* lens, int* block_tables,
+                              int64_t table_stride, int width, int batch, int* free_pages,
+                              int capacity, const int* free_count, int rows, int page_size,
+                              int* lens_out, int* free_count_out, int* starts, int* slots,
+                              int* positions, int* fate, int dev, void* stream) {
+  if (batch < 0 || batch > kMaxBatch || rows < 0 || width < 0 || capacity < 0 || page_size <= 0)
+    return SM100_MARLIN_ERR_PROB_SHAPE;
+  if (!free_count || !free_count_out || !starts || (batch > 0 && (!new_lens || !lens || !lens_out || !fate)) ||
+      (batch > 0 && width > 0 && !block_tables) || (capacity > 0 && !free_pages) ||
+      (rows > 0 && (!slots || !positions)))
+    return SM100_MARLIN_ERR_ARGUMENT;
+  OnDevice on(dev);
+  if (on.error != cudaSuccess) return cuda_fail(on.error);
+  const ScheduleParams p{new_lens, lens, block_tables, table_stride, width, batch, free_pages,
+                         capacity, free_count, rows, page_size, lens_out, free_count_out, starts,
+                         slots, positions, fate};
+  const int smem = 20 * batch;
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        kv4_schedule_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 20 * kMaxBatch);
+    if (e != cudaSuccess) return cuda_fail(e);
+  }
+  // One CTA where the lengths or the count are updated in place: the others
+  // would read them while it writes.
+  const bool in_place = lens_out == lens || free_count_out == free_count;
+  const int ctas = in_place ? 1 : 1 + (rows > batch ? rows : batch) / 2048;
+  kv4_schedule_kernel<<<ctas < 148 ? ctas : 148, kScheduleThreads, smem,
+                        static_cast<cudaStream_t>(stream)>>>(p);
+  return launched();
+}
+
+int sm100_marlin_kv4_append(const void* k, int64_t k_row, int64_t k_head, const void* v,
+                            int64_t v_row, int64_t v_head, void* cache, int pages, int kv_heads,
+                            int page_size, int head_dim, int dtype, const int* slots, int tokens,
+                            int dev, void* stream) {
+  const int bad = check_cache(cache, pages, kv_heads, page_size, head_dim, dtype);
+  if (bad) return bad;
+  if (tokens < 0) return SM100_MARLIN_ERR_PROB_SHAPE;
+  if (tokens == 0) return SM100_MARLIN_OK;
+  if (!k || !v || !slots) return SM100_MARLIN_ERR_ARGUMENT;
+  if (!aligned(k, 2) || !aligned(v, 2)) return SM100_MARLIN_ERR_ALIGNMENT;
+  OnDevice on(dev);
+  if (on.error != cudaSuccess) return cuda_fail(on.error);
+  const bool vector = aligned(k, 16) && aligned(v, 16) && ((k_row | k_head | v_row | v_head) & 7) == 0;
+  const AppendParams p{{static_cast<uint8_t*>(cache), pages, kv_heads, page_size},
+                       static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_row, k_head,
+                       v_row, v_head, slots, tokens, vector};
+  const int64_t threads = 2ll * tokens * kv_heads * (head_dim / 8);
+  return dispatch(dtype, head_dim, [&](auto type, auto dim) {
+    kv4_append_kernel<decltype(type), decltype(dim)::value>
+        <<<static_cast<unsigned>((threads + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return launched();
+  });
+}
+
+int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_size, int head_dim,
+                          int dtype, const int* slots, int tokens, void* k, void* v, int dev,
+                          void* stream) {
+  const int bad = check_cache(cache, pages, kv_heads, page_size, head_dim, dtype);
+  if (bad) return bad;
+  if (tokens < 0) return SM100_MARLIN_ERR_PROB_SHAPE;
+  if (tokens == 0) return SM100_MARLIN_OK;
+  if (!k || !v || !slots) return SM100_MARLIN_ERR_ARGUMENT;
+  if (!aligned(k, 16) || !aligned(v, 16)) return SM100_MARLIN_ERR_ALIGNMENT;
+  OnDevice on(dev);
+  if (on.error != cudaSuccess) return cuda_fail(on.error);
+  const ReadParams p{{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, kv_heads, page_size},
+                     static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), slots, tokens};
+  const int64_t threads = 2ll * tokens * kv_heads * (head_dim / 8);
+  return dispatch(dtype, head_dim, [&](auto type, auto dim) {
+    kv4_read_kernel<decltype(type), decltype(dim)::value>
+        <<<static_cast<unsigned>((threads + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return launched();
+  });
+}
+
+int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, const void* cache,
+                               int pages, int kv_heads, int page_size, int head_dim, int dtype,
+                               const int* block_tables, int64_t table_stride, int width,
+                               const int* lens, const int* starts, int batch, int rows, int q_heads,
+                               int max_new, int window, float scale, void* out, void* workspace,
+                               size_t workspace_bytes, int dev, void* stream) {
+  const int bad = check_cache(cache, pages, kv_heads, page_size, head_dim, dtype);
+  if (bad) return bad;
+  if (batch < 0 || rows < 0 || width < 0 || q_heads <= 0 || q_heads % kv_heads != 0 || max_new < 0 ||
+      (!starts && rows != batch))
+    return SM100_MARLIN_ERR_PROB_SHAPE;
+  if (window < 0) return SM100_MARLIN_ERR_ARGUMENT;
+  if (rows == 0) return SM100_MARLIN_OK;
+  if (!q || !out || (batch > 0 && (!lens || (width > 0 && !block_tables)))) return SM100_MARLIN_ERR_ARGUMENT;
+  if (!aligned(q, 2) || !aligned(out, 16)) return SM100_MARLIN_ERR_ALIGNMENT;
+  OnDevice on(dev);
+  if (on.error != cudaSuccess) return cuda_fail(on.error);
+  const AttentionParams p{{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, kv_heads, page_size},
+                          static_cast<const uint8_t*>(q), q_row, q_head, static_cast<uint8_t*>(out),
+                          block_tables, table_stride, width, lens, starts, batch, rows, q_heads,
+                          q_heads / kv_heads, window, scale};
+  (void)workspace;
+  (void)workspace_bytes;
+  return dispatch(dtype, head_dim, [&](auto type, auto dim) {
+    kv4_attention_kernel<decltype(type), decltype(dim)::value>
+        <<<dim3(rows, q_heads), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return launched();
+  });
+}
+
+size_t sm100_marlin_kv4_workspace_bytes(int dev) {
+  (void)dev;
+  return 0;
+}
+
+}  // extern "C"

@@ -306,6 +306,100 @@ int sm100_marlin_set_decode_kernel(int which);
  * No counterpart in the reference (its profiling is external, via ncu). */
 int sm100_marlin_set_trace_buffer(void* buf);
 
+/*
+ * The 4-bit paged key/value cache.  No counterpart in the reference, which
+ * ends at the linear layers: it is what a server of W4A16 layers streams next
+ * to them.  One cache tensor per layer:
+ *
+ *   cache   [pages][kv_heads][page_size / 16] tiles of 16 tokens, 16-byte
+ *           aligned, contiguous; a tile is 16 * head_dim + 128 bytes: key
+ *           codes (16 rows of head_dim / 2 bytes, channel 2i in the low half
+ *           of byte i), value codes ([2][8][8][head_dim / 16] bytes: half of
+ *           the tile, eighth of the row, token in the half, byte), then 16
+ *           pairs (scale, offset) of the keys and 16 of the values in the
+ *           model's type.
+ *
+ * A row x of one token and head is held as offset = min x, scale =
+ * (max x - min x) / 15 rounded to the model's type and codes
+ * rint((x - offset) / scale), 0..15, in binary32; a row with an infinity or a
+ * NaN stands for NaN.  head_dim is 64 or 128 (else SM100_MARLIN_ERR_KERN_SHAPE),
+ * page_size a multiple of 16, dtype one of the two below, and pages * page_size
+ * at most 2^31 - 1.  A slot is page * page_size + place.
+ */
+#define SM100_MARLIN_FP16 0
+#define SM100_MARLIN_BF16 1
+
+/* What became of a request (kv4_schedule's `fate`). */
+#define SM100_MARLIN_KV4_OK 0
+#define SM100_MARLIN_KV4_NO_PAGES 1 /* the free pages were not enough */
+#define SM100_MARLIN_KV4_TABLE 2    /* it would outgrow its row of the table */
+#define SM100_MARLIN_KV4_ROWS 3     /* its tokens do not fit the step's rows */
+
+/*
+ * One step's block tables and slots, in one launch and without a copy to the
+ * host.  `new_lens[b]` tokens are added to request b, which has `lens[b]` in
+ * the cache; a negative entry ends the request: its pages go back, before any
+ * are handed out.  free_pages[0, *free_count) is a stack of free page ids;
+ * requests take what they need from its top in order.  A request that cannot
+ * be served is refused whole (see `fate`): its length stays and its rows get
+ * slot -1.  Once the pages do not reach, every later request that needs one is
+ * refused too.  Writes
+ *   block_tables   the new entries of requests that grow
+ *   free_pages     the pages given back, from entry *free_count on
+ *   lens_out, free_count_out   after the step (may be lens and free_count)
+ *   starts         [batch + 1] first row of each request (of all, refused too)
+ *   slots, positions   [rows]; past the last request's rows -1 and 0
+ *   fate           [batch], SM100_MARLIN_KV4_*
+ * batch is at most 8192.
+ */
+int sm100_marlin_kv4_schedule(const int* new_lens, const int* lens, int* block_tables,
+                              int64_t table_stride, int width, int batch, int* free_pages,
+                              int capacity, const int* free_count, int rows, int page_size,
+                              int* lens_out, int* free_count_out, int* starts, int* slots,
+                              int* positions, int* fate, int dev, void* stream);
+
+/* Quantises the rows of k and v (element (token, head, c) at token * *_row +
+ * head * *_head + c, 16-bit aligned) into the cache at `slots[token]`; rows
+ * whose slot is outside the cache are skipped.  Two rows of one call must not
+ * have the same slot. */
+int sm100_marlin_kv4_append(const void* k, int64_t k_row, int64_t k_head, const void* v,
+                            int64_t v_row, int64_t v_head, void* cache, int pages, int kv_heads,
+                            int page_size, int head_dim, int dtype, const int* slots, int tokens,
+                            int dev, void* stream);
+
+/* Reads the values at `slots` back into k and v, [tokens][kv_heads][head_dim]
+ * (16-byte aligned): code * scale + offset, rounded to the model's type; zeros
+ * where the slot is outside the cache. */
+int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_size, int head_dim,
+                          int dtype, const int* slots, int tokens, void* k, void* v, int dev,
+                          void* stream);
+
+/*
+ * out[row, h] = softmax over keys j of (scale * q[row, h] . k[j, h / G]) times
+ * v[j, h / G], G = q_heads / kv_heads.  Request b's rows are [starts[b],
+ * starts[b + 1]) (starts NULL: row b alone, and rows == batch) and are the
+ * last tokens of the lens[b] that it has in the cache: row i of n sees keys up
+ * to its own position lens[b] - n + i and, with window > 0, only the last
+ * `window` of those.  A row that sees nothing, and rows past the last request,
+ * get zeros; entries of the table outside the cache are keys that nobody sees.
+ *   q          element (row, head, c) at row * q_row + head * q_head + c
+ *   out        [rows][q_heads][head_dim], 16-byte aligned
+ *   max_new    no request has more rows than this (it picks the kernel: not
+ *              more work, and no result, hangs on how close it is)
+ *   workspace  sm100_marlin_kv4_workspace_bytes(dev) bytes, 16-byte aligned,
+ *              all zero on entry and left so; calls that may overlap need
+ *              their own
+ */
+int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, const void* cache,
+                               int pages, int kv_heads, int page_size, int head_dim, int dtype,
+                               const int* block_tables, int64_t table_stride, int width,
+                               const int* lens, const int* starts, int batch, int rows, int q_heads,
+                               int max_new, int window, float scale, void* out, void* workspace,
+                               size_t workspace_bytes, int dev, void* stream);
+
+/* Bytes of kv4_attention's workspace on a device. */
+size_t sm100_marlin_kv4_workspace_bytes(int dev);
+
 #ifdef __cplusplus
 }
 #endif
