@@ -1,14 +1,20 @@
 // C ABI and launches of the 4-bit paged key/value cache (kv4_*.cuh).
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/sm100_marlin.h"
 #include "kv4_attention.cuh"
 #include "kv4_cache.cuh"
+#include "kv4_decode.cuh"
 #include "kv4_schedule.cuh"
 
 namespace sm100 {
 
-int cuda_fail(cudaError_t e);  // sm100_marlin.cu
+// sm100_marlin.cu
+int cuda_fail(cudaError_t e);
+int kernel_status(int dev, int** out);  // device address of the status word
+int sm_count(int dev, int* sms);
 
 namespace {
 
@@ -45,6 +51,50 @@ int check_cache(const void* cache, int pages, int heads, int page_size, int dim,
   if (static_cast<int64_t>(pages) * page_size > 0x7fffffffll) return SM100_MARLIN_ERR_PROB_SHAPE;
   if (!cache && pages > 0) return SM100_MARLIN_ERR_ARGUMENT;
   return aligned(cache, 16) ? SM100_MARLIN_OK : SM100_MARLIN_ERR_ALIGNMENT;
+}
+
+// The opt-in to more than 48 KB of shared memory, once per kernel and device.
+template <auto Kernel>
+int allow_smem(int dev, int bytes) {
+  static std::atomic<uint64_t> done{0};
+  if (dev >= 0 && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return SM100_MARLIN_OK;
+  const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_fail(e);
+  if (dev >= 0 && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return SM100_MARLIN_OK;
+}
+
+// Requests with at most this many query rows for a key/value head go to the
+// decode kernel, others to the prompt kernel.
+constexpr int kFewRows = 32;
+
+// Counters of the decode kernel's grid, then its parts.
+constexpr size_t kCounterBytes = 4096;
+size_t workspace_bytes(int sms) {
+  return kCounterBytes + static_cast<size_t>(sms) * 2 * DecodeCfg<128, 2>::kPart * 2 * sizeof(float);
+}
+
+template <class T, int D, int NT>
+int launch_decode(DecodeParams p, int sms, int dev, cudaStream_t stream) {
+  using Cfg = DecodeCfg<D, NT>;
+  static_assert(Cfg::kCtas * Cfg::kPart <= 2 * DecodeCfg<128, 2>::kPart, "workspace");
+  const int bad = allow_smem<kv4_decode_kernel<T, D, NT>>(dev, Cfg::kSmem);
+  if (bad) return bad;
+  // The kernel keeps a sum per request in shared memory: larger batches go in slices.
+  const int batch = p.batch;
+  int done = 0;
+  do {
+    const int n = batch - done < kDecodeBatch ? batch - done : kDecodeBatch;
+    p.batch = n;
+    p.pad = done + n == batch;
+    kv4_decode_kernel<T, D, NT><<<sms * Cfg::kCtas, 256, Cfg::kSmem, stream>>>(p);
+    p.lens += n;
+    p.tables += n * p.table_stride;
+    p.row0 += n;
+    if (p.starts) p.starts += n;
+    done += n;
+  } while (done < batch);
+  return launched();
 }
 
 // f(T{}, std::integral_constant-like D) for the cache's type and head size.
@@ -159,22 +209,39 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
   if (!aligned(q, 2) || !aligned(out, 16)) return SM100_MARLIN_ERR_ALIGNMENT;
   OnDevice on(dev);
   if (on.error != cudaSuccess) return cuda_fail(on.error);
-  const AttentionParams p{{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, kv_heads, page_size},
-                          static_cast<const uint8_t*>(q), q_row, q_head, static_cast<uint8_t*>(out),
-                          block_tables, table_stride, width, lens, starts, batch, rows, q_heads,
-                          q_heads / kv_heads, window, scale};
-  (void)workspace;
-  (void)workspace_bytes;
+  int sms = 0;
+  int* status = nullptr;
+  const int failed = sm_count(dev, &sms) | kernel_status(dev, &status);
+  if (failed) return failed;
+  if (!workspace || workspace_bytes < sm100::workspace_bytes(sms)) return SM100_MARLIN_ERR_SCRATCH;
+  if (!aligned(workspace, 16)) return SM100_MARLIN_ERR_ALIGNMENT;
+  const Cache c{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, kv_heads, page_size};
+  const int group = q_heads / kv_heads;
+  const bool vector = aligned(q, 16) && ((q_row | q_head) & 7) == 0;
+  const int64_t most = static_cast<int64_t>(starts ? max_new : 1) * group;
+  const DecodeParams few{c, static_cast<const uint8_t*>(q), q_row, q_head, vector,
+                         static_cast<uint8_t*>(out), block_tables, table_stride, width, lens, starts,
+                         0, batch, rows, 1, q_heads, group, window, kFewRows, scale,
+                         static_cast<int*>(workspace),
+                         reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status};
+  const AttentionParams many{c, static_cast<const uint8_t*>(q), q_row, q_head, static_cast<uint8_t*>(out),
+                             block_tables, table_stride, width, lens, starts, batch, rows, q_heads,
+                             group, window, scale, kFewRows};
+  const cudaStream_t on_stream = static_cast<cudaStream_t>(stream);
   return dispatch(dtype, head_dim, [&](auto type, auto dim) {
-    kv4_attention_kernel<decltype(type), decltype(dim)::value>
-        <<<dim3(rows, q_heads), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    using T = decltype(type);
+    constexpr int D = decltype(dim)::value;
+    const int bad = most <= 8 ? launch_decode<T, D, 1>(few, sms, dev, on_stream)
+                              : launch_decode<T, D, 2>(few, sms, dev, on_stream);
+    if (bad || most <= kFewRows) return bad;
+    kv4_attention_kernel<T, D><<<dim3(rows, q_heads), 128, 0, on_stream>>>(many);
     return launched();
   });
 }
 
 size_t sm100_marlin_kv4_workspace_bytes(int dev) {
-  (void)dev;
-  return 0;
+  int sms = 0;
+  return sm_count(dev, &sms) ? 0 : workspace_bytes(sms);
 }
 
 }  // extern "C"

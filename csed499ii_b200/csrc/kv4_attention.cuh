@@ -29,6 +29,7 @@ struct AttentionParams {
   int group;             // query heads per key/value head
   int window;            // 0: none
   float scale;
+  int most;              // requests with at most this many query rows a group are left alone
 };
 
 // First index whose (ascending) entry is above `x`; n if there is none.
@@ -61,6 +62,7 @@ __global__ void __launch_bounds__(128) kv4_attention_kernel(const __grid_constan
     first = b < p.batch ? p.starts[b] : row;
     end = b < p.batch ? p.starts[b + 1] : row;
   }
+  if (b >= p.batch || static_cast<int64_t>(end - first) * p.group <= p.most) return;
   const int64_t room = static_cast<int64_t>(p.width) * p.cache.page_size;
   const int len = b < p.batch ? static_cast<int>(min(static_cast<int64_t>(p.lens[b]), room)) : 0;
   const int position = len - (end - row);  // of this row

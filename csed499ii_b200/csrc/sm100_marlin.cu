@@ -202,6 +202,13 @@ int device_status_ptr(int dev, int** out) {
   return SM100_MARLIN_OK;
 }
 
+}  // namespace
+
+int kernel_status(int dev, int** out) { return device_status_ptr(dev, out); }
+int sm_count(int dev, int* sms) { return device_sms(dev, sms); }
+
+namespace {
+
 // Column-tile width (in 64-column chunks).  Wider tiles re-read the
 // activations less often, but when there are fewer tiles than CTAs some CTA
 // works entirely inside one tile and finishes at the same time as the CTA

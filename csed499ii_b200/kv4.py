@@ -289,6 +289,9 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
         0 if starts is None else starts.data_ptr(), batch, rows, q_heads, max_new, window,
         1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), workspace.data_ptr(),
         4 * workspace.numel(), dev, stream)
+    if err == _ext.ERR_SCRATCH:
+        need = _ext.load().sm100_marlin_kv4_workspace_bytes(dev) // 4
+        raise RuntimeError(f"workspace must be of size at least {need}.")
     if err:
         _raise("kv4_attention", err)
     return out
