@@ -4,9 +4,9 @@
 #include <atomic>
 
 #include "../../include/sm100_marlin.h"
-#include "kv4_attention.cuh"
 #include "kv4_cache.cuh"
 #include "kv4_decode.cuh"
+#include "kv4_prompt.cuh"
 #include "kv4_schedule.cuh"
 
 namespace sm100 {
@@ -94,6 +94,27 @@ int launch_decode(DecodeParams p, int sms, int dev, cudaStream_t stream) {
     if (p.starts) p.starts += n;
     done += n;
   } while (done < batch);
+  return launched();
+}
+
+template <class T, int D>
+int launch_prompt(PromptParams p, int dev, cudaStream_t stream) {
+  const int bad = allow_smem<kv4_prompt_kernel<T, D>>(dev, PromptCfg<D>::kSmem);
+  if (bad) return bad;
+  // No more items than full ones and one rest for each request that is served;
+  // CTAs without an item leave at once.
+  const int64_t rows = static_cast<int64_t>(p.rows) * p.group;
+  for (int done = 0, batch = p.batch; done < batch; done += kPromptBatch) {
+    p.batch = batch - done < kPromptBatch ? batch - done : kPromptBatch;
+    const int64_t rests = rows / (p.most + 1);
+    const int64_t items = rows / 256 + (rests < p.batch ? rests : p.batch);
+    if (items > 0)
+      kv4_prompt_kernel<T, D><<<dim3(static_cast<unsigned>(items), p.cache.heads), kPromptThreads,
+                                PromptCfg<D>::kSmem, stream>>>(p);
+    p.lens += p.batch;
+    p.tables += p.batch * p.table_stride;
+    p.starts += p.batch;
+  }
   return launched();
 }
 
@@ -218,24 +239,23 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
   const Cache c{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, kv_heads, page_size};
   const int group = q_heads / kv_heads;
   const bool vector = aligned(q, 16) && ((q_row | q_head) & 7) == 0;
+  const int few_rows = group > kFewRows ? group : kFewRows;  // a single token is always few
   const int64_t most = static_cast<int64_t>(starts ? max_new : 1) * group;
   const DecodeParams few{c, static_cast<const uint8_t*>(q), q_row, q_head, vector,
                          static_cast<uint8_t*>(out), block_tables, table_stride, width, lens, starts,
-                         0, batch, rows, 1, q_heads, group, window, kFewRows, scale,
+                         0, batch, rows, 1, q_heads, group, window, few_rows, scale,
                          static_cast<int*>(workspace),
                          reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status};
-  const AttentionParams many{c, static_cast<const uint8_t*>(q), q_row, q_head, static_cast<uint8_t*>(out),
-                             block_tables, table_stride, width, lens, starts, batch, rows, q_heads,
-                             group, window, scale, kFewRows};
+  const PromptParams many{c, static_cast<const uint8_t*>(q), q_row, q_head, vector, static_cast<uint8_t*>(out),
+                          block_tables, table_stride, width, lens, starts, batch, rows, q_heads,
+                          group, window, few_rows, scale, status};
   const cudaStream_t on_stream = static_cast<cudaStream_t>(stream);
   return dispatch(dtype, head_dim, [&](auto type, auto dim) {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value;
     const int bad = most <= 8 ? launch_decode<T, D, 1>(few, sms, dev, on_stream)
                               : launch_decode<T, D, 2>(few, sms, dev, on_stream);
-    if (bad || most <= kFewRows) return bad;
-    kv4_attention_kernel<T, D><<<dim3(rows, q_heads), 128, 0, on_stream>>>(many);
-    return launched();
+    return bad || most <= few_rows ? bad : launch_prompt<T, D>(many, dev, on_stream);
   });
 }
 

@@ -10,10 +10,13 @@
 //
 // Codes 0..15 are exact in 16 bits and scale and offset stay in 32 bits
 // outside the products, so nothing is dequantised and nothing is rounded but
-// the weights w = p s.  Their rounding error would be multiplied by codes that
-// are all positive; the exact correction 8 (w - rounded w) in the offset term
-// makes them act as if centred on 8, which is what rounding a weight of a
-// dequantised value costs.
+// the weights w = p s (to half, whatever the model's type).  The exponential
+// gives w itself, its argument is the score plus log2 s, and the running
+// maximum is that of these arguments: a half then holds the weights that
+// matter whatever sizes the values have, and p is w / s in 32 bits.  The
+// rounding errors would be multiplied by codes that are all positive; the exact
+// correction 8 (w - rounded w) in the offset term makes them act as if centred
+// on 8, which is what rounding a weight of a dequantised value costs.
 //
 // mma.m16n8k16 takes 16 tokens (scores) or 16 channels (result) as its rows
 // and 8 query rows as its columns; the 8 query heads of a group fill it.  Codes
@@ -201,6 +204,25 @@ __device__ __forceinline__ uint32_t key_odd(uint32_t w) {
   return BF16 ? lop3<kLutAndOr>(w >> 4, 0x000f000fu, 0x43004300u) : w & 0x00f000f0u;
 }
 
+// log2 e: scores are kept as exponents of two.
+constexpr float kLog2e = 1.4426950408889634f;
+
+// What the weights need to know of a row of values: its scale's logarithm and
+// reciprocal, and its value at code 8 over the scale.  A row without a scale
+// has all codes 0, so any scale tells the same values; a small one rounds its
+// weights where nothing shows.
+struct ValueRow {
+  float log_s, inv_s, at_8;
+};
+__device__ __forceinline__ ValueRow value_row(float2 pair) {
+  const float s = pair.x > 0x1p-60f ? pair.x : fmaxf(fabsf(pair.y) * 0x1p-10f, 0x1p-60f);
+  ValueRow r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r.log_s) : "f"(s));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inv_s) : "f"(s));
+  r.at_8 = fmaf(pair.y, r.inv_s, 8.f);
+  return r;
+}
+
 // A part of an item, or all of it: results (already divided by the sum), the
 // running maximum of the scores (times log2 e) and the sum of the weights.
 struct Segment {
@@ -322,8 +344,7 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
     int place[NT][2];                               // positions of this lane's two rows
     float acc[NT][D / 16][4];
     float top[NT][2], l[NT][2], a1[NT][2], a2[NT][2];
-    uint32_t exponent = 1;  // of the largest value scale so far: weights are kept relative to it
-    const float c2 = p.scale * 1.4426950408889634f;
+    const float c2 = p.scale * kLog2e;
     const float c1 = kBf ? c2 : c2 * 16777216.f;
     bool fresh = true;
     int64_t item_begin = 0, item_end = 0;
@@ -333,7 +354,6 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
         fresh = false;
         item_begin = begin + i - (at.tile - at.s.tile0);
         item_end = item_begin + at.s.tiles;
-        exponent = 1;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int r = at.chunk * kRows + nt * 8 + g;
@@ -400,8 +420,9 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
           k1[0] = y.x, k1[1] = y.y;
         }
         const float2 kp0 = T::up(lds32(tile + off_k_pair(D, g))), kp1 = T::up(lds32(tile + off_k_pair(D, g + 8)));
-        const float2 vp0 = T::up(lds32(tile + off_v_pair(D, g))), vp1 = T::up(lds32(tile + off_v_pair(D, g + 8)));
-        float x[NT][4];
+        const ValueRow v0 = value_row(T::up(lds32(tile + off_v_pair(D, g))));
+        const ValueRow v1 = value_row(T::up(lds32(tile + off_v_pair(D, g + 8))));
+        float x[NT][4];  // arguments of the weights
         {
           float e[NT][4] = {}, o[NT][4] = {};
 #pragma unroll
@@ -425,7 +446,8 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const float dot = fmaf(o[nt][c], kBf ? 1.f : 0.0625f, e[nt][c]);
-              x[nt][c] = fmaf(c < 2 ? s0 : s1, dot, (c < 2 ? z0 : z1) * sumq[nt][c & 1]);
+              x[nt][c] = fmaf(c < 2 ? s0 : s1, dot,
+                              fmaf(c < 2 ? z0 : z1, sumq[nt][c & 1], c < 2 ? v0.log_s : v1.log_s));
             }
         }
         // what of the tile each row sees; most tiles are seen whole
@@ -433,11 +455,7 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
         const bool whole = j0 + kTile <= at.s.len - at.s.n + 1 &&
                            (p.window == 0 || j0 >= at.s.len - p.window);
         bool seen[NT][4];
-        uint32_t sb = max(__float_as_uint(vp0.x) < 0x7f800000u ? __float_as_uint(vp0.x) : 0u,
-                          __float_as_uint(vp1.x) < 0x7f800000u ? __float_as_uint(vp1.x) : 0u);
         if (!whole) {
-          sb = max(j0 + g < at.s.len && __float_as_uint(vp0.x) < 0x7f800000u ? __float_as_uint(vp0.x) : 0u,
-                   j0 + g + 8 < at.s.len && __float_as_uint(vp1.x) < 0x7f800000u ? __float_as_uint(vp1.x) : 0u);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -448,17 +466,14 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
               if (!seen[nt][c]) x[nt][c] = -CUDART_INF_F;
             }
         }
-        // The maximum moves only where a score passes it by more than 8 (a
+        // The maximum moves only where an argument passes it by more than 8 (a
         // factor of 256, harmless in the sums), so most tiles need no exchange.
-        bool moves = (sb >> 23) > exponent;
+        bool moves = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 4; ++c) moves |= x[nt][c] > top[nt][c & 1] + 8.f;
         if (__any_sync(0xffffffffu, moves)) {
-          const uint32_t ex = max(exponent, __reduce_max_sync(0xffffffffu, sb) >> 23);
-          const float shift = ex - exponent > 126u ? 0.f : __uint_as_float((127u - (ex - exponent)) << 23);
-          exponent = ex;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float f[2];
@@ -472,7 +487,6 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
               top[nt][c] = m;
               l[nt][c] *= f[c];
               a1[nt][c] *= f[c];
-              f[c] *= shift;
               a2[nt][c] *= f[c];
             }
 #pragma unroll
@@ -485,21 +499,17 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
           }
         }
         // weights, and their sums
-        const float unit = __uint_as_float((254u - exponent) << 23);
-        const float ws0 = vp0.x * unit, ws1 = vp1.x * unit;
-        const float vz0 = fmaf(vp0.x, 8.f, vp0.y), vz1 = fmaf(vp1.x, 8.f, vp1.y);
         uint32_t wb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float w[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float e = exp2_approx(x[nt][c] - top[nt][c & 1]);
-            w[c] = e * (c < 2 ? ws0 : ws1);
-            float z = e * (c < 2 ? vz0 : vz1);
-            if (!whole && !seen[nt][c]) w[c] = z = 0.f;  // whatever lies there
-            l[nt][c & 1] += e;
-            a1[nt][c & 1] += z;
+            w[c] = exp2_approx(x[nt][c] - top[nt][c & 1]);
+            // where nothing is seen, scale and offset may be anything
+            const bool none = !whole && !seen[nt][c];
+            l[nt][c & 1] = fmaf(w[c], none ? 0.f : c < 2 ? v0.inv_s : v1.inv_s, l[nt][c & 1]);
+            a1[nt][c & 1] = fmaf(w[c], none ? 0.f : c < 2 ? v0.at_8 : v1.at_8, a1[nt][c & 1]);
           }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -550,7 +560,6 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
       const bool is_head = !all && ends && item_begin < begin && i + 1 < count;
       float* part = is_head ? reinterpret_cast<float*>(smem + Cfg::kOffParts) + warp * kPart
                             : reinterpret_cast<float*>(smem + warp * kDepth * kBytes);
-      const float big = __uint_as_float(exponent << 23);
       if (!all && lane == 0)
         segments[2 * warp + (is_head ? 0 : 1)] = {item_begin, item_end, here.b, here.head, here.chunk};
 #pragma unroll
@@ -568,8 +577,8 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
           float y[D / 8];
 #pragma unroll
           for (int x = 0; x < D / 16; ++x) {
-            y[2 * x] = (big * fmaf(acc[nt][x][c], 16777216.f, -8.f * a2[nt][c]) + a1[nt][c]) * over;
-            y[2 * x + 1] = (big * fmaf(acc[nt][x][c + 2], 1048576.f, -8.f * a2[nt][c]) + a1[nt][c]) * over;
+            y[2 * x] = (fmaf(acc[nt][x][c], 16777216.f, -8.f * a2[nt][c]) + a1[nt][c]) * over;
+            y[2 * x + 1] = (fmaf(acc[nt][x][c + 2], 1048576.f, -8.f * a2[nt][c]) + a1[nt][c]) * over;
           }
           const int r = nt * 8 + 2 * t + c, row = here.chunk * kRows + r;
           if (row >= here.s.n * p.group) continue;

@@ -1,0 +1,625 @@
+// Attention over the 4-bit cache for requests with many query rows (prompts,
+// pieces of prompts), on tcgen05.
+//
+// 4 * D operations per visible (query, key) pair and head bound it.  A CTA
+// takes 256 query rows of one key/value head (rows are (token, head of the
+// group) pairs, so all heads of a group share what is read) as two tiles of
+// 128, and walks over the keys in steps of 128:
+//
+//   S = Q (C_k - 8)^T     tcgen05.mma, Q and the codes in shared memory
+//   P                     in the softmax warps' registers, back to tensor
+//                         memory in the place of S
+//   O += P (C_v - 8)      tcgen05.mma, P from tensor memory
+//
+// As in the decode kernel the operands are codes, exact in 16 bits, and the
+// rows' scales and offsets stay in 32 bits: a score is s_k S + z_k sum(q) with
+// z = offset + 8 scale, the exponential gives the weight w = p s_v that goes
+// back, and sum(p) = sum(w / s_v) and sum(p z_v) = sum(w z_v / s_v), one number
+// a row, join the result at the end.  That costs the softmax warps three more
+// multiply-adds a pair than plain attention, in two-wide f32x2 instructions,
+// and saves every rounding but the weights'.
+//
+// Four warps turn codes into operand tiles (two stages of each), one thread
+// issues the products, and four warps per query tile do the softmax, one row a
+// thread.  While one query tile is in its softmax the other one's products
+// run.  The running maximum is only moved when an argument passes it by more than
+// 8 (a factor of 256): then the step's weights are made again and the
+// accumulator in tensor memory is scaled, which is rare after the first steps.
+#pragma once
+
+#include <math_constants.h>
+
+#include "kv4_decode.cuh"
+#include "marlin24_prefill.cuh"
+
+namespace sm100 {
+namespace kv4 {
+
+constexpr int kPromptBatch = 8192;  // requests of a launch
+constexpr int kPromptThreads = 13 * 32;
+constexpr int kStep = 128;          // keys of a step
+
+struct PromptParams {
+  Cache cache;
+  const uint8_t* q;      // element (row, head, c) at q_row * row + q_head * head + c
+  int64_t q_row, q_head;
+  int q_aligned;         // 1: every row of q starts on a 16-byte boundary
+  uint8_t* out;          // [rows][q_heads][D]
+  const int* tables;     // [batch][table_stride], `width` entries used
+  int64_t table_stride;
+  int width;
+  const int* lens;       // tokens of each request in the cache, the step's own among them
+  const int* starts;     // [batch + 1] first row of each request
+  int batch;
+  int rows;              // of q
+  int q_heads;
+  int group;             // query heads per key/value head
+  int window;            // 0: none
+  int most;              // requests with at most this many query rows a group are left alone
+  float scale;
+  int* status;
+};
+
+template <int D>
+struct PromptCfg {
+  static constexpr int kQ = 128 * D * 2;       // a query tile
+  static constexpr int kK = kStep * D * 2;     // a key or value tile
+  static constexpr int kOffK = 2 * kQ;         // two stages
+  static constexpr int kOffV = kOffK + 2 * kK; // two stages
+  static constexpr int kOffPairs = kOffV + 2 * kK;     // [4] Constants
+  static constexpr int kOffMisc = kOffPairs + 4 * 64 * 40;
+  static constexpr int kSmem = kOffMisc + 1024 + 1024;  // and room to align
+  static constexpr uint32_t kColS = 0, kColO = 256, kCols = 512;
+};
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+      "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Two floats in one register pair, for the two-wide instructions.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(F2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Eight codes (nibbles 0..7 of `w`) less 8 as 16-bit numbers, in the order
+// 0, 4, 1, 5, 2, 6, 3, 7.
+template <bool BF16>
+__device__ __forceinline__ uint4 centred(uint32_t w) {
+  uint4 r;
+  if constexpr (BF16) {
+    const uint32_t k136 = 0x43084308u;  // 128 + 8 twice
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t y = lop3<kLutAndOr>(w >> (4 * i), 0x000f000fu, 0x43004300u);
+      const __nv_bfloat162 z = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&k136));
+      x[i] = *reinterpret_cast<const uint32_t*>(&z);
+    }
+    r = make_uint4(x[0], x[1], x[2], x[3]);
+  } else {
+    half2 a, b, c, d;
+    dequant_pair(w, a, b);
+    dequant_pair(w >> 8, c, d);
+    r = make_uint4(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b),
+                   *reinterpret_cast<uint32_t*>(&c), *reinterpret_cast<uint32_t*>(&d));
+  }
+  return r;
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
+// First index whose (ascending) entry is above `x`; n if there is none.
+__device__ __forceinline__ int first_above(const int* a, int n, int x) {
+  int lo = 0;
+  while (n > 0) {
+    const int half = n >> 1;
+    if (a[lo + half] <= x) {
+      lo += half + 1;
+      n -= half + 1;
+    } else {
+      n = half;
+    }
+  }
+  return lo;
+}
+
+// The rows of a request that this kernel serves, as 256-row items.
+__device__ __forceinline__ int prompt_items(const PromptParams& p, int b) {
+  const int first = min(max(p.starts[b], 0), p.rows);
+  const int64_t rows = static_cast<int64_t>(min(p.starts[b + 1], p.rows) - first) * p.group;
+  return rows > p.most ? static_cast<int>((rows + 255) / 256) : 0;
+}
+
+// What the softmax needs to know of a step's keys, two by two.
+struct Constants {
+  float4 key[kStep / 2];   // scales, values at code 8, both times scale * log2 e
+  float4 value[kStep / 2]; // ValueRow: log_s, inv_s
+  float2 at_8[kStep / 2];
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    kv4_prompt_kernel(const __grid_constant__ PromptParams p) {
+  using Cfg = PromptCfg<D>;
+  constexpr int kBytes = tile_bytes(D);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  Constants* constants = reinterpret_cast<Constants*>(smem + Cfg::kOffPairs);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffMisc);
+  const uint32_t bar = smem_addr(bars);
+  // barriers
+  const uint32_t q_ready = bar, k_full = bar + 8, k_empty = bar + 24, v_full = bar + 40,
+                 v_empty = bar + 56, s_full = bar + 72, p_ready = bar + 88, o_done = bar + 104,
+                 c_full = bar + 120 /* four */, finished = bar + 152;
+  uint64_t* tile_at = bars + 20;                                        // [4][8]
+  uint32_t* valid = reinterpret_cast<uint32_t*>(bars + 52);             // [4][4]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 68);
+  volatile int* drain_flag = abort_flag + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 69);
+  int* sums = reinterpret_cast<int*>(bars + 70);                        // [16]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int head = blockIdx.y;
+
+  // --- which rows -------------------------------------------------------------
+  int* pre = reinterpret_cast<int*>(smem);  // where the tiles will be
+  int total = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kPromptThreads) {
+    const int b = b0 + threadIdx.x;
+    int x = b < p.batch ? prompt_items(p, b) : 0;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, i);
+      if (lane >= i) x += y;
+    }
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    int all = 0;
+    for (int i = 0; i < 13; ++i) {
+      if (i == warp) x += all;
+      all += sums[i];
+    }
+    if (b < p.batch) pre[b] = total + x;
+    total += all;
+    __syncthreads();
+  }
+  // the last items first: within a request they have the most keys
+  const int item = total - 1 - static_cast<int>(blockIdx.x);
+  if (item < 0) return;
+  const int b = first_above(pre, p.batch, item);
+  const int tile = item - (b ? pre[b - 1] : 0);
+  const int first = min(max(p.starts[b], 0), p.rows), n = min(p.starts[b + 1], p.rows) - first;
+  const int64_t room = static_cast<int64_t>(p.width) * p.cache.page_size;
+  const int len = static_cast<int>(min(static_cast<int64_t>(p.lens[b]), room));
+  const int rows = min(256, n * p.group - tile * 256);
+  const int tiles_q = rows > 128 ? 2 : 1;
+  const int before = len - n;  // position of the request's row 0
+  const int lo_pos = before + tile * 256 / p.group, hi_pos = before + (tile * 256 + rows - 1) / p.group;
+  const int from = p.window ? max(0, lo_pos - p.window + 1) : 0;
+  const int to = min(len, hi_pos + 1);
+  const int step0 = from / kStep;
+  const int steps = to > from ? (to + kStep - 1) / kStep - step0 : 0;
+  __syncthreads();  // `pre` is read
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_ready, 4 * tiles_q);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + 8 * i, 4);
+      mbar_init(k_empty + 8 * i, 1);
+      mbar_init(v_full + 8 * i, 4);
+      mbar_init(v_empty + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_ready + 8 * i, 4);
+      mbar_init(o_done + 8 * i, 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(c_full + 8 * i, 4);
+    mbar_init(finished, 1);
+    *abort_flag = *drain_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) tmem_alloc(smem_addr(tmem_slot), Cfg::kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+  auto wait = [&](uint32_t at, int phase) {  // one thread
+    ok = ok && mbar_wait_bounded(at, phase & 1, abort_flag);
+    return ok;
+  };
+  auto wait_warp = [&](uint32_t at, int phase) {
+    ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(at, phase & 1, abort_flag));
+    return ok;
+  };
+
+  if (warp < 8) {
+    // ------------------------------------------------------------- softmax
+    const int qi = warp >> 2, row = (warp & 3) * 32 + lane;
+    if (qi < tiles_q) {
+      const int r = tile * 256 + qi * 128 + row;
+      const int token = r / p.group, h = head * p.group + r % p.group;
+      const bool live = qi * 128 + row < rows;
+      // this row of Q, its channels in the order that `centred` gives the codes
+      float sumq = 0.f;
+      {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) +
+                              p.q_row * (first + token) + p.q_head * h;
+        const uint32_t dst = smem_addr(smem) + qi * Cfg::kQ + row * 128;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (live) {
+            if (p.q_aligned) {
+              x = *reinterpret_cast<const uint4*>(src + 8 * c);
+            } else {
+              uint32_t y[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z)
+                y[z] = src[8 * c + 2 * z] | static_cast<uint32_t>(src[8 * c + 2 * z + 1]) << 16;
+              x = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          }
+          const float2 f0 = T::up(x.x), f1 = T::up(x.y), f2 = T::up(x.z), f3 = T::up(x.w);
+          sumq += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+          sts128(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4),
+                 make_uint4(prmt(x.x, x.z, 0x5410), prmt(x.x, x.z, 0x7632), prmt(x.y, x.w, 0x5410),
+                            prmt(x.y, x.w, 0x7632)));
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t s_at = tmem + lanes + Cfg::kColS + 128 * qi;
+      const uint32_t o_at = tmem + lanes + Cfg::kColO + D * qi;
+      const int pos = before + token;
+      const int tile_lo = before + (tile * 256 + qi * 128) / p.group;
+      const int tile_hi = before + (tile * 256 + min(rows, qi * 128 + 128) - 1) / p.group;
+      float top = kLowest, l = 0.f, off = 0.f;
+      for (int it = 0; it < steps; ++it) {
+        const int buf = it & 3;
+        if (!wait_warp(c_full + 8 * buf, it >> 2) || !wait_warp(s_full + 8 * qi, it)) break;
+        tc_fence_after();
+        const Constants& k = constants[buf];
+        const int j0 = (step0 + it) * kStep;
+        const bool whole = j0 + kStep <= tile_lo + 1 && (p.window == 0 || j0 > tile_hi - p.window) &&
+                           (valid[4 * buf] & valid[4 * buf + 1] & valid[4 * buf + 2] & valid[4 * buf + 3]) ==
+                               0xffffffffu;
+        uint32_t weights[64];
+        float lt, offt;
+        while (true) {
+          float mx = kLowest;
+          F2 l2 = 0, off2 = 0;
+          const F2 q2 = pack2(sumq, sumq), top2 = pack2(-top, -top);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tmem_ld32(s_at + 32 * c, s);
+            const uint32_t there = valid[4 * buf + c];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float4 ks = k.key[16 * c + i / 2], vs = k.value[16 * c + i / 2];
+              const float2 z = k.at_8[16 * c + i / 2];
+              F2 x = fma2(pack2(ks.x, ks.y), pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
+                          fma2(pack2(ks.z, ks.w), q2, pack2(vs.x, vs.y)));
+              if (!whole) {
+                float2 y = unpack2(x);
+                const int j = j0 + 32 * c + i;
+                const int oldest = p.window ? pos - p.window : -1;
+                if (j > pos || j <= oldest || !(there >> i & 1)) y.x = -CUDART_INF_F;
+                if (j + 1 > pos || j + 1 <= oldest || !(there >> (i + 1) & 1)) y.y = -CUDART_INF_F;
+                x = pack2(y.x, y.y);
+              }
+              const float2 xs = unpack2(x);
+              mx = fmaxf(mx, fmaxf(xs.x, xs.y));
+              const float2 y = unpack2(add2(x, top2));
+              const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+              const F2 w2 = pack2(w.x, w.y);
+              if (whole) {
+                l2 = fma2(w2, pack2(vs.z, vs.w), l2);
+                off2 = fma2(w2, pack2(z.x, z.y), off2);
+              } else {  // what is not seen may be anything
+                const bool n0 = xs.x == -CUDART_INF_F, n1 = xs.y == -CUDART_INF_F;
+                l2 = fma2(w2, pack2(n0 ? 0.f : vs.z, n1 ? 0.f : vs.w), l2);
+                off2 = fma2(w2, pack2(n0 ? 0.f : z.x, n1 ? 0.f : z.y), off2);
+              }
+              weights[16 * c + i / 2] = Half::down(w.x, w.y);
+            }
+          }
+          const float2 la = unpack2(l2), oa = unpack2(off2);
+          lt = la.x + la.y;
+          offt = oa.x + oa.y;
+          if (!__any_sync(0xffffffffu, mx > top + 8.f)) break;
+          // move the maximum: scale what there is, and make the weights again
+          const float f = exp2_approx(top - fmaxf(top, mx));
+          top = fmaxf(top, mx);
+          l *= f;
+          off *= f;
+          if (it > 0) {
+            if (!wait_warp(o_done + 8 * qi, it - 1)) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(o_at + 32 * c, o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_store_32(o_at + 32 * c, o);
+            }
+          }
+        }
+        if (!ok) break;
+        l += lt;
+        off += offt;
+        tmem_store_32(s_at, weights);
+        tmem_store_32(s_at + 32, weights + 32);
+        tmem_store_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready + 8 * qi);
+      }
+      if (steps > 0 && wait_warp(o_done + 8 * qi, steps - 1)) tc_fence_after();
+      const float over = l == 0.f ? 0.f : 1.f / l;
+      uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(first + token) * p.q_heads + h) * D);
+      if (ok) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (steps > 0) tmem_ld32(o_at + 32 * c, o);
+          if (!live) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float a = __uint_as_float(o[8 * i + 2 * x]), d = __uint_as_float(o[8 * i + 2 * x + 1]);
+              w[x] = l == 0.f || steps == 0 ? 0u : T::down((a + off) * over, (d + off) * over);
+            }
+            *reinterpret_cast<uint4*>(dst + 64 * c + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------- codes to operand tiles
+    constexpr int kUnits = D / 32;  // 16-byte loads of key codes a thread
+    constexpr int kWordsV = D / 64; // words of value codes per token a thread
+    const int dw = warp - 8, id = dw * 32 + lane;
+    const float c2 = p.scale * kLog2e;
+    const int per_page = p.cache.page_size / kTile;
+    auto look_up = [&](int it) {  // where the step's eight cache tiles are
+      if (dw == 0 && lane < 8 && it < steps) {
+        const int t = (step0 + it) * 8 + lane;
+        uint64_t at = 0;
+        if (static_cast<int64_t>(t) * kTile < len) {
+          const int page = p.tables[p.table_stride * b + t / per_page];
+          if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.pages))
+            at = reinterpret_cast<uint64_t>(p.cache.page_tiles<D>(page, head) + t % per_page * kBytes);
+        }
+        tile_at[8 * (it & 3) + lane] = at;
+      }
+    };
+    uint4 kr[kUnits], vr[2 * kWordsV];
+    uint32_t kp = 0, vp = 0;
+    bool here = false;
+    auto load = [&](int it) {
+      if (it >= steps) return;
+      const uint64_t* at = tile_at + 8 * (it & 3);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int rest = (u * 128 + id) >> 3, chunk = rest % kUnits, half = rest / kUnits;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(at[half >> 1]);
+        kr[u] = src ? *reinterpret_cast<const uint4*>(src + off_k(D, (half & 1) * 8 + (lane & 7)) + 16 * chunk)
+                    : make_uint4(0, 0, 0, 0);
+      }
+      {
+        const int half = (lane & 7) + 8 * (dw & 1), piece = (lane >> 3) + 4 * (dw >> 1);
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(at[half >> 1]);
+#pragma unroll
+        for (int u = 0; u < 2 * kWordsV; ++u)
+          vr[u] = src ? *reinterpret_cast<const uint4*>(src + off_v(D, (half & 1) * 8, piece) + 16 * u)
+                      : make_uint4(0, 0, 0, 0);
+      }
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(at[id >> 4]);
+      here = src != nullptr && (step0 + it) * kStep + id < len;
+      kp = here ? *reinterpret_cast<const uint32_t*>(src + off_k_pair(D, id & 15)) : 0u;
+      vp = here ? *reinterpret_cast<const uint32_t*>(src + off_v_pair(D, id & 15)) : 0u;
+    };
+    look_up(0);
+    look_up(1);
+    named_bar_sync(1, 128);
+    load(0);
+    // Once a wait has given up these warps run on without waiting: they meet at a
+    // barrier every step, which none of them may leave alone.
+    for (int it = 0; it < steps; ++it) {
+      uint4 kc[kUnits], vc[2 * kWordsV];
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) kc[u] = kr[u];
+#pragma unroll
+      for (int u = 0; u < 2 * kWordsV; ++u) vc[u] = vr[u];
+      const float2 ks = T::up(kp), vs = T::up(vp);
+      const bool there = here;
+      look_up(it + 2);
+      load(it + 1);
+      named_bar_sync(1, 128);
+      const int stage = it & 1, buf = it & 3;
+      if (it >= 2) wait_warp(k_empty + 8 * stage, (it >> 1) - 1);
+      {
+        Constants& c = constants[buf];
+        const ValueRow v = value_row(vs);
+        float* kf = reinterpret_cast<float*>(&c.key[id >> 1]) + (id & 1);
+        kf[0] = ks.x * c2;
+        kf[2] = fmaf(ks.x, 8.f, ks.y) * c2;
+        float* vf = reinterpret_cast<float*>(&c.value[id >> 1]) + (id & 1);
+        vf[0] = v.log_s;
+        vf[2] = v.inv_s;
+        reinterpret_cast<float*>(&c.at_8[id >> 1])[id & 1] = v.at_8;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) valid[4 * buf + dw] = mask;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c_full + 8 * buf);
+      }
+      {
+        const uint32_t dst = smem_addr(smem) + Cfg::kOffK + stage * Cfg::kK;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          const int rest = (u * 128 + id) >> 3, chunk = rest % kUnits, half = rest / kUnits;
+          const int key = half * 8 + (lane & 7);
+          const uint32_t w[4] = {kc[u].x, kc[u].y, kc[u].z, kc[u].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c8 = chunk * 4 + i;  // eighth channel group of the row
+            sts128(dst + (c8 >> 3) * (kStep * 128) + key * 128 + (((c8 & 7) ^ (key & 7)) << 4),
+                   centred<T::kBf16>(w[i]));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k_full + 8 * stage);
+      }
+      if (it >= 2) wait_warp(v_empty + 8 * stage, (it >> 1) - 1);
+      {
+        const uint32_t dst = smem_addr(smem) + Cfg::kOffV + stage * Cfg::kK;
+        const int half = (lane & 7) + 8 * (dw & 1), piece = (lane >> 3) + 4 * (dw >> 1);
+        // words of the eight tokens: [token][kWordsV]
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(vc);
+#pragma unroll
+        for (int o = 0; o < kWordsV; ++o) {
+          uint32_t y[2][4];  // channels 0..3 and 4..7 of the octet, tokens in pairs
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            y[0][t] = prmt(w[(2 * t) * kWordsV + o], w[(2 * t + 1) * kWordsV + o], 0x5410);
+            y[1][t] = prmt(w[(2 * t) * kWordsV + o], w[(2 * t + 1) * kWordsV + o], 0x7632);
+          }
+#pragma unroll
+          for (int part = 0; part < 4; ++part) {  // channels 2 part and 2 part + 1
+            half2 even[4], odd[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) dequant_pair(y[part >> 1][t] >> (8 * (part & 1)), even[t], odd[t]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int d = piece * (D / 8) + 8 * o + 2 * part + x;
+              const half2* z = x ? odd : even;
+              sts128(dst + (half >> 3) * (D * 128) + d * 128 + (((half & 7) ^ (d & 7)) << 4),
+                     make_uint4(*reinterpret_cast<const uint32_t*>(&z[0]), *reinterpret_cast<const uint32_t*>(&z[1]),
+                                *reinterpret_cast<const uint32_t*>(&z[2]), *reinterpret_cast<const uint32_t*>(&z[3])));
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full + 8 * stage);
+      }
+    }
+  } else if (lane == 0 && steps > 0) {
+    // ------------------------------------------------------------ products
+    constexpr uint32_t types = T::kBf16 ? (1u << 7) | (1u << 10) : 0u;
+    constexpr uint32_t id_s = umma_idesc_f16_f32(kStep) | types, id_o = umma_idesc_f16_f32(D);
+    const uint32_t base = smem_addr(smem);
+    auto scores = [&](int qi, int stage) {
+      const uint64_t a = umma_desc_sw128_k(base + qi * Cfg::kQ);
+      const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffK + stage * Cfg::kK);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
+        umma_f16(tmem + Cfg::kColS + 128 * qi, a + (at >> 4), bd + (at >> 4), id_s, k > 0);
+      }
+    };
+    auto result = [&](int qi, int stage, bool more) {
+      const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kK);
+#pragma unroll
+      for (int k = 0; k < kStep / 16; ++k) {
+        const uint32_t at = (k >> 2) * (D * 128) + (k & 3) * 32;
+        umma_f16_ts(tmem + Cfg::kColO + D * qi, tmem + Cfg::kColS + 128 * qi + 8 * k, bd + (at >> 4), id_o,
+                    more || k > 0);
+      }
+    };
+    if (wait(q_ready, 0) && wait(k_full, 0)) {
+      tc_fence_after();
+      for (int qi = 0; qi < tiles_q; ++qi) {
+        scores(qi, 0);
+        umma_commit(s_full + 8 * qi);
+      }
+      umma_commit(k_empty);
+      for (int it = 0; it < steps && ok; ++it) {
+        const int stage = it & 1, next = (it + 1) & 1;
+        const bool more = it + 1 < steps;
+        for (int qi = 0; qi < tiles_q; ++qi) {
+          if (!wait(v_full + 8 * stage, it >> 1) || !wait(p_ready + 8 * qi, it)) break;
+          tc_fence_after();
+          result(qi, stage, it > 0);
+          umma_commit(o_done + 8 * qi);
+          if (more) {
+            if (!wait(k_full + 8 * next, (it + 1) >> 1)) break;
+            tc_fence_after();
+            scores(qi, next);
+            umma_commit(s_full + 8 * qi);
+          }
+        }
+        umma_commit(v_empty + 8 * stage);
+        if (more) umma_commit(k_empty + 8 * next);
+      }
+    }
+    umma_commit(finished);
+    mbar_wait_bounded(finished, 0, drain_flag);
+  }
+  if (!ok && lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::kCols);
+  }
+}
+
+}  // namespace kv4
+}  // namespace sm100
