@@ -236,6 +236,8 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
   if (failed) return failed;
   if (!workspace || workspace_bytes < sm100::workspace_bytes(sms)) return SM100_MARLIN_ERR_SCRATCH;
   if (!aligned(workspace, 16)) return SM100_MARLIN_ERR_ALIGNMENT;
+  // a window that holds all that a table can is none
+  if (window >= static_cast<int64_t>(width) * page_size) window = 0;
   const Cache c{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, kv_heads, page_size};
   const int group = q_heads / kv_heads;
   const bool vector = aligned(q, 16) && ((q_row | q_head) & 7) == 0;

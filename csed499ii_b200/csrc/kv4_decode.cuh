@@ -100,7 +100,7 @@ __device__ __forceinline__ Span span_of(const DecodeParams& p, int b) {
   const int64_t rows = static_cast<int64_t>(s.n) * p.group;
   const bool mine = s.n > 0 && rows <= p.most;
   s.chunks = mine ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
-  const int from = p.window ? max(0, s.len - s.n - p.window + 1) : 0;
+  const int from = p.window && s.len - s.n >= p.window ? s.len - s.n - p.window + 1 : 0;
   s.tile0 = from / kTile;
   s.tiles = mine && s.len > 0 ? (s.len + kTile - 1) / kTile - s.tile0 : 0;
   return s;
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
         // what of the tile each row sees; most tiles are seen whole
         const int j0 = at.tile * kTile;
         const bool whole = j0 + kTile <= at.s.len - at.s.n + 1 &&
-                           (p.window == 0 || j0 >= at.s.len - p.window);
+                           (p.window == 0 || at.s.len - j0 <= p.window);
         bool seen[NT][4];
         if (!whole) {
 #pragma unroll
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
             for (int c = 0; c < 4; ++c) {
               const int j = j0 + g + (c < 2 ? 0 : 8);
               seen[nt][c] = j <= place[nt][c & 1] && j < at.s.len &&
-                            (p.window == 0 || j > place[nt][c & 1] - p.window);
+                            (p.window == 0 || place[nt][c & 1] - j < p.window);
               if (!seen[nt][c]) x[nt][c] = -CUDART_INF_F;
             }
         }

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int tiles_q = rows > 128 ? 2 : 1;
   const int before = len - n;  // position of the request's row 0
   const int lo_pos = before + tile * 256 / p.group, hi_pos = before + (tile * 256 + rows - 1) / p.group;
-  const int from = p.window ? max(0, lo_pos - p.window + 1) : 0;
+  const int from = p.window && lo_pos >= p.window ? lo_pos - p.window + 1 : 0;
   const int to = min(len, hi_pos + 1);
   const int step0 = from / kStep;
   const int steps = to > from ? (to + kStep - 1) / kStep - step0 : 0;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         tc_fence_after();
         const Constants& k = constants[buf];
         const int j0 = (step0 + it) * kStep;
-        const bool whole = j0 + kStep <= tile_lo + 1 && (p.window == 0 || j0 > tile_hi - p.window) &&
+        const bool whole = j0 + kStep <= tile_lo + 1 && (p.window == 0 || tile_hi - j0 < p.window) &&
                            (valid[4 * buf] & valid[4 * buf + 1] & valid[4 * buf + 2] & valid[4 * buf + 3]) ==
                                0xffffffffu;
         uint32_t weights[64];
@@ -354,9 +354,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               if (!whole) {
                 float2 y = unpack2(x);
                 const int j = j0 + 32 * c + i;
-                const int oldest = p.window ? pos - p.window : -1;
-                if (j > pos || j <= oldest || !(there >> i & 1)) y.x = -CUDART_INF_F;
-                if (j + 1 > pos || j + 1 <= oldest || !(there >> (i + 1) & 1)) y.y = -CUDART_INF_F;
+                const int back = p.window ? p.window : 0x7fffffff;  // a query sees less far than this
+                if (j > pos || pos - j >= back || !(there >> i & 1)) y.x = -CUDART_INF_F;
+                if (j + 1 > pos || pos - j - 1 >= back || !(there >> (i + 1) & 1)) y.y = -CUDART_INF_F;
                 x = pack2(y.x, y.y);
               }
               const float2 xs = unpack2(x);

@@ -17,7 +17,6 @@ the layout byte by byte.  Nothing here copies to the host or waits for the GPU.
 """
 from __future__ import annotations
 
-import math
 from typing import NamedTuple
 
 import torch
@@ -38,6 +37,13 @@ _DIMS = {8 * 64 + 64: 64, 8 * 128 + 64: 128}
 
 def _raise(name, err):
     raise RuntimeError(f"{name}: sm100_marlin error {err}: {_ext.describe(err)}")
+
+
+def _entry(name):
+    """The C entry sm100_marlin_<name>: through the CPython binding, or through
+    ctypes where that has not been built."""
+    fast = _ext._fast if _ext._fast_tried else _ext.fast()
+    return getattr(_ext.load(), "sm100_marlin_" + name) if fast is None else getattr(fast, name)
 
 
 def _check_ints(name, t, dev, numel=None):
@@ -131,18 +137,26 @@ def kv4_schedule(new_lens, lens, block_tables, free_pages, free_count, rows, pag
         a CUDA graph updates them in place)
     """
     dev = new_lens.get_device()
-    if dev < 0:
-        raise RuntimeError("new_lens must be a CUDA tensor")
-    batch = new_lens.numel()
-    _check_ints("new_lens", new_lens, dev)
-    _check_ints("lens", lens, dev, batch)
-    _check_ints("free_pages", free_pages, dev)
-    _check_ints("free_count", free_count, dev, 1)
-    _check_tables(block_tables, dev, batch)
-    if batch > 8192:
-        raise RuntimeError("kv4_schedule takes at most 8192 requests")
-    if rows < 0 or page_size <= 0:
-        raise RuntimeError("rows must not be negative, page_size must be positive")
+    batch, tables_shape = new_lens.numel(), block_tables.shape
+    # one combined test; the checks with their messages only run when it fails
+    if not (dev >= 0 and new_lens.dtype is _INT32 and lens.dtype is _INT32 and lens.get_device() == dev
+            and lens.numel() == batch <= 8192 and block_tables.dtype is _INT32
+            and block_tables.get_device() == dev and len(tables_shape) == 2 and tables_shape[0] == batch
+            and free_pages.dtype is _INT32 and free_pages.get_device() == dev
+            and free_count.dtype is _INT32 and free_count.get_device() == dev and free_count.numel() == 1
+            and new_lens.is_contiguous() and lens.is_contiguous() and block_tables.is_contiguous()
+            and free_pages.is_contiguous() and rows >= 0 and 0 < page_size < 2**31):
+        if dev < 0:
+            raise RuntimeError("new_lens must be a CUDA tensor")
+        _check_ints("new_lens", new_lens, dev)
+        _check_ints("lens", lens, dev, batch)
+        _check_ints("free_pages", free_pages, dev)
+        _check_ints("free_count", free_count, dev, 1)
+        _check_tables(block_tables, dev, batch)
+        if batch > 8192:
+            raise RuntimeError("kv4_schedule takes at most 8192 requests")
+        if rows < 0 or not 0 < page_size < 2**31:
+            raise RuntimeError("rows must not be negative, page_size must be positive")
     if lens_out is None:
         lens_out = torch.empty_like(lens)
     else:
@@ -151,16 +165,16 @@ def kv4_schedule(new_lens, lens, block_tables, free_pages, free_count, rows, pag
         free_count_out = torch.empty_like(free_count)
     else:
         _check_ints("free_count_out", free_count_out, dev, 1)
-    starts = torch.empty(batch + 1, dtype=_INT32, device=new_lens.device)
-    slots = torch.empty(rows, dtype=_INT32, device=new_lens.device)
-    positions = torch.empty(rows, dtype=_INT32, device=new_lens.device)
-    fate = torch.empty(batch, dtype=_INT32, device=new_lens.device)
-    err = _ext.load().sm100_marlin_kv4_schedule(
+    device = new_lens.device
+    starts = torch.empty(batch + 1, dtype=_INT32, device=device)
+    slots = torch.empty(rows, dtype=_INT32, device=device)
+    positions = torch.empty(rows, dtype=_INT32, device=device)
+    fate = torch.empty_like(lens)
+    err = _entry("kv4_schedule")(
         new_lens.data_ptr(), lens.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-        block_tables.size(1), batch, free_pages.data_ptr(), free_pages.numel(),
-        free_count.data_ptr(), rows, page_size, lens_out.data_ptr(), free_count_out.data_ptr(),
-        starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), fate.data_ptr(), dev,
-        _stream_ptr(dev))
+        tables_shape[1], batch, free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), rows,
+        page_size, lens_out.data_ptr(), free_count_out.data_ptr(), starts.data_ptr(), slots.data_ptr(),
+        positions.data_ptr(), fate.data_ptr(), dev, _stream_ptr(dev))
     if err:
         _raise("kv4_schedule", err)
     return KV4Step(lens_out, free_count_out, starts, slots, positions, fate)
@@ -186,16 +200,20 @@ def kv4_append(k, v, cache, slots):
         outside the cache (-1) are skipped
     """
     pages, heads, page_size, dim, dtype, dev = _cache_shape(cache)
-    _check_rows("k", k, cache, heads, dim, dev)
-    _check_rows("v", v, cache, heads, dim, dev)
-    tokens = k.size(0)
-    if v.size(0) != tokens:
-        raise RuntimeError("k and v must have the same number of tokens")
-    _check_ints("slots", slots, dev, tokens)
-    err = _ext.load().sm100_marlin_kv4_append(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-        cache.data_ptr(), pages, heads, page_size, dim, dtype, slots.data_ptr(), tokens, dev,
-        _stream_ptr(dev))
+    shape, k_at, v_at, kind = k.shape, k.stride(), v.stride(), cache.dtype
+    tokens = shape[0] if shape else 0
+    if not (k.dtype is kind and v.dtype is kind and k.get_device() == dev and v.get_device() == dev
+            and shape == (tokens, heads, dim) == v.shape and k_at[2] == 1 and v_at[2] == 1
+            and slots.dtype is _INT32 and slots.get_device() == dev and slots.numel() == tokens
+            and slots.is_contiguous()):
+        _check_rows("k", k, cache, heads, dim, dev)
+        _check_rows("v", v, cache, heads, dim, dev)
+        if v.size(0) != tokens:
+            raise RuntimeError("k and v must have the same number of tokens")
+        _check_ints("slots", slots, dev, tokens)
+    err = _entry("kv4_append")(
+        k.data_ptr(), k_at[0], k_at[1], v.data_ptr(), v_at[0], v_at[1], cache.data_ptr(), pages, heads,
+        page_size, dim, dtype, slots.data_ptr(), tokens, dev, _stream_ptr(dev))
     if err:
         _raise("kv4_append", err)
 
@@ -208,9 +226,8 @@ def kv4_read(cache, slots):
     tokens = slots.numel()
     k = torch.empty((tokens, heads, dim), dtype=cache.dtype, device=cache.device)
     v = torch.empty_like(k)
-    err = _ext.load().sm100_marlin_kv4_read(cache.data_ptr(), pages, heads, page_size, dim, dtype,
-                                            slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(),
-                                            dev, _stream_ptr(dev))
+    err = _entry("kv4_read")(cache.data_ptr(), pages, heads, page_size, dim, dtype, slots.data_ptr(),
+                             tokens, k.data_ptr(), v.data_ptr(), dev, _stream_ptr(dev))
     if err:
         _raise("kv4_read", err)
     return k, v
@@ -256,24 +273,28 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
         current stream
     """
     pages, heads, page_size, dim, dtype, dev = _cache_shape(cache)
-    _check_rows("q", q, cache, None, dim, dev)
-    rows, q_heads = q.size(0), q.size(1)
+    shape, at, tables_shape, batch = q.shape, q.stride(), block_tables.shape, lens.numel()
+    if not (q.dtype is cache.dtype and q.get_device() == dev and len(shape) == 3 and shape[2] == dim
+            and at[2] == 1 and lens.dtype is _INT32 and lens.get_device() == dev and lens.is_contiguous()
+            and block_tables.dtype is _INT32 and block_tables.get_device() == dev
+            and len(tables_shape) == 2 and tables_shape[0] == batch and block_tables.is_contiguous()):
+        _check_rows("q", q, cache, None, dim, dev)
+        _check_ints("lens", lens, dev)
+        _check_tables(block_tables, dev, batch)
+    rows, q_heads = shape[0], shape[1]
     if q_heads == 0 or q_heads % heads != 0:
         raise RuntimeError(f"q must have a multiple of {heads} heads, got {q_heads}")
-    batch = lens.numel()
-    _check_ints("lens", lens, dev, batch)
-    _check_tables(block_tables, dev, batch)
     if starts is None:
         if rows != batch:
             raise RuntimeError(f"without starts q must have one row for each of the {batch} requests")
-        max_new = 1
+        max_new, starts_at = 1, 0
     else:
         _check_ints("starts", starts, dev, batch + 1)
-        max_new = rows if max_new is None else max_new
-    if window < 0 or max_new < 0:
-        raise ValueError("window and max_new must not be negative")
+        max_new, starts_at = rows if max_new is None else max_new, starts.data_ptr()
+    if not (0 <= window < 2**31 and 0 <= max_new < 2**31):
+        raise ValueError("window and max_new must not be negative, and be below 2**31")
     if out is None:
-        out = torch.empty((rows, q_heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
     else:
         _check_rows("out", out, cache, q_heads, dim, dev)
         if out.size(0) != rows or not out.is_contiguous():
@@ -283,12 +304,11 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
         workspace = _workspace(dev, stream)
     else:
         _check_ints("workspace", workspace, dev)
-    err = _ext.load().sm100_marlin_kv4_attention(
-        q.data_ptr(), q.stride(0), q.stride(1), cache.data_ptr(), pages, heads, page_size, dim, dtype,
-        block_tables.data_ptr(), block_tables.stride(0), block_tables.size(1), lens.data_ptr(),
-        0 if starts is None else starts.data_ptr(), batch, rows, q_heads, max_new, window,
-        1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), workspace.data_ptr(),
-        4 * workspace.numel(), dev, stream)
+    err = _entry("kv4_attention")(
+        q.data_ptr(), at[0], at[1], cache.data_ptr(), pages, heads, page_size, dim, dtype,
+        block_tables.data_ptr(), block_tables.stride(0), tables_shape[1], lens.data_ptr(), starts_at,
+        batch, rows, q_heads, max_new, window, dim**-0.5 if scale is None else scale, out.data_ptr(),
+        workspace.data_ptr(), 4 * workspace.numel(), dev, stream)
     if err == _ext.ERR_SCRATCH:
         need = _ext.load().sm100_marlin_kv4_workspace_bytes(dev) // 4
         raise RuntimeError(f"workspace must be of size at least {need}.")
