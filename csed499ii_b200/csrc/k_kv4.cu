@@ -75,19 +75,24 @@ size_t workspace_bytes(int sms) {
 }
 
 template <class T, int D, int NT>
-int launch_decode(DecodeParams p, int sms, int dev, cudaStream_t stream) {
+int launch_decode(DecodeParams p, int64_t most, int sms, int dev, cudaStream_t stream) {
   using Cfg = DecodeCfg<D, NT>;
   static_assert(Cfg::kCtas * Cfg::kPart <= 2 * DecodeCfg<128, 2>::kPart, "workspace");
   const int bad = allow_smem<kv4_decode_kernel<T, D, NT>>(dev, Cfg::kSmem);
   if (bad) return bad;
-  // The kernel keeps a sum per request in shared memory: larger batches go in slices.
-  const int batch = p.batch;
+  // The kernel keeps a sum per request in shared memory, and counts tiles in 32
+  // bits: larger batches go in slices.
+  const int64_t tiles = static_cast<int64_t>(p.width) * (p.cache.page_size / kTile) *
+                        p.cache.heads * ((most + Cfg::kRows - 1) / Cfg::kRows);  // of a request, at most
+  const int64_t fit = 0x7fffffffll / (tiles > 0 ? tiles : 1);
+  if (fit < 1) return SM100_MARLIN_ERR_PROB_SHAPE;
+  const int slice = static_cast<int>(fit < kDecodeBatch ? fit : kDecodeBatch), batch = p.batch;
   int done = 0;
   do {
-    const int n = batch - done < kDecodeBatch ? batch - done : kDecodeBatch;
+    const int n = batch - done < slice ? batch - done : slice;
     p.batch = n;
     p.pad = done + n == batch;
-    kv4_decode_kernel<T, D, NT><<<sms * Cfg::kCtas, 256, Cfg::kSmem, stream>>>(p);
+    kv4_decode_kernel<T, D, NT><<<sms * Cfg::kCtas, Cfg::kThreads, Cfg::kSmem, stream>>>(p);
     p.lens += n;
     p.tables += n * p.table_stride;
     p.row0 += n;
@@ -243,6 +248,7 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
   const bool vector = aligned(q, 16) && ((q_row | q_head) & 7) == 0;
   const int few_rows = group > kFewRows ? group : kFewRows;  // a single token is always few
   const int64_t most = static_cast<int64_t>(starts ? max_new : 1) * group;
+  const int64_t few_most = most < few_rows ? most : few_rows;
   const DecodeParams few{c, static_cast<const uint8_t*>(q), q_row, q_head, vector,
                          static_cast<uint8_t*>(out), block_tables, table_stride, width, lens, starts,
                          0, batch, rows, 1, q_heads, group, window, few_rows, scale,
@@ -255,8 +261,8 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
   return dispatch(dtype, head_dim, [&](auto type, auto dim) {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value;
-    const int bad = most <= 8 ? launch_decode<T, D, 1>(few, sms, dev, on_stream)
-                              : launch_decode<T, D, 2>(few, sms, dev, on_stream);
+    const int bad = most <= 8 ? launch_decode<T, D, 1>(few, few_most, sms, dev, on_stream)
+                              : launch_decode<T, D, 2>(few, few_most, sms, dev, on_stream);
     return bad || most <= few_rows ? bad : launch_prompt<T, D>(many, dev, on_stream);
   });
 }

@@ -40,7 +40,8 @@
 namespace sm100 {
 namespace kv4 {
 
-constexpr int kDecodeBatch = 1024;  // requests of a launch: 8 bytes of shared memory each
+constexpr int kDecodeBatch = 1024;  // requests of a launch: 4 bytes of shared memory each
+constexpr int kLeast = 16;          // tiles of a CTA: fewer are not worth sharing an item
 
 struct DecodeParams {
   Cache cache;
@@ -70,14 +71,16 @@ struct DecodeParams {
 template <int D, int NT>
 struct DecodeCfg {
   static constexpr int kWarps = 8;
+  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kDepth = 4;             // tiles in a warp's ring
   static constexpr int kRows = 8 * NT;         // query rows of an item
   static constexpr int kPart = kRows * (D + 2);  // floats: results, maxima, sums
   static constexpr int kRing = kWarps * kDepth * tile_bytes(D);
   static constexpr int kOffParts = kRing;
   static constexpr int kOffPre = kOffParts + kWarps * kPart * 4;
-  static constexpr int kOffMisc = kOffPre + kDecodeBatch * 8;
-  static constexpr int kSmem = kOffMisc + 2048;
+  static constexpr int kOffMisc = kOffPre + kDecodeBatch * 4;
+  static constexpr int kMisc = 1424 + 64 * kRows;
+  static constexpr int kSmem = kOffMisc + kMisc;
   static constexpr int kCtas = kSmem <= 113 * 1024 ? 2 : 1;  // of an SM
   // a warp's last part takes the place of its ring
   static_assert(kPart * 4 <= kDepth * tile_bytes(D), "part does not fit the ring");
@@ -106,14 +109,14 @@ __device__ __forceinline__ Span span_of(const DecodeParams& p, int b) {
   return s;
 }
 
-// One place in the row of all tiles.
+// One item (a request, a key/value head, kRows of its query rows) and a tile.
 struct Walk {
   Span s;
   int b, head, chunk, tile;  // tile of the request
 };
 
 template <int ROWS>
-__device__ __forceinline__ Walk walk_to(const DecodeParams& p, const int64_t* pre, int64_t at) {
+__device__ __forceinline__ Walk walk_to(const DecodeParams& p, const int* pre, int at) {
   int lo = 0, n = p.batch - 1;  // the first request whose end is past `at`
   while (n > 0) {
     const int half = n >> 1;
@@ -127,35 +130,28 @@ __device__ __forceinline__ Walk walk_to(const DecodeParams& p, const int64_t* pr
   Walk w;
   w.b = lo;
   w.s = span_of<ROWS>(p, lo);
-  const int64_t off = at - (lo ? pre[lo - 1] : 0);
+  const int off = at - (lo ? pre[lo - 1] : 0);
   const int tiles = max(w.s.tiles, 1);
-  const int item = static_cast<int>(off / tiles);
-  w.tile = w.s.tile0 + static_cast<int>(off - static_cast<int64_t>(item) * tiles);
+  const int item = off / tiles;
+  w.tile = w.s.tile0 + off - item * tiles;
   w.head = item / max(w.s.chunks, 1);
   w.chunk = item - w.head * max(w.s.chunks, 1);
   return w;
 }
 
-// To the next tile; true where that begins another item.
+// To the first tile of the next item; only called while there is one.
 template <int ROWS>
-__device__ __forceinline__ bool walk_on(const DecodeParams& p, Walk& w) {
-  if (++w.tile < w.s.tile0 + w.s.tiles) return false;
+__device__ __forceinline__ void next_item(const DecodeParams& p, Walk& w) {
   if (++w.chunk == w.s.chunks) {
     w.chunk = 0;
     if (++w.head == p.cache.heads) {
       w.head = 0;
       do {
-        if (++w.b >= p.batch) return true;  // the end of all work
-        w.s = span_of<ROWS>(p, w.b);
-      } while (w.s.tiles == 0);
+        w.s = span_of<ROWS>(p, ++w.b);
+      } while (w.s.tiles == 0 && w.b + 1 < p.batch);
     }
   }
   w.tile = w.s.tile0;
-  return true;
-}
-
-__device__ __forceinline__ int page_of(const DecodeParams& p, const Walk& w) {
-  return w.b < p.batch ? p.tables[p.table_stride * w.b + w.tile / (p.cache.page_size / kTile)] : -1;
 }
 
 template <bool BF16>
@@ -185,6 +181,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
 }
 
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
@@ -226,59 +226,58 @@ __device__ __forceinline__ ValueRow value_row(float2 pair) {
 // A part of an item, or all of it: results (already divided by the sum), the
 // running maximum of the scores (times log2 e) and the sum of the weights.
 struct Segment {
-  long long begin, end;  // the item's place in the row of all tiles; begin < 0: none
+  int begin, end;  // the item's place in the row of all tiles; begin < 0: none
   int b, head, chunk;
 };
 
 constexpr float kLowest = -3.0e38f;
 
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
+__global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::kCtas)
     kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   using Cfg = DecodeCfg<D, NT>;
   constexpr int kRows = Cfg::kRows, kPart = Cfg::kPart, kDepth = Cfg::kDepth, kBytes = tile_bytes(D);
   constexpr int kWords = D / 32;  // code words of a lane in a row of keys
   constexpr bool kBf = T::kBf16;
   extern __shared__ __align__(128) uint8_t smem[];
-  int64_t* pre = reinterpret_cast<int64_t*>(smem + Cfg::kOffPre);
+  int* pre = reinterpret_cast<int*>(smem + Cfg::kOffPre);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffMisc);            // [warps][depth]
-  int* there = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 256);               // [warps][depth]
-  Segment* segments = reinterpret_cast<Segment*>(smem + Cfg::kOffMisc + 384);    // [warps][2]
-  int64_t* sums = reinterpret_cast<int64_t*>(smem + Cfg::kOffMisc + 1024);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kOffMisc + 1152);
-  volatile int* drain_flag = abort_flag + 2;
-  int* last_flag = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 1156);
-  static_assert(sizeof(Segment) * 16 <= 640, "segments");
+  int* there = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 512);               // [warps][depth]
+  Segment* segments = reinterpret_cast<Segment*>(smem + Cfg::kOffMisc + 640);    // [warps][2]
+  int* sums = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 1280);               // [warps]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kOffMisc + 1408);
+  volatile int* drain_flag = abort_flag + 1;
+  int* last_flag = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 1416);
+  float* join_w = reinterpret_cast<float*>(smem + Cfg::kOffMisc + 1424);         // [2 warps][rows]
+  static_assert(sizeof(Segment) * 16 <= 640 && 1424 + 4 * 16 * kRows <= Cfg::kMisc, "shared memory");
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_addr(smem) + warp * kDepth * kBytes;
-  const uint32_t bar0 = smem_addr(bars + warp * kDepth);
 
-  if (lane < kDepth) mbar_init(bar0 + 8 * lane, 1);
+  if (lane < kDepth) mbar_init(smem_addr(bars + kDepth * warp + lane), 1);
   if (lane == 0) segments[2 * warp].begin = segments[2 * warp + 1].begin = -1;
   if (threadIdx.x == 0) *abort_flag = *drain_flag = 0;
   fence_mbar_init();
 
   // --- the row of all tiles: where each request's end is -------------------
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 256) {
+  int total = 0;  // the host keeps it below 2^31
+  for (int b0 = 0; b0 < p.batch; b0 += Cfg::kThreads) {
     const int b = b0 + threadIdx.x;
-    int64_t x = 0;
+    int x = 0;
     if (b < p.batch) {
       const Span s = span_of<kRows>(p, b);
-      x = static_cast<int64_t>(p.cache.heads) * s.chunks * s.tiles;
+      x = p.cache.heads * s.chunks * s.tiles;
     }
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, i);
+      const int y = __shfl_up_sync(0xffffffffu, x, i);
       if (lane >= i) x += y;
     }
     if (lane == 31) sums[warp] = x;
     __syncthreads();
-    int64_t all = 0;
+    int all = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < Cfg::kWarps; ++i) {
       if (i == warp) x += all;
       all += sums[i];
     }
@@ -294,66 +293,85 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
       if (pre[b] != (b ? pre[b - 1] : 0)) continue;
       const Span s = span_of<kRows>(p, b);
       if (s.chunks == 0) continue;
-      for (int64_t i = 16 * threadIdx.x; i < s.n * row_bytes; i += 16 * 256)
+      for (int64_t i = 16 * threadIdx.x; i < s.n * row_bytes; i += 16 * Cfg::kThreads)
         *reinterpret_cast<uint4*>(p.out + s.first * row_bytes + i) = make_uint4(0, 0, 0, 0);
     }
     const int end = !p.starts || !p.pad ? p.rows : p.batch ? max(p.starts[p.batch], 0) : 0;
     for (int row = min(end, p.rows) + blockIdx.x; row < p.rows; row += gridDim.x)
-      for (int64_t i = 16 * threadIdx.x; i < row_bytes; i += 16 * 256)
+      for (int64_t i = 16 * threadIdx.x; i < row_bytes; i += 16 * Cfg::kThreads)
         *reinterpret_cast<uint4*>(p.out + row * row_bytes + i) = make_uint4(0, 0, 0, 0);
   }
 
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * Cfg::kWarps;
-  const int64_t quota = max((total + warps - 1) / warps, static_cast<int64_t>(2));
-  const int64_t cta_begin = quota * Cfg::kWarps * blockIdx.x;
-  if (cta_begin >= total) return;
-  const int64_t begin = min(cta_begin + quota * warp, total);
-  const int64_t end = min(begin + quota, total);
-  const int count = static_cast<int>(end - begin);
+  const int quota = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kLeast);  // of a CTA
+  if (static_cast<int64_t>(quota) * blockIdx.x >= total) return;
+  const int cta_begin = quota * blockIdx.x;
+  const int cta_end = min(cta_begin + quota, total);
+  const int share = (cta_end - cta_begin + Cfg::kWarps - 1) / Cfg::kWarps;
+  const int begin = min(cta_begin + share * warp, cta_end);
+  const int count = min(begin + share, cta_end) - begin;
 
   // --- this warp's run ------------------------------------------------------
   if (count > 0) {
-    Walk in = walk_to<kRows>(p, pre, begin), at = in;
-    int page = page_of(p, in);
-    int issued = 0;
+    const uint32_t ring = smem_addr(smem) + warp * kDepth * kBytes;
+    const uint32_t full = smem_addr(bars + kDepth * warp);
+    Walk at = walk_to<kRows>(p, pre, begin);
+
+    // The copies run ahead of the work: `in` is the item of the next one, and
+    // a page's number is looked up a page early.
+    Walk in = at;
+    const int per_page = p.cache.page_size / kTile;
     const uint64_t policy = policy_evict_first();
-    // starts the copy of the next tile of the run; its page was looked up a tile ago
+    int issued = 0, entry, nth, page, next;  // nth tile of the page
+    auto start = [&]() {
+      entry = in.tile / per_page;
+      nth = in.tile - entry * per_page;
+      const int* table = p.tables + p.table_stride * in.b;
+      page = table[entry];
+      next = entry + 1 < p.width ? table[entry + 1] : -1;
+    };
     auto issue = [&]() {
       const int slot = issued % kDepth;
       const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.pages);
       if (lane == 0) {
         there[warp * kDepth + slot] = ok;
         if (ok) {
-          const uint8_t* src = p.cache.page_tiles<D>(page, in.head) +
-                               in.tile % (p.cache.page_size / kTile) * kBytes;
-          mbar_arrive_expect_tx(bar0 + 8 * slot, kBytes);
-          bulk_g2s(ring + slot * kBytes, src, kBytes, bar0 + 8 * slot, policy);
+          mbar_arrive_expect_tx(full + 8 * slot, kBytes);
+          bulk_g2s(ring + slot * kBytes, p.cache.page_tiles<D>(page, in.head) + nth * kBytes, kBytes,
+                   full + 8 * slot, policy);
         } else {
-          mbar_arrive(bar0 + 8 * slot);
+          mbar_arrive(full + 8 * slot);
         }
       }
-      if (++issued < count) {
-        walk_on<kRows>(p, in);
-        page = page_of(p, in);
+      if (++issued == count) return;
+      if (++in.tile == in.s.tile0 + in.s.tiles) {
+        next_item<kRows>(p, in);
+        start();
+      } else if (++nth == per_page) {
+        nth = 0;
+        ++entry;
+        page = next;
+        next = entry + 1 < p.width ? p.tables[p.table_stride * in.b + entry + 1] : -1;
       }
     };
+    // the first queries are on their way while the first pages are looked up
+    if (at.chunk * kRows + (lane >> 2) < at.s.n * p.group)
+      prefetch_l1(p.q + 2 * (p.q_row * (at.s.first + (at.chunk * kRows + (lane >> 2)) / p.group) +
+                             p.q_head * (at.head * p.group + (at.chunk * kRows + (lane >> 2)) % p.group) + t * (D / 4)));
+    start();
     for (int i = 0; i < kDepth && issued < count; ++i) issue();
 
     uint32_t qe[NT][kWords][2], qo[NT][kWords][2];  // queries: even and odd nibbles' channels
     float sumq[NT][2];
     int place[NT][2];                               // positions of this lane's two rows
     float acc[NT][D / 16][4];
-    float top[NT][2], l[NT][2], a1[NT][2], a2[NT][2];
+    float top[NT][2], l[NT][2], a1[NT][2], ones[NT][4];
     const float c2 = p.scale * kLog2e;
     const float c1 = kBf ? c2 : c2 * 16777216.f;
-    bool fresh = true;
-    int64_t item_begin = 0, item_end = 0;
-
-    for (int i = 0; i < count; ++i) {
-      if (fresh) {
-        fresh = false;
-        item_begin = begin + i - (at.tile - at.s.tile0);
-        item_end = item_begin + at.s.tiles;
+    int i = 0;  // tiles done
+    while (i < count) {
+      const int item_begin = begin + i - (at.tile - at.s.tile0), item_end = item_begin + at.s.tiles;
+      const int stop = min(at.s.tile0 + at.s.tiles, at.tile + count - i);
+      {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int r = at.chunk * kRows + nt * 8 + g;
@@ -389,7 +407,7 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
             sumq[nt][c] = __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
             place[nt][c] = at.s.len - at.s.n + (at.chunk * kRows + nt * 8 + 2 * t + c) / p.group;
             top[nt][c] = kLowest;
-            l[nt][c] = a1[nt][c] = a2[nt][c] = 0.f;
+            l[nt][c] = a1[nt][c] = ones[nt][c] = ones[nt][c + 2] = 0.f;
           }
 #pragma unroll
           for (int x = 0; x < D / 16; ++x)
@@ -398,16 +416,15 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
         }
       }
 
-      const int slot = i % kDepth;
-      const uint32_t tile = ring + slot * kBytes;
-      if (!mbar_wait_bounded(bar0 + 8 * slot, (i / kDepth) & 1, abort_flag)) {
-        if (lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
-        // the copies still in flight land before the CTA's memory is handed on
-        for (int j = i; j < issued; ++j)
-          mbar_wait_bounded(bar0 + 8 * (j % kDepth), (j / kDepth) & 1, drain_flag);
-        break;
-      }
-      if (there[warp * kDepth + slot]) {
+      bool lost = false;
+      for (; at.tile < stop; ++at.tile, ++i) {
+        const int slot = i % kDepth;
+        const uint32_t tile = ring + slot * kBytes;
+        if (!mbar_wait_bounded(full + 8 * slot, (i / kDepth) & 1, abort_flag)) {
+          lost = true;
+          break;
+        }
+        if (there[warp * kDepth + slot]) {
         // scores
         uint32_t k0[kWords], k1[kWords];
         if constexpr (D == 128) {
@@ -420,8 +437,8 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
           k1[0] = y.x, k1[1] = y.y;
         }
         const float2 kp0 = T::up(lds32(tile + off_k_pair(D, g))), kp1 = T::up(lds32(tile + off_k_pair(D, g + 8)));
-        const ValueRow v0 = value_row(T::up(lds32(tile + off_v_pair(D, g))));
-        const ValueRow v1 = value_row(T::up(lds32(tile + off_v_pair(D, g + 8))));
+        ValueRow v0 = value_row(T::up(lds32(tile + off_v_pair(D, g))));
+        ValueRow v1 = value_row(T::up(lds32(tile + off_v_pair(D, g + 8))));
         float x[NT][4];  // arguments of the weights
         {
           float e[NT][4] = {}, o[NT][4] = {};
@@ -454,17 +471,25 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
         const int j0 = at.tile * kTile;
         const bool whole = j0 + kTile <= at.s.len - at.s.n + 1 &&
                            (p.window == 0 || at.s.len - j0 <= p.window);
-        bool seen[NT][4];
         if (!whole) {
+          // A row of values that stands for NaN counts through its scores where
+          // it is seen; where it is not, scale and offset may be anything.
+          const bool bad0 = !(fabsf(v0.at_8) <= 3.4e38f), bad1 = !(fabsf(v1.at_8) <= 3.4e38f);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const int j = j0 + g + (c < 2 ? 0 : 8);
-              seen[nt][c] = j <= place[nt][c & 1] && j < at.s.len &&
-                            (p.window == 0 || place[nt][c & 1] - j < p.window);
-              if (!seen[nt][c]) x[nt][c] = -CUDART_INF_F;
+              const bool seen = j <= place[nt][c & 1] && j < at.s.len &&
+                                (p.window == 0 || place[nt][c & 1] - j < p.window);
+              if (!seen) {
+                x[nt][c] = -CUDART_INF_F;
+              } else if (c < 2 ? bad0 : bad1) {
+                x[nt][c] = CUDART_NAN_F;
+              }
             }
+          if (bad0 || j0 + g >= at.s.len) v0.inv_s = v0.at_8 = 0.f;
+          if (bad1 || j0 + g + 8 >= at.s.len) v1.inv_s = v1.at_8 = 0.f;
         }
         // The maximum moves only where an argument passes it by more than 8 (a
         // factor of 256, harmless in the sums), so most tiles need no exchange.
@@ -472,7 +497,7 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) moves |= x[nt][c] > top[nt][c & 1] + 8.f;
+          for (int c = 0; c < 4; ++c) moves |= x[nt][c] - top[nt][c & 1] > 8.f;
         if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -487,7 +512,7 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
               top[nt][c] = m;
               l[nt][c] *= f[c];
               a1[nt][c] *= f[c];
-              a2[nt][c] *= f[c];
+              ones[nt][c] *= f[c];
             }
 #pragma unroll
             for (int y = 0; y < D / 16; ++y) {
@@ -499,6 +524,7 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
           }
         }
         // weights, and their sums
+        constexpr uint32_t kOnes = 0x3c003c00u;  // 1.0 twice: the sum of the rounded weights
         uint32_t wb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -506,19 +532,12 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             w[c] = exp2_approx(x[nt][c] - top[nt][c & 1]);
-            // where nothing is seen, scale and offset may be anything
-            const bool none = !whole && !seen[nt][c];
-            l[nt][c & 1] = fmaf(w[c], none ? 0.f : c < 2 ? v0.inv_s : v1.inv_s, l[nt][c & 1]);
-            a1[nt][c & 1] = fmaf(w[c], none ? 0.f : c < 2 ? v0.at_8 : v1.at_8, a1[nt][c & 1]);
+            l[nt][c & 1] = fmaf(w[c], c < 2 ? v0.inv_s : v1.inv_s, l[nt][c & 1]);
+            a1[nt][c & 1] = fmaf(w[c], c < 2 ? v0.at_8 : v1.at_8, a1[nt][c & 1]);
           }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t y = Half::down(w[2 * c], w[2 * c + 1]);
-            const float2 back = Half::up(y);
-            a2[nt][0] += back.x;
-            a2[nt][1] += back.y;
-            wb[nt][c] = transpose_8x8(y);
-          }
+          wb[nt][0] = transpose_8x8(Half::down(w[0], w[1]));
+          wb[nt][1] = transpose_8x8(Half::down(w[2], w[3]));
+          mma_16816<false>(ones[nt], kOnes, kOnes, kOnes, kOnes, wb[nt][0], wb[nt][1]);
         }
         // result
         constexpr int kOctets = D / 64;
@@ -547,21 +566,25 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
                                z8 & 0x000f000fu, z8 & 0x00f000f0u, wb[nt][0], wb[nt][1]);
             }
           }
+        }
+        __syncwarp();  // the slot is read
+        if (issued < count) issue();
       }
-      __syncwarp();  // the slot is read
-      if (issued < count) issue();
+      if (lost) {
+        if (lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
+        // the copies that may be in flight land before the CTA's memory is handed on
+        for (; i < issued; ++i)
+          mbar_wait_bounded(full + 8 * (i % kDepth), (i / kDepth) & 1, drain_flag);
+        break;
+      }
 
       // --- the end of an item, or of the run --------------------------------
-      const Walk here = at;
-      const bool ends = walk_on<kRows>(p, at);
-      if (!ends && i + 1 < count) continue;
-      fresh = true;
-      const bool all = item_begin >= begin && item_end <= end;
-      const bool is_head = !all && ends && item_begin < begin && i + 1 < count;
+      const bool all = item_begin >= begin && item_end <= begin + count;
+      const bool is_head = item_begin < begin && i < count;
       float* part = is_head ? reinterpret_cast<float*>(smem + Cfg::kOffParts) + warp * kPart
                             : reinterpret_cast<float*>(smem + warp * kDepth * kBytes);
       if (!all && lane == 0)
-        segments[2 * warp + (is_head ? 0 : 1)] = {item_begin, item_end, here.b, here.head, here.chunk};
+        segments[2 * warp + (is_head ? 0 : 1)] = {item_begin, item_end, at.b, at.head, at.chunk};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -570,21 +593,20 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
           for (int s = 4; s < 32; s <<= 1) {
             l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], s);
             a1[nt][c] += __shfl_xor_sync(0xffffffffu, a1[nt][c], s);
-            a2[nt][c] += __shfl_xor_sync(0xffffffffu, a2[nt][c], s);
           }
           const float over = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];
           // this lane has channels [D/8 g, D/8 (g + 1)) of the row
           float y[D / 8];
 #pragma unroll
           for (int x = 0; x < D / 16; ++x) {
-            y[2 * x] = (fmaf(acc[nt][x][c], 16777216.f, -8.f * a2[nt][c]) + a1[nt][c]) * over;
-            y[2 * x + 1] = (fmaf(acc[nt][x][c + 2], 1048576.f, -8.f * a2[nt][c]) + a1[nt][c]) * over;
+            y[2 * x] = (fmaf(acc[nt][x][c], 16777216.f, -8.f * ones[nt][c]) + a1[nt][c]) * over;
+            y[2 * x + 1] = (fmaf(acc[nt][x][c + 2], 1048576.f, -8.f * ones[nt][c]) + a1[nt][c]) * over;
           }
-          const int r = nt * 8 + 2 * t + c, row = here.chunk * kRows + r;
-          if (row >= here.s.n * p.group) continue;
+          const int r = nt * 8 + 2 * t + c, row = at.chunk * kRows + r;
+          if (row >= at.s.n * p.group) continue;
           if (all) {
-            uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(here.s.first + row / p.group) * p.q_heads +
-                                         here.head * p.group + row % p.group) * D + D / 8 * g);
+            uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(at.s.first + row / p.group) * p.q_heads +
+                                         at.head * p.group + row % p.group) * D + D / 8 * g);
 #pragma unroll
             for (int x = 0; x < D / 64; ++x)
               *reinterpret_cast<uint4*>(dst + 16 * x) =
@@ -598,18 +620,25 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
             if (g == 0) part[kRows * D + r] = top[nt][c], part[kRows * D + kRows + r] = l[nt][c];
           }
         }
+      if (i < count) next_item<kRows>(p, at);
     }
   }
   __syncthreads();
   if (*abort_flag) return;
 
   // --- parts of this CTA's warps, joined -------------------------------------
-  const int64_t cta_quota = quota * Cfg::kWarps;
-  const int64_t cta_end = min(cta_begin + cta_quota, total);
   auto part_of = [&](int s) -> const float* {
     return s & 1 ? reinterpret_cast<const float*>(smem + (s >> 1) * kDepth * kBytes)
                  : reinterpret_cast<const float*>(smem + Cfg::kOffParts) + (s >> 1) * kPart;
   };
+  auto store = [&](const Segment& seg, const Span& sp, int r, int c, const float4& x) {
+    const int row = seg.chunk * kRows + r;
+    *reinterpret_cast<uint2*>(
+        p.out + 2 * ((static_cast<int64_t>(sp.first + row / p.group) * p.q_heads + seg.head * p.group +
+                      row % p.group) * D + c)) = make_uint2(T::down(x.x, x.y), T::down(x.z, x.w));
+  };
+  int open[2] = {-1, -1};  // segments of the items that other CTAs share: from before, into the next
+#pragma unroll 1
   for (int s0 = 0; s0 < 2 * Cfg::kWarps;) {
     const Segment seg = segments[s0];
     if (seg.begin < 0) {
@@ -621,68 +650,123 @@ __global__ void __launch_bounds__(256, DecodeCfg<D, NT>::kCtas)
     const Span sp = span_of<kRows>(p, seg.b);
     const int rows = min(kRows, sp.n * p.group - seg.chunk * kRows);
     const bool all = seg.begin >= cta_begin && seg.end <= cta_end;
-    const int c0 = static_cast<int>(seg.begin / cta_quota), c1 = static_cast<int>((seg.end - 1) / cta_quota);
-    float* to = p.partials + (2ll * blockIdx.x + (seg.begin < cta_begin ? 0 : 1)) * kPart;
-    auto store = [&](int i, float lo, float hi) {
-      const int row = seg.chunk * kRows + i / (D / 2);
-      *reinterpret_cast<uint32_t*>(
-          p.out + 2 * ((static_cast<int64_t>(sp.first + row / p.group) * p.q_heads + seg.head * p.group +
-                        row % p.group) * D + 2 * (i % (D / 2)))) = T::down(lo, hi);
-    };
-    for (int i = threadIdx.x; i < rows * (D / 2); i += 256) {
-      const int r = i / (D / 2);
-      float m = kLowest;
+    const int side = seg.begin < cta_begin ? 0 : 1;
+    float* to = p.partials + (2ll * blockIdx.x + side) * kPart;
+    if (!all) open[side] = s0;
+#pragma unroll 1
+    for (int r = threadIdx.x; r < rows; r += Cfg::kThreads) {
+      float m = kLowest, sum = 0.f;
+#pragma unroll 1
       for (int s = s0; s < s1; ++s)
         if (segments[s].begin >= 0) m = fmaxf(m, part_of(s)[kRows * D + r]);
-      float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll 1
       for (int s = s0; s < s1; ++s) {
         if (segments[s].begin < 0) continue;
-        const float* part = part_of(s);
-        const float w = part[kRows * D + kRows + r] * exp2_approx(part[kRows * D + r] - m);
-        const float2 v = *reinterpret_cast<const float2*>(part + 2 * i);
+        const float w = part_of(s)[kRows * D + kRows + r] * exp2_approx(part_of(s)[kRows * D + r] - m);
+        join_w[s * kRows + r] = w;
         sum += w;
-        x = fmaf(w, v.x, x);
-        y = fmaf(w, v.y, y);
       }
       const float over = sum == 0.f ? 0.f : 1.f / sum;
-      if (all) {
-        store(i, x * over, y * over);
-      } else {
-        *reinterpret_cast<float2*>(to + 2 * i) = make_float2(x * over, y * over);
-        if (i % (D / 2) == 0) to[kRows * D + r] = m, to[kRows * D + kRows + r] = sum;
-      }
+#pragma unroll 1
+      for (int s = s0; s < s1; ++s) join_w[s * kRows + r] *= over;
+      if (!all) to[kRows * D + r] = m, to[kRows * D + kRows + r] = sum;
     }
-    if (!all) {
-      // the last CTA to bring its part joins them, in CTA order
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) *last_flag = atomicAdd(p.counters + c0, 1) == c1 - c0;
-      __syncthreads();
-      if (*last_flag) {
-        __threadfence();
-        auto from = [&](int c) -> const float* {
-          return p.partials + (2ll * c + (c == c0 ? 1 : 0)) * kPart;
-        };
-        for (int i = threadIdx.x; i < rows * (D / 2); i += 256) {
-          const int r = i / (D / 2);
-          float m = kLowest;
-          for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(from(c) + kRows * D + r));
-          float sum = 0.f, x = 0.f, y = 0.f;
-          for (int c = c0; c <= c1; ++c) {
-            const float w = __ldcg(from(c) + kRows * D + kRows + r) * exp2_approx(__ldcg(from(c) + kRows * D + r) - m);
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(from(c) + 2 * i));
-            sum += w;
-            x = fmaf(w, v.x, x);
-            y = fmaf(w, v.y, y);
-          }
-          const float over = sum == 0.f ? 0.f : 1.f / sum;
-          store(i, x * over, y * over);
-        }
-        if (threadIdx.x == 0) p.counters[c0] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < rows * (D / 4); i += Cfg::kThreads) {
+      const int r = i / (D / 4);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int s = s0; s < s1; ++s) {
+        if (segments[s].begin < 0) continue;
+        const float w = join_w[s * kRows + r];
+        const float4 v = *reinterpret_cast<const float4*>(part_of(s) + 4 * i);
+        x = make_float4(fmaf(w, v.x, x.x), fmaf(w, v.y, x.y), fmaf(w, v.z, x.z), fmaf(w, v.w, x.w));
       }
-      __syncthreads();
+      if (all) {
+        store(seg, sp, r, 4 * (i % (D / 4)), x);
+      } else {
+        *reinterpret_cast<float4*>(to + 4 * i) = x;
+      }
     }
     s0 = s1;
+  }
+  if (open[0] < 0 && open[1] < 0) return;
+
+  // --- items of several CTAs: the last to bring its part joins them ----------
+  __threadfence();
+  __syncthreads();
+  float* weights = reinterpret_cast<float*>(smem);               // [ctas][rows]: the rings are done with
+  float4* sheets = reinterpret_cast<float4*>(smem + Cfg::kRing); // [sheets][rows * D / 4]: so are the parts
+  static_assert(Cfg::kThreads * 16 <= Cfg::kWarps * kPart * 4, "sheets");
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    if (open[side] < 0) continue;
+    const Segment seg = segments[open[side]];
+    const int c0 = seg.begin / quota, c1 = (seg.end - 1) / quota;
+    if (threadIdx.x == 0) *last_flag = atomicAdd(p.counters + c0, 1) == c1 - c0;
+    __syncthreads();
+    if (*last_flag) {
+      __threadfence();
+      if (threadIdx.x == 0) p.counters[c0] = 0;
+      const Span sp = span_of<kRows>(p, seg.b);
+      const int rows = min(kRows, sp.n * p.group - seg.chunk * kRows), ctas = c1 - c0 + 1;
+      auto from = [&](int c) -> const float* {
+        return p.partials + (2ll * (c0 + c) + (c == 0 ? 1 : 0)) * kPart;
+      };
+#pragma unroll 1
+      for (int r = warp; r < rows; r += Cfg::kWarps) {  // a warp a row
+        float m = kLowest, sum = 0.f;
+#pragma unroll 1
+        for (int c = lane; c < ctas; c += 32) m = fmaxf(m, __ldcg(from(c) + kRows * D + r));
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+#pragma unroll 1
+        for (int c = lane; c < ctas; c += 32) {
+          const float w = __ldcg(from(c) + kRows * D + kRows + r) * exp2_approx(__ldcg(from(c) + kRows * D + r) - m);
+          weights[c * kRows + r] = w;
+          sum += w;
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        const float over = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+        for (int c = lane; c < ctas; c += 32) weights[c * kRows + r] *= over;
+      }
+      __syncthreads();
+      // few rows: several sheets of threads, each over some of the CTAs
+      const int sheet = rows * (D / 4), count = max(1, min(256 / sheet, ctas));
+#pragma unroll 1
+      for (int i0 = threadIdx.x; i0 < count * sheet; i0 += Cfg::kThreads) {
+        const int i = i0 % sheet, r = i / (D / 4);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = i0 / sheet; c < ctas; c += count) {
+          const float w = weights[c * kRows + r];
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(from(c) + 4 * i));
+          x = make_float4(fmaf(w, v.x, x.x), fmaf(w, v.y, x.y), fmaf(w, v.z, x.z), fmaf(w, v.w, x.w));
+        }
+        if (count == 1) {
+          store(seg, sp, r, 4 * (i % (D / 4)), x);
+        } else {
+          sheets[i0] = x;
+        }
+      }
+      if (count > 1) {
+        __syncthreads();
+#pragma unroll 1
+        for (int i = threadIdx.x; i < sheet; i += Cfg::kThreads) {
+          float4 x = sheets[i];
+#pragma unroll 1
+          for (int c = 1; c < count; ++c) {
+            const float4 v = sheets[c * sheet + i];
+            x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+          }
+          store(seg, sp, i / (D / 4), 4 * (i % (D / 4)), x);
+        }
+      }
+    }
+    __syncthreads();
   }
 }
 
