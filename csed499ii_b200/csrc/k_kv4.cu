@@ -71,20 +71,19 @@ constexpr int kFewRows = 32;
 // Counters of the decode kernel's grid, then its parts.
 constexpr size_t kCounterBytes = 4096;
 size_t workspace_bytes(int sms) {
-  return kCounterBytes + static_cast<size_t>(sms) * 2 * DecodeCfg<128, 2>::kPart * 2 * sizeof(float);
+  return kCounterBytes + static_cast<size_t>(sms) * 2 * DecodeCfg<128, 2>::kPart * sizeof(float);
 }
 
 template <class T, int D, int NT>
 int launch_decode(DecodeParams p, int64_t most, int sms, int dev, cudaStream_t stream) {
   using Cfg = DecodeCfg<D, NT>;
-  static_assert(Cfg::kCtas * Cfg::kPart <= 2 * DecodeCfg<128, 2>::kPart, "workspace");
   const int bad = allow_smem<kv4_decode_kernel<T, D, NT>>(dev, Cfg::kSmem);
   if (bad) return bad;
-  // The kernel keeps a sum per request in shared memory, and counts tiles in 32
+  // The kernel keeps a sum per request in shared memory, and counts steps in 32
   // bits: larger batches go in slices.
-  const int64_t tiles = static_cast<int64_t>(p.width) * (p.cache.page_size / kTile) *
+  const int64_t steps = (static_cast<int64_t>(p.width) * p.cache.page_size / kStepTokens + 1) *
                         p.cache.heads * ((most + Cfg::kRows - 1) / Cfg::kRows);  // of a request, at most
-  const int64_t fit = 0x7fffffffll / (tiles > 0 ? tiles : 1);
+  const int64_t fit = 0x3fffffffll / steps;
   if (fit < 1) return SM100_MARLIN_ERR_PROB_SHAPE;
   const int slice = static_cast<int>(fit < kDecodeBatch ? fit : kDecodeBatch), batch = p.batch;
   int done = 0;
@@ -92,7 +91,7 @@ int launch_decode(DecodeParams p, int64_t most, int sms, int dev, cudaStream_t s
     const int n = batch - done < slice ? batch - done : slice;
     p.batch = n;
     p.pad = done + n == batch;
-    kv4_decode_kernel<T, D, NT><<<sms * Cfg::kCtas, Cfg::kThreads, Cfg::kSmem, stream>>>(p);
+    kv4_decode_kernel<T, D, NT><<<sms, Cfg::kThreads, Cfg::kSmem, stream>>>(p);
     p.lens += n;
     p.tables += n * p.table_stride;
     p.row0 += n;

@@ -25,12 +25,12 @@
 // both exact in the product; for bf16 queries the codes are OR-ed into the
 // mantissa of 128 (128 + c) and the offset term takes the 128 back.
 //
-// Work is dealt in tiles: all tiles of all (request, head) pairs in a row, cut
-// into equal runs, one per warp, whatever the lengths are.  A warp streams its
-// run through its own ring of bulk copies, over the borders of pairs; what it
-// has of a pair that other warps share is joined in the CTA through shared
-// memory, and between CTAs through the workspace by whichever finishes last,
-// in CTA order, so results do not depend on timing.
+// Work is dealt in steps of two tiles: all steps of all (request, head) pairs in
+// a row, cut into equal runs, one per warp, whatever the lengths are.  A warp
+// streams its run through its own ring of bulk copies, over the borders of
+// pairs; what it has of a pair that other warps share is joined in the CTA
+// through shared memory, and between CTAs through the workspace by whichever
+// finishes last, in CTA order, so results do not depend on timing.
 #pragma once
 
 #include <math_constants.h>
@@ -40,8 +40,10 @@
 namespace sm100 {
 namespace kv4 {
 
-constexpr int kDecodeBatch = 1024;  // requests of a launch: 4 bytes of shared memory each
-constexpr int kLeast = 16;          // tiles of a CTA: fewer are not worth sharing an item
+constexpr int kDecodeBatch = 1024;    // requests of a launch: 4 bytes of shared memory each
+constexpr int kStepTokens = 2 * kTile;  // a step: two tiles
+constexpr int kLeastSteps = 16;         // of a CTA: fewer are not worth sharing an item
+constexpr int kRoundSteps = 32;         // a CTA takes up to so many more to end with an item
 
 struct DecodeParams {
   Cache cache;
@@ -70,26 +72,27 @@ struct DecodeParams {
 
 template <int D, int NT>
 struct DecodeCfg {
-  static constexpr int kWarps = 8;
+  // One CTA an SM: the fewer parts an item has, the sooner they are joined.
+  static constexpr int kWarps = D == 128 && NT == 2 ? 8 : 16;  // 252 registers, 128
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kDepth = 4;             // tiles in a warp's ring
+  static constexpr int kDepth = 2;             // steps in a warp's ring
+  static constexpr int kSlot = 2 * tile_bytes(D);
   static constexpr int kRows = 8 * NT;         // query rows of an item
   static constexpr int kPart = kRows * (D + 2);  // floats: results, maxima, sums
-  static constexpr int kRing = kWarps * kDepth * tile_bytes(D);
+  static constexpr int kRing = kWarps * kDepth * kSlot;
   static constexpr int kOffParts = kRing;
-  static constexpr int kOffPre = kOffParts + kWarps * kPart * 4;
+  static constexpr int kOffTokens = kOffParts + kWarps * kPart * 4;
+  static constexpr int kOffPre = kOffTokens + kWarps * 32 * 20;
   static constexpr int kOffMisc = kOffPre + kDecodeBatch * 4;
-  static constexpr int kMisc = 1424 + 64 * kRows;
-  static constexpr int kSmem = kOffMisc + kMisc;
-  static constexpr int kCtas = kSmem <= 113 * 1024 ? 2 : 1;  // of an SM
+  static constexpr int kSmem = kOffMisc + 1280;
   // a warp's last part takes the place of its ring
-  static_assert(kPart * 4 <= kDepth * tile_bytes(D), "part does not fit the ring");
+  static_assert(kPart * 4 <= kDepth * kSlot, "part does not fit the ring");
 };
 
 // What a launch knows about one request.
 struct Span {
   int first, n, len;    // query rows, tokens
-  int tile0, tiles;     // that any of its rows sees
+  int step0, steps;     // that any of its rows sees
   int chunks;           // of query rows
 };
 
@@ -102,17 +105,17 @@ __device__ __forceinline__ Span span_of(const DecodeParams& p, int b) {
   s.len = static_cast<int>(min(static_cast<int64_t>(p.lens[b]), room));
   const int64_t rows = static_cast<int64_t>(s.n) * p.group;
   const bool mine = s.n > 0 && rows <= p.most;
-  s.chunks = mine ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
+  s.chunks = mine ? (static_cast<int>(rows) + ROWS - 1) / ROWS : 0;
   const int from = p.window && s.len - s.n >= p.window ? s.len - s.n - p.window + 1 : 0;
-  s.tile0 = from / kTile;
-  s.tiles = mine && s.len > 0 ? (s.len + kTile - 1) / kTile - s.tile0 : 0;
+  s.step0 = from / kStepTokens;
+  s.steps = mine && s.len > 0 ? (s.len - 1) / kStepTokens + 1 - s.step0 : 0;
   return s;
 }
 
-// One item (a request, a key/value head, kRows of its query rows) and a tile.
+// One item (a request, a key/value head, ROWS of its query rows) and a step.
 struct Walk {
   Span s;
-  int b, head, chunk, tile;  // tile of the request
+  int b, head, chunk, step;  // step of the request
 };
 
 template <int ROWS>
@@ -131,15 +134,15 @@ __device__ __forceinline__ Walk walk_to(const DecodeParams& p, const int* pre, i
   w.b = lo;
   w.s = span_of<ROWS>(p, lo);
   const int off = at - (lo ? pre[lo - 1] : 0);
-  const int tiles = max(w.s.tiles, 1);
-  const int item = off / tiles;
-  w.tile = w.s.tile0 + off - item * tiles;
+  const int steps = max(w.s.steps, 1);
+  const int item = off / steps;
+  w.step = w.s.step0 + off - item * steps;
   w.head = item / max(w.s.chunks, 1);
   w.chunk = item - w.head * max(w.s.chunks, 1);
   return w;
 }
 
-// To the first tile of the next item; only called while there is one.
+// To the first step of the next item; only called while there is one.
 template <int ROWS>
 __device__ __forceinline__ void next_item(const DecodeParams& p, Walk& w) {
   if (++w.chunk == w.s.chunks) {
@@ -148,10 +151,10 @@ __device__ __forceinline__ void next_item(const DecodeParams& p, Walk& w) {
       w.head = 0;
       do {
         w.s = span_of<ROWS>(p, ++w.b);
-      } while (w.s.tiles == 0 && w.b + 1 < p.batch);
+      } while (w.s.steps == 0 && w.b + 1 < p.batch);
     }
   }
-  w.tile = w.s.tile0;
+  w.step = w.s.step0;
 }
 
 template <bool BF16>
@@ -167,6 +170,23 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
         "{%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+// The same with a fresh accumulator.
+template <bool BF16>
+__device__ __forceinline__ void mma_16816_z(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
   }
 }
 
@@ -223,63 +243,114 @@ __device__ __forceinline__ ValueRow value_row(float2 pair) {
   return r;
 }
 
-// A part of an item, or all of it: results (already divided by the sum), the
-// running maximum of the scores (times log2 e) and the sum of the weights.
+// What there is of an item in one place: results (already divided by the sum),
+// the running maximum of the weights' arguments and the sum of the weights.
 struct Segment {
-  int begin, end;  // the item's place in the row of all tiles; begin < 0: none
+  int begin, end;        // the item's place in the row of all steps; begin < 0: none
   int b, head, chunk;
 };
 
 constexpr float kLowest = -3.0e38f;
 
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
+  return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+  return x;
+}
+
+// Channels [N lane, N (lane + 1)) of a row.
+template <int N>
+struct Slice {
+  float x[N];
+  __device__ __forceinline__ void add(float w, const float* row, int lane) {
+    if constexpr (N == 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(row) + lane);
+      x[0] = fmaf(w, v.x, x[0]), x[1] = fmaf(w, v.y, x[1]);
+      x[2] = fmaf(w, v.z, x[2]), x[3] = fmaf(w, v.w, x[3]);
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(row) + lane);
+      x[0] = fmaf(w, v.x, x[0]), x[1] = fmaf(w, v.y, x[1]);
+    }
+  }
+  __device__ __forceinline__ void add_shared(float w, const float* row, int lane) {
+    if constexpr (N == 4) {
+      const float4 v = reinterpret_cast<const float4*>(row)[lane];
+      x[0] = fmaf(w, v.x, x[0]), x[1] = fmaf(w, v.y, x[1]);
+      x[2] = fmaf(w, v.z, x[2]), x[3] = fmaf(w, v.w, x[3]);
+    } else {
+      const float2 v = reinterpret_cast<const float2*>(row)[lane];
+      x[0] = fmaf(w, v.x, x[0]), x[1] = fmaf(w, v.y, x[1]);
+    }
+  }
+  __device__ __forceinline__ void put(float* row, int lane) const {
+    if constexpr (N == 4) {
+      reinterpret_cast<float4*>(row)[lane] = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      reinterpret_cast<float2*>(row)[lane] = make_float2(x[0], x[1]);
+    }
+  }
+};
+
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::kCtas)
+__global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
     kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   using Cfg = DecodeCfg<D, NT>;
-  constexpr int kRows = Cfg::kRows, kPart = Cfg::kPart, kDepth = Cfg::kDepth, kBytes = tile_bytes(D);
+  constexpr int kWarps = Cfg::kWarps, kRows = Cfg::kRows, kPart = Cfg::kPart, kDepth = Cfg::kDepth;
+  constexpr int kBytes = tile_bytes(D), kSlot = Cfg::kSlot;
   constexpr int kWords = D / 32;  // code words of a lane in a row of keys
   constexpr bool kBf = T::kBf16;
   extern __shared__ __align__(128) uint8_t smem[];
   int* pre = reinterpret_cast<int*>(smem + Cfg::kOffPre);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffMisc);            // [warps][depth]
-  int* there = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 512);               // [warps][depth]
-  Segment* segments = reinterpret_cast<Segment*>(smem + Cfg::kOffMisc + 640);    // [warps][2]
-  int* sums = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 1280);               // [warps]
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kOffMisc + 1408);
+  int* there = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 256);               // [warps][depth]
+  Segment* segments = reinterpret_cast<Segment*>(smem + Cfg::kOffMisc + 384);    // [warps][2]
+  int* sums = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 1024);               // [3][warps]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kOffMisc + 1216);
   volatile int* drain_flag = abort_flag + 1;
-  int* last_flag = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 1416);
-  float* join_w = reinterpret_cast<float*>(smem + Cfg::kOffMisc + 1424);         // [2 warps][rows]
-  static_assert(sizeof(Segment) * 16 <= 640 && 1424 + 4 * 16 * kRows <= Cfg::kMisc, "shared memory");
+  int* last_flag = reinterpret_cast<int*>(smem + Cfg::kOffMisc + 1224);          // [2]
+  static_assert(sizeof(Segment) * 32 <= 640, "shared memory");
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
 
   if (lane < kDepth) mbar_init(smem_addr(bars + kDepth * warp + lane), 1);
-  if (lane == 0) segments[2 * warp].begin = segments[2 * warp + 1].begin = -1;
+  if (lane < 2) segments[2 * warp + lane].begin = -1;
   if (threadIdx.x == 0) *abort_flag = *drain_flag = 0;
   fence_mbar_init();
 
-  // --- the row of all tiles: where each request's end is -------------------
-  int total = 0;  // the host keeps it below 2^31
+  // --- the row of all steps: where each request's end is -------------------
+  int total = 0;  // the host keeps it below 2^30
+  int longest = 0, shortest = 0x7fffffff;  // items
   for (int b0 = 0; b0 < p.batch; b0 += Cfg::kThreads) {
     const int b = b0 + threadIdx.x;
-    int x = 0;
+    int x = 0, most = 0, least = 0x7fffffff;
     if (b < p.batch) {
       const Span s = span_of<kRows>(p, b);
-      x = p.cache.heads * s.chunks * s.tiles;
+      x = p.cache.heads * s.chunks * s.steps;
+      most = s.steps;
+      if (x > 0) least = s.steps;
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, i);
       if (lane >= i) x += y;
     }
-    if (lane == 31) sums[warp] = x;
+    if (lane == 31) sums[warp] = x, sums[kWarps + warp] = most, sums[2 * kWarps + warp] = least;
     __syncthreads();
     int all = 0;
 #pragma unroll
-    for (int i = 0; i < Cfg::kWarps; ++i) {
+    for (int i = 0; i < kWarps; ++i) {
       if (i == warp) x += all;
       all += sums[i];
+      longest = max(longest, sums[kWarps + i]);
+      shortest = min(shortest, sums[2 * kWarps + i]);
     }
     if (b < p.batch) pre[b] = total + x;
     total += all;
@@ -289,74 +360,113 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
   // --- rows that see nothing ------------------------------------------------
   {
     const int64_t row_bytes = 2ll * p.q_heads * D;
+#pragma unroll 1
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
       if (pre[b] != (b ? pre[b - 1] : 0)) continue;
       const Span s = span_of<kRows>(p, b);
       if (s.chunks == 0) continue;
+#pragma unroll 1
       for (int64_t i = 16 * threadIdx.x; i < s.n * row_bytes; i += 16 * Cfg::kThreads)
         *reinterpret_cast<uint4*>(p.out + s.first * row_bytes + i) = make_uint4(0, 0, 0, 0);
     }
     const int end = !p.starts || !p.pad ? p.rows : p.batch ? max(p.starts[p.batch], 0) : 0;
+#pragma unroll 1
     for (int row = min(end, p.rows) + blockIdx.x; row < p.rows; row += gridDim.x)
+#pragma unroll 1
       for (int64_t i = 16 * threadIdx.x; i < row_bytes; i += 16 * Cfg::kThreads)
         *reinterpret_cast<uint4*>(p.out + row * row_bytes + i) = make_uint4(0, 0, 0, 0);
   }
 
-  const int quota = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kLeast);  // of a CTA
-  if (static_cast<int64_t>(quota) * blockIdx.x >= total) return;
-  const int cta_begin = quota * blockIdx.x;
-  const int cta_end = min(cta_begin + quota, total);
-  const int share = (cta_end - cta_begin + Cfg::kWarps - 1) / Cfg::kWarps;
+  // --- this CTA's steps -----------------------------------------------------
+  // Joining an item over CTAs costs about as much as kRoundSteps steps of one.
+  // Where all items are as long, a CTA's share is rounded up to whole ones if
+  // that takes no more, or else every item gets the same CTAs to itself.
+  const int ctas = gridDim.x, cta = blockIdx.x;
+  int quota = (total + ctas - 1) / ctas, per_item = 0;  // CTAs that an item has to itself
+  const bool even = longest == shortest;
+  const int whole = even ? (quota + longest - 1) / longest * longest : 0;
+  if (even && whole - quota <= kRoundSteps) {
+    quota = whole;
+  } else if (even && total / longest <= ctas) {
+    quota = max((longest - 1) / (ctas / (total / longest)) + 1, kLeastSteps);
+    per_item = (longest - 1) / quota + 1;
+  } else {
+    quota = max(quota, kLeastSteps);
+  }
+  if (per_item ? cta / per_item >= total / longest : static_cast<int64_t>(quota) * cta >= total) return;
+  const int cta_begin = per_item ? cta / per_item * longest + cta % per_item * quota : quota * cta;
+  const int cta_end = min(cta_begin + quota, per_item ? (cta / per_item + 1) * longest : total);
+  // first and last CTA of the item in [begin, end)
+  auto first_cta = [&](int begin) { return per_item ? begin / longest * per_item : begin / quota; };
+  auto last_cta = [&](int begin, int end) {
+    return per_item ? begin / longest * per_item + per_item - 1 : (end - 1) / quota;
+  };
+  const int share = (cta_end - cta_begin + kWarps - 1) / kWarps;
   const int begin = min(cta_begin + share * warp, cta_end);
   const int count = min(begin + share, cta_end) - begin;
 
   // --- this warp's run ------------------------------------------------------
   if (count > 0) {
-    const uint32_t ring = smem_addr(smem) + warp * kDepth * kBytes;
+    const uint32_t ring = smem_addr(smem) + warp * kDepth * kSlot;
     const uint32_t full = smem_addr(bars + kDepth * warp);
+    // of each token of a step: key scale, key offset, log2 of the value scale
+    float* tokens = reinterpret_cast<float*>(smem + Cfg::kOffTokens) + warp * 160;
+    float2* token_sums = reinterpret_cast<float2*>(tokens + 96);  // 1 / value scale, value at code 8 / scale
     Walk at = walk_to<kRows>(p, pre, begin);
+    // the first queries are on their way while the first pages are looked up
+    {
+      const int r = at.chunk * kRows + g;
+      if (r < at.s.n * p.group)
+        prefetch_l1(p.q + 2 * (p.q_row * (at.s.first + r / p.group) +
+                               p.q_head * (at.head * p.group + r % p.group) + t * (D / 4)));
+    }
 
-    // The copies run ahead of the work: `in` is the item of the next one, and
-    // a page's number is looked up a page early.
+    // The copies run ahead of the work: `in` is the place of the next one, and
+    // its pages are looked up a step early.
     Walk in = at;
     const int per_page = p.cache.page_size / kTile;
     const uint64_t policy = policy_evict_first();
-    int issued = 0, entry, nth, page, next;  // nth tile of the page
+    int issued = 0, entry, nth, page0, page1;  // nth tile of the table's entry
+    auto look_up = [&](bool both) {
+      const int* table = p.tables + p.table_stride * in.b + entry;
+      if (both) page0 = table[0];
+      page1 = page0;
+      if (nth + 1 == per_page) page1 = (2 * in.step + 1) * kTile < in.s.len ? table[1] : -1;
+    };
     auto start = [&]() {
-      entry = in.tile / per_page;
-      nth = in.tile - entry * per_page;
-      const int* table = p.tables + p.table_stride * in.b;
-      page = table[entry];
-      next = entry + 1 < p.width ? table[entry + 1] : -1;
+      entry = 2 * in.step / per_page;
+      nth = 2 * in.step - entry * per_page;
+      look_up(true);
     };
     auto issue = [&]() {
       const int slot = issued % kDepth;
-      const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.pages);
       if (lane == 0) {
-        there[warp * kDepth + slot] = ok;
-        if (ok) {
-          mbar_arrive_expect_tx(full + 8 * slot, kBytes);
-          bulk_g2s(ring + slot * kBytes, p.cache.page_tiles<D>(page, in.head) + nth * kBytes, kBytes,
-                   full + 8 * slot, policy);
+        const bool ok0 = static_cast<uint32_t>(page0) < static_cast<uint32_t>(p.cache.pages);
+        const bool ok1 = static_cast<uint32_t>(page1) < static_cast<uint32_t>(p.cache.pages);
+        const uint32_t dst = ring + slot * kSlot, bar = full + 8 * slot;
+        there[warp * kDepth + slot] = (ok0 ? 1 : 0) | (ok1 ? 2 : 0);
+        if (nth + 1 < per_page && ok0) {  // both tiles of one page
+          mbar_arrive_expect_tx(bar, 2 * kBytes);
+          bulk_g2s(dst, p.cache.page_tiles<D>(page0, in.head) + nth * kBytes, 2 * kBytes, bar, policy);
+        } else if (ok0 || ok1) {
+          mbar_arrive_expect_tx(bar, (ok0 ? kBytes : 0) + (ok1 ? kBytes : 0));
+          if (ok0) bulk_g2s(dst, p.cache.page_tiles<D>(page0, in.head) + nth * kBytes, kBytes, bar, policy);
+          if (ok1) bulk_g2s(dst + kBytes, p.cache.page_tiles<D>(page1, in.head), kBytes, bar, policy);
         } else {
-          mbar_arrive(full + 8 * slot);
+          mbar_arrive(bar);
         }
       }
       if (++issued == count) return;
-      if (++in.tile == in.s.tile0 + in.s.tiles) {
+      if (++in.step == in.s.step0 + in.s.steps) {
         next_item<kRows>(p, in);
         start();
-      } else if (++nth == per_page) {
-        nth = 0;
-        ++entry;
-        page = next;
-        next = entry + 1 < p.width ? p.tables[p.table_stride * in.b + entry + 1] : -1;
+      } else {
+        nth += 2;
+        const int old = entry;
+        while (nth >= per_page) nth -= per_page, ++entry;
+        look_up(entry != old);
       }
     };
-    // the first queries are on their way while the first pages are looked up
-    if (at.chunk * kRows + (lane >> 2) < at.s.n * p.group)
-      prefetch_l1(p.q + 2 * (p.q_row * (at.s.first + (at.chunk * kRows + (lane >> 2)) / p.group) +
-                             p.q_head * (at.head * p.group + (at.chunk * kRows + (lane >> 2)) % p.group) + t * (D / 4)));
     start();
     for (int i = 0; i < kDepth && issued < count; ++i) issue();
 
@@ -367,81 +477,93 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
     float top[NT][2], l[NT][2], a1[NT][2], ones[NT][4];
     const float c2 = p.scale * kLog2e;
     const float c1 = kBf ? c2 : c2 * 16777216.f;
-    int i = 0;  // tiles done
+    int i = 0;  // steps done
     while (i < count) {
-      const int item_begin = begin + i - (at.tile - at.s.tile0), item_end = item_begin + at.s.tiles;
-      const int stop = min(at.s.tile0 + at.s.tiles, at.tile + count - i);
-      {
+      const int item_begin = begin + i - (at.step - at.s.step0), item_end = item_begin + at.s.steps;
+      const int stop = min(at.s.step0 + at.s.steps, at.step + count - i);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int r = at.chunk * kRows + nt * 8 + g;
-          const int token = r / p.group, h = at.head * p.group + r % p.group;
-          float sum = 0.f;
-          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) +
-                                p.q_row * (at.s.first + token) + p.q_head * h + t * (D / 4);
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = at.chunk * kRows + nt * 8 + g;
+        const int token = r / p.group, h = at.head * p.group + r - token * p.group;
+        float sum = 0.f;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) +
+                              p.q_row * (at.s.first + token) + p.q_head * h + t * (D / 4);
 #pragma unroll
-          for (int w = 0; w < kWords; ++w) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (token < at.s.n) {
-              if (p.q_aligned) {
-                x = *reinterpret_cast<const uint4*>(src + 8 * w);
-              } else {
-                uint32_t y[4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z)
-                  y[z] = src[8 * w + 2 * z] | static_cast<uint32_t>(src[8 * w + 2 * z + 1]) << 16;
-                x = make_uint4(y[0], y[1], y[2], y[3]);
-              }
+        for (int w = 0; w < kWords; ++w) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (token < at.s.n) {
+            if (p.q_aligned) {
+              x = *reinterpret_cast<const uint4*>(src + 8 * w);
+            } else {
+              x = make_uint4(src[8 * w] | src[8 * w + 1] << 16, src[8 * w + 2] | src[8 * w + 3] << 16,
+                             src[8 * w + 4] | src[8 * w + 5] << 16, src[8 * w + 6] | src[8 * w + 7] << 16);
             }
-            qe[nt][w][0] = prmt_b32(x.x, x.z, 0x5410);
-            qe[nt][w][1] = prmt_b32(x.y, x.w, 0x5410);
-            qo[nt][w][0] = prmt_b32(x.x, x.z, 0x7632);
-            qo[nt][w][1] = prmt_b32(x.y, x.w, 0x7632);
-            const float2 f0 = T::up(x.x), f1 = T::up(x.y), f2 = T::up(x.z), f3 = T::up(x.w);
-            sum += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
           }
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            sumq[nt][c] = __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
-            place[nt][c] = at.s.len - at.s.n + (at.chunk * kRows + nt * 8 + 2 * t + c) / p.group;
-            top[nt][c] = kLowest;
-            l[nt][c] = a1[nt][c] = ones[nt][c] = ones[nt][c + 2] = 0.f;
-          }
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[nt][x][c] = 0.f;
+          qe[nt][w][0] = prmt_b32(x.x, x.z, 0x5410);
+          qe[nt][w][1] = prmt_b32(x.y, x.w, 0x5410);
+          qo[nt][w][0] = prmt_b32(x.x, x.z, 0x7632);
+          qo[nt][w][1] = prmt_b32(x.y, x.w, 0x7632);
+          const float2 f0 = T::up(x.x), f1 = T::up(x.y), f2 = T::up(x.z), f3 = T::up(x.w);
+          sum += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
         }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          sumq[nt][c] = __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
+          place[nt][c] = at.s.len - at.s.n + (at.chunk * kRows + nt * 8 + 2 * t + c) / p.group;
+          top[nt][c] = kLowest;
+          l[nt][c] = a1[nt][c] = ones[nt][c] = ones[nt][c + 2] = 0.f;
+        }
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[nt][x][c] = 0.f;
       }
 
       bool lost = false;
-      for (; at.tile < stop; ++at.tile, ++i) {
+      for (; at.step < stop; ++at.step, ++i) {
         const int slot = i % kDepth;
-        const uint32_t tile = ring + slot * kBytes;
+        const uint32_t data = ring + slot * kSlot;
         if (!mbar_wait_bounded(full + 8 * slot, (i / kDepth) & 1, abort_flag)) {
           lost = true;
           break;
         }
-        if (there[warp * kDepth + slot]) {
-        // scores
-        uint32_t k0[kWords], k1[kWords];
-        if constexpr (D == 128) {
-          const uint4 x = lds128(tile + 16 * lane), y = lds128(tile + 512 + 16 * lane);
-          k0[0] = x.x, k0[1] = x.y, k0[2] = x.z, k0[3] = x.w;
-          k1[0] = y.x, k1[1] = y.y, k1[2] = y.z, k1[3] = y.w;
-        } else {
-          const uint2 x = lds64(tile + 8 * lane), y = lds64(tile + 256 + 8 * lane);
-          k0[0] = x.x, k0[1] = x.y;
-          k1[0] = y.x, k1[1] = y.y;
-        }
-        const float2 kp0 = T::up(lds32(tile + off_k_pair(D, g))), kp1 = T::up(lds32(tile + off_k_pair(D, g + 8)));
-        ValueRow v0 = value_row(T::up(lds32(tile + off_v_pair(D, g))));
-        ValueRow v1 = value_row(T::up(lds32(tile + off_v_pair(D, g + 8))));
-        float x[NT][4];  // arguments of the weights
+        const int j0 = at.step * kStepTokens;
+        // Scale and offset of this lane's token, for all lanes.  A token that is
+        // not there weighs nothing, whatever lies in its place; a row of values
+        // that stands for NaN counts through its scores.
         {
-          float e[NT][4] = {}, o[NT][4] = {};
+          const uint32_t tile = data + (lane >> 4) * kBytes;
+          const float2 kp = T::up(lds32(tile + off_k_pair(D, lane & 15)));
+          const ValueRow v = value_row(T::up(lds32(tile + off_v_pair(D, lane & 15))));
+          float4 x = make_float4(kp.x * c1, (kBf ? fmaf(kp.x, -128.f, kp.y) : kp.y) * c2, v.log_s, v.inv_s);
+          float at_8 = v.at_8;
+          if (!(fabsf(at_8) <= 3.4e38f)) x.y = CUDART_NAN_F, x.w = at_8 = 0.f;
+          if (j0 + lane >= at.s.len || !(there[warp * kDepth + slot] >> (lane >> 4) & 1))
+            x = make_float4(0.f, 0.f, -CUDART_INF_F, 0.f), at_8 = 0.f;
+          tokens[lane] = x.x;
+          tokens[32 + lane] = x.y;
+          tokens[64 + lane] = x.z;
+          token_sums[lane] = make_float2(x.w, at_8);
+        }
+        __syncwarp();
+        // the arguments of the weights
+        float x[2][NT][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t tile = data + u * kBytes;
+          uint32_t k0[kWords], k1[kWords];
+          if constexpr (D == 128) {
+            const uint4 y = lds128(tile + 16 * lane), z = lds128(tile + 512 + 16 * lane);
+            k0[0] = y.x, k0[1] = y.y, k0[2] = y.z, k0[3] = y.w;
+            k1[0] = z.x, k1[1] = z.y, k1[2] = z.z, k1[3] = z.w;
+          } else {
+            const uint2 y = lds64(tile + 8 * lane), z = lds64(tile + 256 + 8 * lane);
+            k0[0] = y.x, k0[1] = y.y;
+            k1[0] = z.x, k1[1] = z.y;
+          }
+          float e[NT][4], o[NT][4];
 #pragma unroll
           for (int w = 0; w < kWords; ++w) {
             const uint32_t h0 = k0[w] >> 8, h1 = k1[w] >> 8;
@@ -451,60 +573,55 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
             const uint32_t oa2 = key_odd<kBf>(h0), oa3 = key_odd<kBf>(h1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_16816<kBf>(e[nt], ea0, ea1, ea2, ea3, qe[nt][w][0], qe[nt][w][1]);
-              mma_16816<kBf>(o[nt], oa0, oa1, oa2, oa3, qo[nt][w][0], qo[nt][w][1]);
+              if (w == 0) {
+                mma_16816_z<kBf>(e[nt], ea0, ea1, ea2, ea3, qe[nt][w][0], qe[nt][w][1]);
+                mma_16816_z<kBf>(o[nt], oa0, oa1, oa2, oa3, qo[nt][w][0], qo[nt][w][1]);
+              } else {
+                mma_16816<kBf>(e[nt], ea0, ea1, ea2, ea3, qe[nt][w][0], qe[nt][w][1]);
+                mma_16816<kBf>(o[nt], oa0, oa1, oa2, oa3, qo[nt][w][0], qo[nt][w][1]);
+              }
             }
           }
-          const float s0 = kp0.x * c1, s1 = kp1.x * c1;
-          const float z0 = (kBf ? fmaf(kp0.x, -128.f, kp0.y) : kp0.y) * c2;
-          const float z1 = (kBf ? fmaf(kp1.x, -128.f, kp1.y) : kp1.y) * c2;
+          const float3 y = make_float3(tokens[16 * u + g], tokens[32 + 16 * u + g], tokens[64 + 16 * u + g]);
+          const float3 z = make_float3(tokens[16 * u + g + 8], tokens[40 + 16 * u + g], tokens[72 + 16 * u + g]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const float dot = fmaf(o[nt][c], kBf ? 1.f : 0.0625f, e[nt][c]);
-              x[nt][c] = fmaf(c < 2 ? s0 : s1, dot,
-                              fmaf(c < 2 ? z0 : z1, sumq[nt][c & 1], c < 2 ? v0.log_s : v1.log_s));
+              x[u][nt][c] = c < 2 ? fmaf(y.x, dot, fmaf(y.y, sumq[nt][c & 1], y.z))
+                                  : fmaf(z.x, dot, fmaf(z.y, sumq[nt][c & 1], z.z));
             }
         }
-        // what of the tile each row sees; most tiles are seen whole
-        const int j0 = at.tile * kTile;
-        const bool whole = j0 + kTile <= at.s.len - at.s.n + 1 &&
-                           (p.window == 0 || at.s.len - j0 <= p.window);
-        if (!whole) {
-          // A row of values that stands for NaN counts through its scores where
-          // it is seen; where it is not, scale and offset may be anything.
-          const bool bad0 = !(fabsf(v0.at_8) <= 3.4e38f), bad1 = !(fabsf(v1.at_8) <= 3.4e38f);
+        // rows that see less than others
+        if ((at.s.n > 1 && j0 + kStepTokens > at.s.len - at.s.n + 1) || (p.window != 0 && at.s.len - j0 > p.window)) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int j = j0 + g + (c < 2 ? 0 : 8);
-              const bool seen = j <= place[nt][c & 1] && j < at.s.len &&
-                                (p.window == 0 || place[nt][c & 1] - j < p.window);
-              if (!seen) {
-                x[nt][c] = -CUDART_INF_F;
-              } else if (c < 2 ? bad0 : bad1) {
-                x[nt][c] = CUDART_NAN_F;
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const int j = j0 + 16 * u + g + (c < 2 ? 0 : 8);
+                if (j > place[nt][c & 1] || (p.window != 0 && place[nt][c & 1] - j >= p.window))
+                  x[u][nt][c] = -CUDART_INF_F;
               }
-            }
-          if (bad0 || j0 + g >= at.s.len) v0.inv_s = v0.at_8 = 0.f;
-          if (bad1 || j0 + g + 8 >= at.s.len) v1.inv_s = v1.at_8 = 0.f;
         }
         // The maximum moves only where an argument passes it by more than 8 (a
-        // factor of 256, harmless in the sums), so most tiles need no exchange.
+        // factor of 256, harmless in the sums), so most steps need no exchange.
         bool moves = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) moves |= x[nt][c] - top[nt][c & 1] > 8.f;
+          for (int c = 0; c < 2; ++c)
+            moves |= fmaxf(fmaxf(x[0][nt][c], x[0][nt][c + 2]), fmaxf(x[1][nt][c], x[1][nt][c + 2])) > top[nt][c] + 8.f;
         if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float f[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float m = fmaxf(top[nt][c], fmaxf(x[nt][c], x[nt][c + 2]));
+              float m = fmaxf(fmaxf(x[0][nt][c], x[0][nt][c + 2]), fmaxf(x[1][nt][c], x[1][nt][c + 2]));
+              m = fmaxf(top[nt][c], m);
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -523,51 +640,55 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
             }
           }
         }
-        // weights, and their sums
-        constexpr uint32_t kOnes = 0x3c003c00u;  // 1.0 twice: the sum of the rounded weights
-        uint32_t wb[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float w[4];
+        for (int u = 0; u < 2; ++u) {
+          // weights, and their sums
+          constexpr uint32_t kOnes = 0x3c003c00u;  // 1.0 twice: the sum of the rounded weights
+          const float2 s0 = token_sums[16 * u + g], s1 = token_sums[16 * u + g + 8];
+          uint32_t wb[NT][2];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            w[c] = exp2_approx(x[nt][c] - top[nt][c & 1]);
-            l[nt][c & 1] = fmaf(w[c], c < 2 ? v0.inv_s : v1.inv_s, l[nt][c & 1]);
-            a1[nt][c & 1] = fmaf(w[c], c < 2 ? v0.at_8 : v1.at_8, a1[nt][c & 1]);
-          }
-          wb[nt][0] = transpose_8x8(Half::down(w[0], w[1]));
-          wb[nt][1] = transpose_8x8(Half::down(w[2], w[3]));
-          mma_16816<false>(ones[nt], kOnes, kOnes, kOnes, kOnes, wb[nt][0], wb[nt][1]);
-        }
-        // result
-        constexpr int kOctets = D / 64;
-        uint32_t va[kOctets], vb[kOctets], vc[kOctets], vd[kOctets];  // tokens 2t, 2t+1, 2t+8, 2t+9
-        if constexpr (D == 128) {
-          const uint4 y = lds128(tile + 8 * D + 16 * lane), z = lds128(tile + 12 * D + 16 * lane);
-          va[0] = y.x, va[1] = y.y, vb[0] = y.z, vb[1] = y.w;
-          vc[0] = z.x, vc[1] = z.y, vd[0] = z.z, vd[1] = z.w;
-        } else {
-          const uint2 y = lds64(tile + 8 * D + 8 * lane), z = lds64(tile + 12 * D + 8 * lane);
-          va[0] = y.x, vb[0] = y.y;
-          vc[0] = z.x, vd[0] = z.y;
-        }
+          for (int nt = 0; nt < NT; ++nt) {
+            float w[4];
 #pragma unroll
-        for (int o = 0; o < kOctets; ++o)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t sel = half ? 0x7632 : 0x5410;
-            const uint32_t y = prmt_b32(va[o], vb[o], sel), z = prmt_b32(vc[o], vd[o], sel);
-            const uint32_t y8 = y >> 8, z8 = z >> 8;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_16816<false>(acc[nt][4 * o + 2 * half], y & 0x000f000fu, y & 0x00f000f0u,
-                               z & 0x000f000fu, z & 0x00f000f0u, wb[nt][0], wb[nt][1]);
-              mma_16816<false>(acc[nt][4 * o + 2 * half + 1], y8 & 0x000f000fu, y8 & 0x00f000f0u,
-                               z8 & 0x000f000fu, z8 & 0x00f000f0u, wb[nt][0], wb[nt][1]);
+            for (int c = 0; c < 4; ++c) {
+              w[c] = exp2_approx(x[u][nt][c] - top[nt][c & 1]);
+              l[nt][c & 1] = fmaf(w[c], c < 2 ? s0.x : s1.x, l[nt][c & 1]);
+              a1[nt][c & 1] = fmaf(w[c], c < 2 ? s0.y : s1.y, a1[nt][c & 1]);
             }
+            wb[nt][0] = transpose_8x8(Half::down(w[0], w[1]));
+            wb[nt][1] = transpose_8x8(Half::down(w[2], w[3]));
+            mma_16816<false>(ones[nt], kOnes, kOnes, kOnes, kOnes, wb[nt][0], wb[nt][1]);
           }
+          // result
+          const uint32_t tile = data + u * kBytes;
+          constexpr int kOctets = D / 64;
+          uint32_t va[kOctets], vb[kOctets], vc[kOctets], vd[kOctets];  // tokens 2t, 2t+1, 2t+8, 2t+9
+          if constexpr (D == 128) {
+            const uint4 y = lds128(tile + 8 * D + 16 * lane), z = lds128(tile + 12 * D + 16 * lane);
+            va[0] = y.x, va[1] = y.y, vb[0] = y.z, vb[1] = y.w;
+            vc[0] = z.x, vc[1] = z.y, vd[0] = z.z, vd[1] = z.w;
+          } else {
+            const uint2 y = lds64(tile + 8 * D + 8 * lane), z = lds64(tile + 12 * D + 8 * lane);
+            va[0] = y.x, vb[0] = y.y;
+            vc[0] = z.x, vd[0] = z.y;
+          }
+#pragma unroll
+          for (int o = 0; o < kOctets; ++o)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t sel = half ? 0x7632 : 0x5410;
+              const uint32_t y = prmt_b32(va[o], vb[o], sel), z = prmt_b32(vc[o], vd[o], sel);
+              const uint32_t y8 = y >> 8, z8 = z >> 8;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_16816<false>(acc[nt][4 * o + 2 * half], y & 0x000f000fu, y & 0x00f000f0u,
+                                 z & 0x000f000fu, z & 0x00f000f0u, wb[nt][0], wb[nt][1]);
+                mma_16816<false>(acc[nt][4 * o + 2 * half + 1], y8 & 0x000f000fu, y8 & 0x00f000f0u,
+                                 z8 & 0x000f000fu, z8 & 0x00f000f0u, wb[nt][0], wb[nt][1]);
+              }
+            }
         }
-        __syncwarp();  // the slot is read
+        __syncwarp();  // the slot and the tokens' numbers are read
         if (issued < count) issue();
       }
       if (lost) {
@@ -582,7 +703,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
       const bool all = item_begin >= begin && item_end <= begin + count;
       const bool is_head = item_begin < begin && i < count;
       float* part = is_head ? reinterpret_cast<float*>(smem + Cfg::kOffParts) + warp * kPart
-                            : reinterpret_cast<float*>(smem + warp * kDepth * kBytes);
+                            : reinterpret_cast<float*>(smem + warp * kDepth * kSlot);
       if (!all && lane == 0)
         segments[2 * warp + (is_head ? 0 : 1)] = {item_begin, item_end, at.b, at.head, at.chunk};
 #pragma unroll
@@ -597,16 +718,18 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
           const float over = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];
           // this lane has channels [D/8 g, D/8 (g + 1)) of the row
           float y[D / 8];
+          const float rest = fmaf(-8.f, ones[nt][c], a1[nt][c]);
 #pragma unroll
           for (int x = 0; x < D / 16; ++x) {
-            y[2 * x] = (fmaf(acc[nt][x][c], 16777216.f, -8.f * ones[nt][c]) + a1[nt][c]) * over;
-            y[2 * x + 1] = (fmaf(acc[nt][x][c + 2], 1048576.f, -8.f * ones[nt][c]) + a1[nt][c]) * over;
+            y[2 * x] = fmaf(acc[nt][x][c], 16777216.f, rest) * over;
+            y[2 * x + 1] = fmaf(acc[nt][x][c + 2], 1048576.f, rest) * over;
           }
           const int r = nt * 8 + 2 * t + c, row = at.chunk * kRows + r;
           if (row >= at.s.n * p.group) continue;
           if (all) {
-            uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(at.s.first + row / p.group) * p.q_heads +
-                                         at.head * p.group + row % p.group) * D + D / 8 * g);
+            const int token = row / p.group;
+            uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(at.s.first + token) * p.q_heads +
+                                         at.head * p.group + row - token * p.group) * D + D / 8 * g);
 #pragma unroll
             for (int x = 0; x < D / 64; ++x)
               *reinterpret_cast<uint4*>(dst + 16 * x) =
@@ -626,147 +749,154 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
   __syncthreads();
   if (*abort_flag) return;
 
-  // --- parts of this CTA's warps, joined -------------------------------------
+  // --- parts of this CTA's warps, joined: a warp a row -------------------------
+  using Row = Slice<D / 32>;
+  auto store = [&](const Segment& seg, const Span& sp, int r, const Row& x) {
+    const int row = seg.chunk * kRows + r, token = row / p.group;
+    uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(sp.first + token) * p.q_heads + seg.head * p.group +
+                                 row - token * p.group) * D + D / 32 * lane);
+    if constexpr (D == 128) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(T::down(x.x[0], x.x[1]), T::down(x.x[2], x.x[3]));
+    } else {
+      *reinterpret_cast<uint32_t*>(dst) = T::down(x.x[0], x.x[1]);
+    }
+  };
   auto part_of = [&](int s) -> const float* {
-    return s & 1 ? reinterpret_cast<const float*>(smem + (s >> 1) * kDepth * kBytes)
+    return s & 1 ? reinterpret_cast<const float*>(smem + (s >> 1) * kDepth * kSlot)
                  : reinterpret_cast<const float*>(smem + Cfg::kOffParts) + (s >> 1) * kPart;
   };
-  auto store = [&](const Segment& seg, const Span& sp, int r, int c, const float4& x) {
-    const int row = seg.chunk * kRows + r;
-    *reinterpret_cast<uint2*>(
-        p.out + 2 * ((static_cast<int64_t>(sp.first + row / p.group) * p.q_heads + seg.head * p.group +
-                      row % p.group) * D + c)) = make_uint2(T::down(x.x, x.y), T::down(x.z, x.w));
-  };
-  int open[2] = {-1, -1};  // segments of the items that other CTAs share: from before, into the next
+  int open0 = -1, open1 = -1;  // segments of the items that other CTAs share: from before, into the next
+  {
+    const int mine = lane < 2 * kWarps ? segments[lane].begin : -1;
+    uint32_t left = __ballot_sync(0xffffffffu, mine >= 0);
+    int unit = 0;
+    while (left) {
+      const int s0 = __ffs(left) - 1;
+      const Segment seg = segments[s0];
+      const uint32_t group = __ballot_sync(0xffffffffu, mine == seg.begin);
+      left &= ~group;
+      const bool all = seg.begin >= cta_begin && seg.end <= cta_end;
+      const int side = seg.begin < cta_begin ? 0 : 1;
+      if (!all) (side ? open1 : open0) = s0;
+      const Span sp = span_of<kRows>(p, seg.b);
+      const int rows = min(kRows, sp.n * p.group - seg.chunk * kRows);
 #pragma unroll 1
-  for (int s0 = 0; s0 < 2 * Cfg::kWarps;) {
-    const Segment seg = segments[s0];
-    if (seg.begin < 0) {
-      ++s0;
-      continue;
-    }
-    int s1 = s0 + 1;
-    while (s1 < 2 * Cfg::kWarps && (segments[s1].begin < 0 || segments[s1].begin == seg.begin)) ++s1;
-    const Span sp = span_of<kRows>(p, seg.b);
-    const int rows = min(kRows, sp.n * p.group - seg.chunk * kRows);
-    const bool all = seg.begin >= cta_begin && seg.end <= cta_end;
-    const int side = seg.begin < cta_begin ? 0 : 1;
-    float* to = p.partials + (2ll * blockIdx.x + side) * kPart;
-    if (!all) open[side] = s0;
+      for (int r = 0; r < rows; ++r, ++unit) {
+        if (unit % kWarps != warp) continue;
+        const bool in = group >> lane & 1;
+        const float m = in ? part_of(lane)[kRows * D + r] : kLowest;
+        const float top_all = warp_max(m);
+        float w = in ? part_of(lane)[kRows * D + kRows + r] * exp2_approx(m - top_all) : 0.f;
+        const float sum = warp_sum(w);
+        w *= sum == 0.f ? 0.f : 1.f / sum;
+        Row x = {};
 #pragma unroll 1
-    for (int r = threadIdx.x; r < rows; r += Cfg::kThreads) {
-      float m = kLowest, sum = 0.f;
-#pragma unroll 1
-      for (int s = s0; s < s1; ++s)
-        if (segments[s].begin >= 0) m = fmaxf(m, part_of(s)[kRows * D + r]);
-#pragma unroll 1
-      for (int s = s0; s < s1; ++s) {
-        if (segments[s].begin < 0) continue;
-        const float w = part_of(s)[kRows * D + kRows + r] * exp2_approx(part_of(s)[kRows * D + r] - m);
-        join_w[s * kRows + r] = w;
-        sum += w;
-      }
-      const float over = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll 1
-      for (int s = s0; s < s1; ++s) join_w[s * kRows + r] *= over;
-      if (!all) to[kRows * D + r] = m, to[kRows * D + kRows + r] = sum;
-    }
-    __syncthreads();
-#pragma unroll 1
-    for (int i = threadIdx.x; i < rows * (D / 4); i += Cfg::kThreads) {
-      const int r = i / (D / 4);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-      for (int s = s0; s < s1; ++s) {
-        if (segments[s].begin < 0) continue;
-        const float w = join_w[s * kRows + r];
-        const float4 v = *reinterpret_cast<const float4*>(part_of(s) + 4 * i);
-        x = make_float4(fmaf(w, v.x, x.x), fmaf(w, v.y, x.y), fmaf(w, v.z, x.z), fmaf(w, v.w, x.w));
-      }
-      if (all) {
-        store(seg, sp, r, 4 * (i % (D / 4)), x);
-      } else {
-        *reinterpret_cast<float4*>(to + 4 * i) = x;
+        for (uint32_t rest = group; rest; rest &= rest - 1) {
+          const int s = __ffs(rest) - 1;
+          x.add_shared(__shfl_sync(0xffffffffu, w, s), part_of(s) + r * D, lane);
+        }
+        if (all) {
+          store(seg, sp, r, x);
+        } else {
+          float* to = p.partials + (2ll * blockIdx.x + side) * kPart;
+          x.put(to + r * D, lane);
+          if (lane == 0) to[kRows * D + r] = top_all, to[kRows * D + kRows + r] = sum;
+        }
       }
     }
-    s0 = s1;
   }
-  if (open[0] < 0 && open[1] < 0) return;
+  if (open0 < 0 && open1 < 0) return;
 
   // --- items of several CTAs: the last to bring its part joins them ----------
   __threadfence();
   __syncthreads();
-  float* weights = reinterpret_cast<float*>(smem);               // [ctas][rows]: the rings are done with
-  float4* sheets = reinterpret_cast<float4*>(smem + Cfg::kRing); // [sheets][rows * D / 4]: so are the parts
-  static_assert(Cfg::kThreads * 16 <= Cfg::kWarps * kPart * 4, "sheets");
-#pragma unroll 1
+  if (threadIdx.x < 2) {
+    const int s = threadIdx.x ? open1 : open0;
+    int last = 0;
+    if (s >= 0) {
+      const int c0 = first_cta(segments[s].begin), c1 = last_cta(segments[s].begin, segments[s].end);
+      last = atomicAdd(p.counters + c0, 1) == c1 - c0;
+      if (last) p.counters[c0] = 0;
+    }
+    last_flag[threadIdx.x] = last;
+  }
+  __syncthreads();
+  if (!last_flag[0] && !last_flag[1]) return;
+  __threadfence();
+  int rows_of[2];
+#pragma unroll
   for (int side = 0; side < 2; ++side) {
-    if (open[side] < 0) continue;
-    const Segment seg = segments[open[side]];
-    const int c0 = seg.begin / quota, c1 = (seg.end - 1) / quota;
-    if (threadIdx.x == 0) *last_flag = atomicAdd(p.counters + c0, 1) == c1 - c0;
-    __syncthreads();
-    if (*last_flag) {
-      __threadfence();
-      if (threadIdx.x == 0) p.counters[c0] = 0;
-      const Span sp = span_of<kRows>(p, seg.b);
-      const int rows = min(kRows, sp.n * p.group - seg.chunk * kRows), ctas = c1 - c0 + 1;
-      auto from = [&](int c) -> const float* {
-        return p.partials + (2ll * (c0 + c) + (c == 0 ? 1 : 0)) * kPart;
-      };
+    rows_of[side] = 0;
+    if (last_flag[side]) {
+      const Segment& seg = segments[side ? open1 : open0];
+      rows_of[side] = min(kRows, span_of<kRows>(p, seg.b).n * p.group - seg.chunk * kRows);
+    }
+  }
+  // a warp a row of either item, or several, each over some of the CTAs
+  const int units = rows_of[0] + rows_of[1];
+  const int split = units <= kWarps / 2 ? kWarps / units : 1;
+  float* sheets = reinterpret_cast<float*>(smem);  // [warps][D + 4]: the rings are done with
 #pragma unroll 1
-      for (int r = warp; r < rows; r += Cfg::kWarps) {  // a warp a row
-        float m = kLowest, sum = 0.f;
+  for (int unit = warp / split; unit < units; unit += kWarps / split) {
+    const int side = unit >= rows_of[0], r = side ? unit - rows_of[0] : unit, sub = warp % split;
+    const Segment seg = segments[side ? open1 : open0];
+    const int c0 = first_cta(seg.begin), parts = last_cta(seg.begin, seg.end) - c0 + 1;
+    auto from = [&](int c) -> const float* {
+      return p.partials + (2ll * (c0 + c) + (c == 0 ? 1 : 0)) * kPart;
+    };
+    float top_all = kLowest, sum = 0.f;
+    Row x = {};
 #pragma unroll 1
-        for (int c = lane; c < ctas; c += 32) m = fmaxf(m, __ldcg(from(c) + kRows * D + r));
+    for (int base = sub; base < parts; base += 32 * split) {
+      const int c = base + split * lane;
+      const float m = c < parts ? __ldcg(from(c) + kRows * D + r) : kLowest;
+      const float n = c < parts ? __ldcg(from(c) + kRows * D + kRows + r) : 0.f;
+      const float top1 = fmaxf(top_all, warp_max(m)), f = exp2_approx(top_all - top1);
+      const float w = n * exp2_approx(m - top1);
+      top_all = top1;
+      sum = fmaf(sum, f, warp_sum(w));
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+      for (int y = 0; y < D / 32; ++y) x.x[y] *= f;
+      const int here = min(32, (parts - base + split - 1) / split);
 #pragma unroll 1
-        for (int c = lane; c < ctas; c += 32) {
-          const float w = __ldcg(from(c) + kRows * D + kRows + r) * exp2_approx(__ldcg(from(c) + kRows * D + r) - m);
-          weights[c * kRows + r] = w;
-          sum += w;
-        }
+      for (int y = 0; y < here; y += 8) {
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        const float over = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll 1
-        for (int c = lane; c < ctas; c += 32) weights[c * kRows + r] *= over;
-      }
-      __syncthreads();
-      // few rows: several sheets of threads, each over some of the CTAs
-      const int sheet = rows * (D / 4), count = max(1, min(256 / sheet, ctas));
-#pragma unroll 1
-      for (int i0 = threadIdx.x; i0 < count * sheet; i0 += Cfg::kThreads) {
-        const int i = i0 % sheet, r = i / (D / 4);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int c = i0 / sheet; c < ctas; c += count) {
-          const float w = weights[c * kRows + r];
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(from(c) + 4 * i));
-          x = make_float4(fmaf(w, v.x, x.x), fmaf(w, v.y, x.y), fmaf(w, v.z, x.z), fmaf(w, v.w, x.w));
-        }
-        if (count == 1) {
-          store(seg, sp, r, 4 * (i % (D / 4)), x);
-        } else {
-          sheets[i0] = x;
-        }
-      }
-      if (count > 1) {
-        __syncthreads();
-#pragma unroll 1
-        for (int i = threadIdx.x; i < sheet; i += Cfg::kThreads) {
-          float4 x = sheets[i];
-#pragma unroll 1
-          for (int c = 1; c < count; ++c) {
-            const float4 v = sheets[c * sheet + i];
-            x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
-          }
-          store(seg, sp, i / (D / 4), 4 * (i % (D / 4)), x);
+        for (int z = 0; z < 8; ++z) {  // past the end: the last one again, times nothing
+          const float wz = __shfl_sync(0xffffffffu, w, (y + z) & 31);
+          x.add(y + z < here ? wz : 0.f, from(base + split * min(y + z, here - 1)) + r * D, lane);
         }
       }
     }
-    __syncthreads();
+    const float over = split > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int y = 0; y < D / 32; ++y) x.x[y] *= over;
+    if (split > 1) {
+      x.put(sheets + warp * (D + 4), lane);
+      if (lane == 0) sheets[warp * (D + 4) + D] = top_all, sheets[warp * (D + 4) + D + 1] = sum;
+    } else {
+      store(seg, span_of<kRows>(p, seg.b), r, x);
+    }
+  }
+  if (split == 1) return;
+  __syncthreads();
+  if (warp < units) {
+    const int side = warp >= rows_of[0], r = side ? warp - rows_of[0] : warp;
+    float top_all = kLowest, sum = 0.f;
+    Row x = {};
+#pragma unroll 1
+    for (int y = 0; y < split; ++y) top_all = fmaxf(top_all, sheets[(warp * split + y) * (D + 4) + D]);
+#pragma unroll 1
+    for (int y = 0; y < split; ++y) {
+      const float* sheet = sheets + (warp * split + y) * (D + 4);
+      const float f = exp2_approx(sheet[D] - top_all);
+      sum = fmaf(sheet[D + 1], f, sum);
+      x.add_shared(f, sheet, lane);
+    }
+    const float over = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int y = 0; y < D / 32; ++y) x.x[y] *= over;
+    const Segment seg = segments[side ? open1 : open0];
+    store(seg, span_of<kRows>(p, seg.b), r, x);
   }
 }
 
