@@ -23,8 +23,9 @@
 // issues the products, and four warps per query tile do the softmax, one row a
 // thread.  While one query tile is in its softmax the other one's products
 // run.  The running maximum is only moved when an argument passes it by more than
-// 8 (a factor of 256): then the step's weights are made again and the
-// accumulator in tensor memory is scaled, which is rare after the first steps.
+// 8 (a factor of 256): then the step's weights are made again, more slowly, and
+// the accumulator in tensor memory is scaled, which is rare after the first
+// steps.  Steps that some row does not see whole go the slow way too.
 #pragma once
 
 #include <math_constants.h>
@@ -90,6 +91,15 @@ __device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* v)
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
       "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
       "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 
@@ -185,6 +195,13 @@ struct Constants {
   float2 at_8[kStep / 2];
 };
 
+// Arguments of the weights of keys 2i and 2i + 1 of a step, from their products.
+__device__ __forceinline__ F2 arguments(const Constants& k, int i, uint32_t s0, uint32_t s1, F2 sumq) {
+  const float4 ks = k.key[i], vs = k.value[i];
+  return fma2(pack2(ks.x, ks.y), pack2(__uint_as_float(s0), __uint_as_float(s1)),
+              fma2(pack2(ks.z, ks.w), sumq, pack2(vs.x, vs.y)));
+}
+
 template <class T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     kv4_prompt_kernel(const __grid_constant__ PromptParams p) {
@@ -272,11 +289,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
   auto wait = [&](uint32_t at, int phase) {  // one thread
-    ok = ok && mbar_wait_bounded(at, phase & 1, abort_flag);
+    ok = ok && mbar_wait_spin_sleep_bounded(at, phase & 1, abort_flag);
     return ok;
   };
   auto wait_warp = [&](uint32_t at, int phase) {
-    ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(at, phase & 1, abort_flag));
+    ok = __all_sync(0xffffffffu, ok && mbar_wait_spin_sleep_bounded(at, phase & 1, abort_flag));
     return ok;
   };
 
@@ -334,74 +351,102 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const bool whole = j0 + kStep <= tile_lo + 1 && (p.window == 0 || tile_hi - j0 < p.window) &&
                            (valid[4 * buf] & valid[4 * buf + 1] & valid[4 * buf + 2] & valid[4 * buf + 3]) ==
                                0xffffffffu;
-        uint32_t weights[64];
-        float lt, offt;
-        while (true) {
+        const F2 q2 = pack2(sumq, sumq);
+        bool done = false;
+        if (whole && it > 0) {
+          // the step with the maximum as it is
+          uint32_t weights[64];
           float mx = kLowest;
           F2 l2 = 0, off2 = 0;
-          const F2 q2 = pack2(sumq, sumq), top2 = pack2(-top, -top);
+          const F2 top2 = pack2(-top, -top);
 #pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tmem_ld32(s_at + 32 * c, s);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 y = unpack2(add2(arguments(k, 16 * c + i, s[2 * i], s[2 * i + 1], q2), top2));
+              mx = fmaxf(mx, fmaxf(y.x, y.y));
+              const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+              const F2 w2 = pack2(w.x, w.y);
+              const float4 vs = k.value[16 * c + i];
+              const float2 z = k.at_8[16 * c + i];
+              l2 = fma2(w2, pack2(vs.z, vs.w), l2);
+              off2 = fma2(w2, pack2(z.x, z.y), off2);
+              weights[16 * c + i] = Half::down(w.x, w.y);
+            }
+          }
+          done = !__any_sync(0xffffffffu, mx > 8.f);
+          if (done) {
+            const float2 la = unpack2(l2), oa = unpack2(off2);
+            l += la.x + la.y;
+            off += oa.x + oa.y;
+            tmem_store_32(s_at, weights);
+            tmem_store_32(s_at + 32, weights + 32);
+          }
+        }
+        if (!done) {
+          // With the maximum of the step first.  What a row does not see has no
+          // weight, whatever lies in its place.
+          const int back = p.window ? p.window : 0x7fffffff;  // a query sees less far than this
+          auto unseen = [&](int j, uint32_t there) {
+            return j > pos || pos - j >= back || !(there >> (j & 31) & 1);
+          };
+          float mx = kLowest;
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t s[32];
             tmem_ld32(s_at + 32 * c, s);
             const uint32_t there = valid[4 * buf + c];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float4 ks = k.key[16 * c + i / 2], vs = k.value[16 * c + i / 2];
-              const float2 z = k.at_8[16 * c + i / 2];
-              F2 x = fma2(pack2(ks.x, ks.y), pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
-                          fma2(pack2(ks.z, ks.w), q2, pack2(vs.x, vs.y)));
-              if (!whole) {
-                float2 y = unpack2(x);
-                const int j = j0 + 32 * c + i;
-                const int back = p.window ? p.window : 0x7fffffff;  // a query sees less far than this
-                if (j > pos || pos - j >= back || !(there >> i & 1)) y.x = -CUDART_INF_F;
-                if (j + 1 > pos || pos - j - 1 >= back || !(there >> (i + 1) & 1)) y.y = -CUDART_INF_F;
-                x = pack2(y.x, y.y);
-              }
-              const float2 xs = unpack2(x);
-              mx = fmaxf(mx, fmaxf(xs.x, xs.y));
-              const float2 y = unpack2(add2(x, top2));
-              const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-              const F2 w2 = pack2(w.x, w.y);
-              if (whole) {
-                l2 = fma2(w2, pack2(vs.z, vs.w), l2);
-                off2 = fma2(w2, pack2(z.x, z.y), off2);
-              } else {  // what is not seen may be anything
-                const bool n0 = xs.x == -CUDART_INF_F, n1 = xs.y == -CUDART_INF_F;
-                l2 = fma2(w2, pack2(n0 ? 0.f : vs.z, n1 ? 0.f : vs.w), l2);
-                off2 = fma2(w2, pack2(n0 ? 0.f : z.x, n1 ? 0.f : z.y), off2);
-              }
-              weights[16 * c + i / 2] = Half::down(w.x, w.y);
+            for (int i = 0; i < 16; ++i) {
+              const float2 x = unpack2(arguments(k, 16 * c + i, s[2 * i], s[2 * i + 1], q2));
+              const int j = j0 + 32 * c + 2 * i;
+              if (!unseen(j, there)) mx = fmaxf(mx, x.x);
+              if (!unseen(j + 1, there)) mx = fmaxf(mx, x.y);
             }
           }
-          const float2 la = unpack2(l2), oa = unpack2(off2);
-          lt = la.x + la.y;
-          offt = oa.x + oa.y;
-          if (!__any_sync(0xffffffffu, mx > top + 8.f)) break;
-          // move the maximum: scale what there is, and make the weights again
-          const float f = exp2_approx(top - fmaxf(top, mx));
-          top = fmaxf(top, mx);
-          l *= f;
-          off *= f;
-          if (it > 0) {
-            if (!wait_warp(o_done + 8 * qi, it - 1)) break;
-            tc_fence_after();
+          if (__any_sync(0xffffffffu, mx > top + 8.f)) {
+            const float f = exp2_approx(top - fmaxf(top, mx));
+            top = fmaxf(top, mx);
+            l *= f;
+            off *= f;
+            if (it > 0) {
+              if (!wait_warp(o_done + 8 * qi, it - 1)) break;
+              tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o_at + 32 * c, o);
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(o_at + 32 * c, o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_store_32(o_at + 32 * c, o);
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_store_32(o_at + 32 * c, o);
+              }
             }
+          }
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tmem_ld32(s_at + 32 * c, s);
+            const uint32_t there = valid[4 * buf + c];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 x = unpack2(arguments(k, 16 * c + i, s[2 * i], s[2 * i + 1], q2));
+              const float4 vs = k.value[16 * c + i];
+              const float2 z = k.at_8[16 * c + i];
+              const int j = j0 + 32 * c + 2 * i;
+              float2 w = make_float2(exp2_approx(x.x - top), exp2_approx(x.y - top));
+              float2 lw = make_float2(w.x * vs.z, w.y * vs.w), zw = make_float2(w.x * z.x, w.y * z.y);
+              if (unseen(j, there)) w.x = lw.x = zw.x = 0.f;
+              if (unseen(j + 1, there)) w.y = lw.y = zw.y = 0.f;
+              l += lw.x + lw.y;
+              off += zw.x + zw.y;
+              s[i] = Half::down(w.x, w.y);
+            }
+            // its place is that of products already read
+            tmem_store_16(s_at + 16 * c, s);
           }
         }
-        if (!ok) break;
-        l += lt;
-        off += offt;
-        tmem_store_32(s_at, weights);
-        tmem_store_32(s_at + 32, weights + 32);
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
