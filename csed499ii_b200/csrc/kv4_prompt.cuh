@@ -19,10 +19,11 @@
 // multiply-adds a pair than plain attention, in two-wide f32x2 instructions,
 // and saves every rounding but the weights'.
 //
-// Four warps turn codes into operand tiles (two stages of each), one thread
-// issues the products, and four warps per query tile do the softmax, one row a
-// thread.  While one query tile is in its softmax the other one's products
-// run.  The running maximum is only moved when an argument passes it by more than
+// Four warps each turn key and value codes into operand tiles (two stages of
+// each), a thread per query tile issues its products (one thread issues a
+// product of 128 x 128 x 16 every ~90 cycles, the tensor core could take one
+// every 64), and four warps per query tile do the softmax, one row a thread.
+// While one query tile is in its softmax the other one's products run.  The running maximum is only moved when an argument passes it by more than
 // 8 (a factor of 256): then the step's weights are made again, more slowly, and
 // the accumulator in tensor memory is scaled, which is rare after the first
 // steps.  Steps that some row does not see whole go the slow way too.
@@ -37,7 +38,9 @@ namespace sm100 {
 namespace kv4 {
 
 constexpr int kPromptBatch = 8192;  // requests of a launch
-constexpr int kPromptThreads = 13 * 32;
+constexpr int kPromptThreads = 20 * 32;
+// Registers a thread: 96 at launch, then as below (256 * 168 + 256 * 56 + 128 * 32 = 640 * 96).
+constexpr int kSoftmaxRegs = 168, kOperandRegs = 56, kIssueRegs = 32;
 constexpr int kStep = 128;          // keys of a step
 
 struct PromptParams {
@@ -161,6 +164,21 @@ __device__ __forceinline__ uint4 centred(uint32_t w) {
   return r;
 }
 
+template <int N>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 __device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
@@ -214,15 +232,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffMisc);
   const uint32_t bar = smem_addr(bars);
   // barriers
-  const uint32_t q_ready = bar, k_full = bar + 8, k_empty = bar + 24, v_full = bar + 40,
-                 v_empty = bar + 56, s_full = bar + 72, p_ready = bar + 88, o_done = bar + 104,
-                 c_full = bar + 120 /* four */, finished = bar + 152;
-  uint64_t* tile_at = bars + 20;                                        // [4][8]
-  uint32_t* valid = reinterpret_cast<uint32_t*>(bars + 52);             // [4][4]
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 68);
+  const uint32_t q_ready = bar, k_full = bar + 16, k_empty = bar + 32, v_full = bar + 48,
+                 v_empty = bar + 64, s_full = bar + 80, p_ready = bar + 96, o_done = bar + 112,
+                 c_full = bar + 128 /* four */, finished = bar + 160;
+  uint64_t* tile_at = bars + 24;                                        // keys' and values' [4][8]
+  uint32_t* valid = reinterpret_cast<uint32_t*>(bars + 88);             // [4][4]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 96);
   volatile int* drain_flag = abort_flag + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 69);
-  int* sums = reinterpret_cast<int*>(bars + 70);                        // [16]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 97);
+  int* sums = reinterpret_cast<int*>(bars + 98);                        // [20]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.y;
 
@@ -240,7 +258,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (lane == 31) sums[warp] = x;
     __syncthreads();
     int all = 0;
-    for (int i = 0; i < 13; ++i) {
+    for (int i = 0; i < kPromptThreads / 32; ++i) {
       if (i == warp) x += all;
       all += sums[i];
     }
@@ -267,22 +285,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   __syncthreads();  // `pre` is read
 
   if (threadIdx.x == 0) {
-    mbar_init(q_ready, 4 * tiles_q);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(q_ready + 8 * i, 4);
       mbar_init(k_full + 8 * i, 4);
-      mbar_init(k_empty + 8 * i, 1);
+      mbar_init(k_empty + 8 * i, tiles_q);
       mbar_init(v_full + 8 * i, 4);
-      mbar_init(v_empty + 8 * i, 1);
+      mbar_init(v_empty + 8 * i, tiles_q);
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_ready + 8 * i, 4);
       mbar_init(o_done + 8 * i, 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(c_full + 8 * i, 4);
-    mbar_init(finished, 1);
+    mbar_init(finished, tiles_q);
     *abort_flag = *drain_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 12) tmem_alloc(smem_addr(tmem_slot), Cfg::kCols);
+  if (warp == 16) tmem_alloc(smem_addr(tmem_slot), Cfg::kCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -299,6 +317,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
+    take_registers<kSoftmaxRegs>();
     const int qi = warp >> 2, row = (warp & 3) * 32 + lane;
     if (qi < tiles_q) {
       const int r = tile * 256 + qi * 128 + row;
@@ -333,7 +352,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
+      if (lane == 0) mbar_arrive(q_ready + 8 * qi);
 
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t s_at = tmem + lanes + Cfg::kColS + 128 * qi;
@@ -356,8 +375,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (whole && it > 0) {
           // the step with the maximum as it is
           uint32_t weights[64];
-          float mx = kLowest;
-          F2 l2 = 0, off2 = 0;
+          float mx[2] = {kLowest, kLowest};
+          F2 l2[2] = {0, 0}, off2[2] = {0, 0};
           const F2 top2 = pack2(-top, -top);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -366,19 +385,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const float2 y = unpack2(add2(arguments(k, 16 * c + i, s[2 * i], s[2 * i + 1], q2), top2));
-              mx = fmaxf(mx, fmaxf(y.x, y.y));
+              mx[i & 1] = max3(mx[i & 1], y.x, y.y);
               const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
               const F2 w2 = pack2(w.x, w.y);
               const float4 vs = k.value[16 * c + i];
               const float2 z = k.at_8[16 * c + i];
-              l2 = fma2(w2, pack2(vs.z, vs.w), l2);
-              off2 = fma2(w2, pack2(z.x, z.y), off2);
+              l2[i & 1] = fma2(w2, pack2(vs.z, vs.w), l2[i & 1]);
+              off2[i & 1] = fma2(w2, pack2(z.x, z.y), off2[i & 1]);
               weights[16 * c + i] = Half::down(w.x, w.y);
             }
           }
-          done = !__any_sync(0xffffffffu, mx > 8.f);
+          done = !__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) > 8.f);
           if (done) {
-            const float2 la = unpack2(l2), oa = unpack2(off2);
+            const float2 la = unpack2(add2(l2[0], l2[1])), oa = unpack2(add2(off2[0], off2[1]));
             l += la.x + la.y;
             off += oa.x + oa.y;
             tmem_store_32(s_at, weights);
@@ -474,13 +493,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {
     // ------------------------------------------- codes to operand tiles
-    constexpr int kUnits = D / 32;  // 16-byte loads of key codes a thread
-    constexpr int kWordsV = D / 64; // words of value codes per token a thread
-    const int dw = warp - 8, id = dw * 32 + lane;
-    const float c2 = p.scale * kLog2e;
+    // Warps 8-11 the keys' (and what the softmax needs to know), 12-15 the
+    // values'.  Codes are in registers a step ahead; where a step's tiles lie is
+    // looked up two steps ahead.  Once a wait has given up these warps run on
+    // without waiting: they meet at a barrier every step, which none of them
+    // may leave alone.
+    give_registers<kOperandRegs>();
+    const bool keys = warp < 12;
+    const int dw = warp & 3, id = dw * 32 + lane, meet = keys ? 1 : 2;
     const int per_page = p.cache.page_size / kTile;
+    uint64_t* tiles = tile_at + (keys ? 0 : 32);
     auto look_up = [&](int it) {  // where the step's eight cache tiles are
       if (dw == 0 && lane < 8 && it < steps) {
         const int t = (step0 + it) * 8 + lane;
@@ -490,76 +514,60 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.pages))
             at = reinterpret_cast<uint64_t>(p.cache.page_tiles<D>(page, head) + t % per_page * kBytes);
         }
-        tile_at[8 * (it & 3) + lane] = at;
+        tiles[8 * (it & 3) + lane] = at;
       }
     };
-    uint4 kr[kUnits], vr[2 * kWordsV];
-    uint32_t kp = 0, vp = 0;
-    bool here = false;
-    auto load = [&](int it) {
-      if (it >= steps) return;
-      const uint64_t* at = tile_at + 8 * (it & 3);
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int rest = (u * 128 + id) >> 3, chunk = rest % kUnits, half = rest / kUnits;
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(at[half >> 1]);
-        kr[u] = src ? *reinterpret_cast<const uint4*>(src + off_k(D, (half & 1) * 8 + (lane & 7)) + 16 * chunk)
-                    : make_uint4(0, 0, 0, 0);
-      }
-      {
-        const int half = (lane & 7) + 8 * (dw & 1), piece = (lane >> 3) + 4 * (dw >> 1);
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(at[half >> 1]);
-#pragma unroll
-        for (int u = 0; u < 2 * kWordsV; ++u)
-          vr[u] = src ? *reinterpret_cast<const uint4*>(src + off_v(D, (half & 1) * 8, piece) + 16 * u)
-                      : make_uint4(0, 0, 0, 0);
-      }
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(at[id >> 4]);
-      here = src != nullptr && (step0 + it) * kStep + id < len;
-      kp = here ? *reinterpret_cast<const uint32_t*>(src + off_k_pair(D, id & 15)) : 0u;
-      vp = here ? *reinterpret_cast<const uint32_t*>(src + off_v_pair(D, id & 15)) : 0u;
-    };
+    auto tile_of = [&](int it, int i) { return reinterpret_cast<const uint8_t*>(tiles[8 * (it & 3) + i]); };
     look_up(0);
     look_up(1);
-    named_bar_sync(1, 128);
-    load(0);
-    // Once a wait has given up these warps run on without waiting: they meet at a
-    // barrier every step, which none of them may leave alone.
-    for (int it = 0; it < steps; ++it) {
-      uint4 kc[kUnits], vc[2 * kWordsV];
+    named_bar_sync(meet, 128);
+    if (keys) {
+      constexpr int kUnits = D / 32;  // 16-byte loads of a thread
+      const float c2 = p.scale * kLog2e;
+      uint4 codes[kUnits];
+      uint32_t kp = 0, vp = 0;
+      bool here = false;
+      auto load = [&](int it) {
+        if (it >= steps) return;
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) kc[u] = kr[u];
-#pragma unroll
-      for (int u = 0; u < 2 * kWordsV; ++u) vc[u] = vr[u];
-      const float2 ks = T::up(kp), vs = T::up(vp);
-      const bool there = here;
-      look_up(it + 2);
-      load(it + 1);
-      named_bar_sync(1, 128);
-      const int stage = it & 1, buf = it & 3;
-      if (it >= 2) wait_warp(k_empty + 8 * stage, (it >> 1) - 1);
-      {
-        Constants& c = constants[buf];
-        const ValueRow v = value_row(vs);
-        float* kf = reinterpret_cast<float*>(&c.key[id >> 1]) + (id & 1);
-        kf[0] = ks.x * c2;
-        kf[2] = fmaf(ks.x, 8.f, ks.y) * c2;
-        float* vf = reinterpret_cast<float*>(&c.value[id >> 1]) + (id & 1);
-        vf[0] = v.log_s;
-        vf[2] = v.inv_s;
-        reinterpret_cast<float*>(&c.at_8[id >> 1])[id & 1] = v.at_8;
-        const uint32_t mask = __ballot_sync(0xffffffffu, there);
-        if (lane == 0) valid[4 * buf + dw] = mask;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(c_full + 8 * buf);
-      }
-      {
+        for (int u = 0; u < kUnits; ++u) {
+          const int rest = (u * 128 + id) >> 3, chunk = rest % kUnits, half = rest / kUnits;
+          const uint8_t* src = tile_of(it, half >> 1);
+          codes[u] = src ? *reinterpret_cast<const uint4*>(src + off_k(D, (half & 1) * 8 + (lane & 7)) + 16 * chunk)
+                         : make_uint4(0, 0, 0, 0);
+        }
+        const uint8_t* src = tile_of(it, id >> 4);
+        here = src != nullptr && (step0 + it) * kStep + id < len;
+        kp = here ? *reinterpret_cast<const uint32_t*>(src + off_k_pair(D, id & 15)) : 0u;
+        vp = here ? *reinterpret_cast<const uint32_t*>(src + off_v_pair(D, id & 15)) : 0u;
+      };
+      load(0);
+      for (int it = 0; it < steps; ++it) {
+        const int stage = it & 1, buf = it & 3;
+        look_up(it + 2);
+        if (it >= 2) wait_warp(k_empty + 8 * stage, (it >> 1) - 1);
+        {
+          const float2 ks = T::up(kp);
+          const ValueRow v = value_row(T::up(vp));
+          Constants& c = constants[buf];
+          float* kf = reinterpret_cast<float*>(&c.key[id >> 1]) + (id & 1);
+          kf[0] = ks.x * c2;
+          kf[2] = fmaf(ks.x, 8.f, ks.y) * c2;
+          float* vf = reinterpret_cast<float*>(&c.value[id >> 1]) + (id & 1);
+          vf[0] = v.log_s;
+          vf[2] = v.inv_s;
+          reinterpret_cast<float*>(&c.at_8[id >> 1])[id & 1] = v.at_8;
+          const uint32_t mask = __ballot_sync(0xffffffffu, here);
+          if (lane == 0) valid[4 * buf + dw] = mask;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(c_full + 8 * buf);
+        }
         const uint32_t dst = smem_addr(smem) + Cfg::kOffK + stage * Cfg::kK;
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
           const int rest = (u * 128 + id) >> 3, chunk = rest % kUnits, half = rest / kUnits;
           const int key = half * 8 + (lane & 7);
-          const uint32_t w[4] = {kc[u].x, kc[u].y, kc[u].z, kc[u].w};
+          const uint32_t w[4] = {codes[u].x, codes[u].y, codes[u].z, codes[u].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int c8 = chunk * 4 + i;  // eighth channel group of the row
@@ -567,29 +575,42 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                    centred<T::kBf16>(w[i]));
           }
         }
+        load(it + 1);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(k_full + 8 * stage);
+        named_bar_sync(meet, 128);
       }
-      if (it >= 2) wait_warp(v_empty + 8 * stage, (it >> 1) - 1);
-      {
+    } else {
+      constexpr int kWordsV = D / 64;  // words of codes per token a thread
+      const int half = (lane & 7) + 8 * (dw & 1), piece = (lane >> 3) + 4 * (dw >> 1);
+      uint32_t w[8 * kWordsV];         // of the eight tokens of a half tile: [token][kWordsV]
+      auto load = [&](int it) {
+        if (it >= steps) return;
+        const uint8_t* src = tile_of(it, half >> 1);
+#pragma unroll
+        for (int u = 0; u < 2 * kWordsV; ++u) {
+          const uint4 x = src ? *reinterpret_cast<const uint4*>(src + off_v(D, (half & 1) * 8, piece) + 16 * u)
+                              : make_uint4(0, 0, 0, 0);
+          w[4 * u] = x.x, w[4 * u + 1] = x.y, w[4 * u + 2] = x.z, w[4 * u + 3] = x.w;
+        }
+      };
+      load(0);
+      for (int it = 0; it < steps; ++it) {
+        const int stage = it & 1;
+        look_up(it + 2);
+        if (it >= 2) wait_warp(v_empty + 8 * stage, (it >> 1) - 1);
         const uint32_t dst = smem_addr(smem) + Cfg::kOffV + stage * Cfg::kK;
-        const int half = (lane & 7) + 8 * (dw & 1), piece = (lane >> 3) + 4 * (dw >> 1);
-        // words of the eight tokens: [token][kWordsV]
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(vc);
 #pragma unroll
         for (int o = 0; o < kWordsV; ++o) {
-          uint32_t y[2][4];  // channels 0..3 and 4..7 of the octet, tokens in pairs
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            y[0][t] = prmt(w[(2 * t) * kWordsV + o], w[(2 * t + 1) * kWordsV + o], 0x5410);
-            y[1][t] = prmt(w[(2 * t) * kWordsV + o], w[(2 * t + 1) * kWordsV + o], 0x7632);
-          }
-#pragma unroll
-          for (int part = 0; part < 4; ++part) {  // channels 2 part and 2 part + 1
+          for (int part = 0; part < 4; ++part) {  // channels 2 part and 2 part + 1 of the octet
             half2 even[4], odd[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) dequant_pair(y[part >> 1][t] >> (8 * (part & 1)), even[t], odd[t]);
+            for (int t = 0; t < 4; ++t) {  // tokens 2t and 2t + 1
+              const uint32_t y = prmt(w[2 * t * kWordsV + o], w[(2 * t + 1) * kWordsV + o], part < 2 ? 0x5410 : 0x7632);
+              dequant_pair(y >> (8 * (part & 1)), even[t], odd[t]);
+            }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const int d = piece * (D / 8) + 8 * o + 2 * part + x;
@@ -600,67 +621,63 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
           }
         }
+        load(it + 1);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_full + 8 * stage);
+        named_bar_sync(meet, 128);
       }
     }
-  } else if (lane == 0 && steps > 0) {
-    // ------------------------------------------------------------ products
-    constexpr uint32_t types = T::kBf16 ? (1u << 7) | (1u << 10) : 0u;
-    constexpr uint32_t id_s = umma_idesc_f16_f32(kStep) | types, id_o = umma_idesc_f16_f32(D);
-    const uint32_t base = smem_addr(smem);
-    auto scores = [&](int qi, int stage) {
-      const uint64_t a = umma_desc_sw128_k(base + qi * Cfg::kQ);
-      const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffK + stage * Cfg::kK);
+  } else {
+    give_registers<kIssueRegs>();
+    const int qi = warp - 16;
+    if (lane == 0 && qi < tiles_q && steps > 0) {
+      // ---------------------------------------------------------- products
+      constexpr uint32_t types = T::kBf16 ? (1u << 7) | (1u << 10) : 0u;
+      constexpr uint32_t id_s = umma_idesc_f16_f32(kStep) | types, id_o = umma_idesc_f16_f32(D);
+      const uint32_t base = smem_addr(smem);
+      const uint32_t s_at = tmem + Cfg::kColS + 128 * qi, o_at = tmem + Cfg::kColO + D * qi;
+      auto scores = [&](int stage) {
+        const uint64_t a = umma_desc_sw128_k(base + qi * Cfg::kQ);
+        const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffK + stage * Cfg::kK);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
-        umma_f16(tmem + Cfg::kColS + 128 * qi, a + (at >> 4), bd + (at >> 4), id_s, k > 0);
-      }
-    };
-    auto result = [&](int qi, int stage, bool more) {
-      const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kK);
-#pragma unroll
-      for (int k = 0; k < kStep / 16; ++k) {
-        const uint32_t at = (k >> 2) * (D * 128) + (k & 3) * 32;
-        umma_f16_ts(tmem + Cfg::kColO + D * qi, tmem + Cfg::kColS + 128 * qi + 8 * k, bd + (at >> 4), id_o,
-                    more || k > 0);
-      }
-    };
-    if (wait(q_ready, 0) && wait(k_full, 0)) {
-      tc_fence_after();
-      for (int qi = 0; qi < tiles_q; ++qi) {
-        scores(qi, 0);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
+          umma_f16(s_at, a + (at >> 4), bd + (at >> 4), id_s, k > 0);
+        }
         umma_commit(s_full + 8 * qi);
-      }
-      umma_commit(k_empty);
-      for (int it = 0; it < steps && ok; ++it) {
-        const int stage = it & 1, next = (it + 1) & 1;
-        const bool more = it + 1 < steps;
-        for (int qi = 0; qi < tiles_q; ++qi) {
+        umma_commit(k_empty + 8 * stage);
+      };
+      if (wait(q_ready + 8 * qi, 0) && wait(k_full, 0)) {
+        tc_fence_after();
+        scores(0);
+        for (int it = 0; it < steps; ++it) {
+          const int stage = it & 1, next = (it + 1) & 1;
           if (!wait(v_full + 8 * stage, it >> 1) || !wait(p_ready + 8 * qi, it)) break;
           tc_fence_after();
-          result(qi, stage, it > 0);
+          const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kK);
+#pragma unroll
+          for (int k = 0; k < kStep / 16; ++k) {
+            const uint32_t at = (k >> 2) * (D * 128) + (k & 3) * 32;
+            umma_f16_ts(o_at, s_at + 8 * k, bd + (at >> 4), id_o, it > 0 || k > 0);
+          }
           umma_commit(o_done + 8 * qi);
-          if (more) {
+          umma_commit(v_empty + 8 * stage);
+          if (it + 1 < steps) {
             if (!wait(k_full + 8 * next, (it + 1) >> 1)) break;
             tc_fence_after();
-            scores(qi, next);
-            umma_commit(s_full + 8 * qi);
+            scores(next);
           }
         }
-        umma_commit(v_empty + 8 * stage);
-        if (more) umma_commit(k_empty + 8 * next);
       }
+      umma_commit(finished);
+      mbar_wait_bounded(finished, 0, drain_flag);
     }
-    umma_commit(finished);
-    mbar_wait_bounded(finished, 0, drain_flag);
   }
   if (!ok && lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::kCols);
   }
