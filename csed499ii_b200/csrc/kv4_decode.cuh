@@ -235,7 +235,9 @@ struct ValueRow {
   float log_s, inv_s, at_8;
 };
 __device__ __forceinline__ ValueRow value_row(float2 pair) {
-  const float s = pair.x > 0x1p-60f ? pair.x : fmaxf(fabsf(pair.y) * 0x1p-10f, 0x1p-60f);
+  const float s = pair.x >= 0x1p-60f  ? pair.x
+                  : pair.x > 0.f      ? 0x1p-60f
+                                      : fmaxf(fabsf(pair.y) * 0x1p-10f, 0x1p-17f);
   ValueRow r;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r.log_s) : "f"(s));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inv_s) : "f"(s));

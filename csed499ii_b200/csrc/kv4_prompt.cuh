@@ -1,32 +1,45 @@
 // Attention over the 4-bit cache for requests with many query rows (prompts,
 // pieces of prompts), on tcgen05.
 //
-// 4 * D operations per visible (query, key) pair and head bound it.  A CTA
-// takes 256 query rows of one key/value head (rows are (token, head of the
-// group) pairs, so all heads of a group share what is read) as two tiles of
-// 128, and walks over the keys in steps of 128:
+// 4 * D operations per visible (query, key) pair and head bound it, and next to
+// them one exponential a pair (16 an SM and cycle, as long as its two products
+// of 128 channels take).  A CTA takes 256 query rows of one key/value head
+// (rows are (token, head of the group) pairs, so all heads of a group share what
+// is read) as two tiles of 128, and walks over the keys in steps of 112 (128
+// where D is 64):
 //
 //   S = Q (C_k - 8)^T     tcgen05.mma, Q and the codes in shared memory
 //   P                     in the softmax warps' registers, back to tensor
 //                         memory in the place of S
 //   O += P (C_v - 8)      tcgen05.mma, P from tensor memory
 //
-// As in the decode kernel the operands are codes, exact in 16 bits, and the
-// rows' scales and offsets stay in 32 bits: a score is s_k S + z_k sum(q) with
-// z = offset + 8 scale, the exponential gives the weight w = p s_v that goes
-// back, and sum(p) = sum(w / s_v) and sum(p z_v) = sum(w z_v / s_v), one number
-// a row, join the result at the end.  That costs the softmax warps three more
-// multiply-adds a pair than plain attention, in two-wide f32x2 instructions,
-// and saves every rounding but the weights'.
+// As in the decode kernel the operands are codes, exact in 16 bits, so that
+// nothing is rounded but the weights.  What scales and offsets add is put into
+// the same products as 16 more channels, in two or three 16-bit terms each
+// (2^-22 of a value): with z = offset / s_k + 8 a key's argument of the
+// exponential is s_k (S + z sum(q) + log2 s_v / s_k), so its column of S needs
+// one multiply-add; and the columns 1 / s_v and offset / s_v + 8 next to the
+// values' codes give sum(p) and the values' offsets with the result (the weights
+// are w = p s_v).  Without them every pair of keys costs the softmax ten
+// broadcast reads of shared memory, and those bound it (1452 us instead of the
+// figure below).  They are why a step is 112 keys: two tiles of scores and two
+// of 144 channels are all of tensor memory.
+//
+// Numbers that the terms cannot hold (a key's or value's scale out of the usual
+// range, a row of NaN) are added in 32 bits by a careful form of the step.  So
+// is what the weights lose in rounding to half where the values' scales differ
+// by more than a factor of 64: a weight p s_v below 2^-14 is rounded more
+// coarsely, which is nothing to the result but could be to sum(p).  A third form
+// serves steps that some row does not see whole and steps that move the running
+// maximum: the maximum is only moved when an argument passes it by more than 8
+// (a factor of 256), which is rare after the first steps.
 //
 // Four warps each turn key and value codes into operand tiles (two stages of
-// each), a thread per query tile issues its products (one thread issues a
-// product of 128 x 128 x 16 every ~90 cycles, the tensor core could take one
-// every 64), and four warps per query tile do the softmax, one row a thread.
-// While one query tile is in its softmax the other one's products run.  The running maximum is only moved when an argument passes it by more than
-// 8 (a factor of 256): then the step's weights are made again, more slowly, and
-// the accumulator in tensor memory is scaled, which is rare after the first
-// steps.  Steps that some row does not see whole go the slow way too.
+// each), a thread per query tile issues its products (one thread issues one
+// every ~90 cycles, the tensor core could take one every 64), and four warps
+// per query tile do the softmax, one row a thread.  The second query tile starts
+// when the first one's first softmax is done, so that the products of one run
+// while the other is in its softmax.
 #pragma once
 
 #include <math_constants.h>
@@ -41,7 +54,6 @@ constexpr int kPromptBatch = 8192;  // requests of a launch
 constexpr int kPromptThreads = 20 * 32;
 // Registers a thread: 96 at launch, then as below (256 * 168 + 256 * 56 + 128 * 32 = 640 * 96).
 constexpr int kSoftmaxRegs = 168, kOperandRegs = 56, kIssueRegs = 32;
-constexpr int kStep = 128;          // keys of a step
 
 struct PromptParams {
   Cache cache;
@@ -64,17 +76,45 @@ struct PromptParams {
   int* status;
 };
 
+// What the careful form of a step needs to know of its keys (the usual one
+// reads the scales alone).
+struct Numbers {
+  float scale[128];  // of the key, times scale * log2 e
+  float z[128];      // the key's value at code 8 over its scale
+  float log_s[128], inv_s[128], at_8[128];  // ValueRow
+};
+
 template <int D>
 struct PromptCfg {
-  static constexpr int kQ = 128 * D * 2;       // a query tile
-  static constexpr int kK = kStep * D * 2;     // a key or value tile
-  static constexpr int kOffK = 2 * kQ;         // two stages
-  static constexpr int kOffV = kOffK + 2 * kK; // two stages
-  static constexpr int kOffPairs = kOffV + 2 * kK;     // [4] Constants
-  static constexpr int kOffMisc = kOffPairs + 4 * 64 * 40;
-  static constexpr int kSmem = kOffMisc + 1024 + 1024;  // and room to align
-  static constexpr uint32_t kColS = 0, kColO = 256, kCols = 512;
+  static constexpr int kStep = D == 128 ? 112 : 128;  // keys of a step
+  static constexpr int kTiles = kStep / kTile;
+  static constexpr int kN = D + 16;                   // columns of the result: channels and sums
+  // operand tiles of 128-byte rows (64 numbers), and of 32-byte rows (the 16 more)
+  static constexpr int kQ = 128 * D * 2, kQx = 128 * 32;
+  static constexpr int kK = kStep * D * 2, kKx = kStep * 32;
+  static constexpr int kV = 2 * kN * 128;
+  static constexpr int kOffK = 2 * kQ;                // two stages of each
+  static constexpr int kOffV = kOffK + 2 * kK;
+  static constexpr int kOffQx = kOffV + 2 * kV;
+  static constexpr int kOffKx = kOffQx + 2 * kQx;
+  static constexpr int kOffNumbers = kOffKx + 2 * kKx;  // four stages
+  static constexpr int kOffMisc = kOffNumbers + 4 * sizeof(Numbers);
+  static constexpr int kSmem = kOffMisc + 1280 + 1024;  // and room to align
+  static_assert(kSmem <= kPrefillSmemBudget && kK % 1024 == 0 && kV % 1024 == 0 && kKx % 256 == 0, "tiles");
+  static constexpr uint32_t kColS = 0, kColO = 2 * kStep, kCols = 512;
+  static_assert(kColO + 2 * kN <= kCols, "tensor memory");
 };
+
+// Shared-memory matrix descriptor, K-major operand of 32-byte rows, swizzled:
+// groups of 8 rows 256 bytes apart, swizzle mode 6.
+__device__ __forceinline__ uint64_t umma_desc_sw32_k(uint32_t saddr) {
+  uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(1u) << 16;
+  d |= static_cast<uint64_t>(256u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(6u) << 61;
+  return d;
+}
 
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
                                             uint32_t idesc, uint32_t accumulate) {
@@ -85,16 +125,23 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* v) {
+__device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
-      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-      "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// Waits for this thread's loads; `r` is what they brought (named here so that
+// no use of it moves before the wait).
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 
 __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* v) {
@@ -104,6 +151,12 @@ __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* v)
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 __device__ __forceinline__ void tmem_store_wait() {
@@ -125,16 +178,6 @@ __device__ __forceinline__ float2 unpack2(F2 x) {
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   F2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
@@ -206,41 +249,78 @@ __device__ __forceinline__ int prompt_items(const PromptParams& p, int b) {
   return rows > p.most ? static_cast<int>((rows + 255) / 256) : 0;
 }
 
-// What the softmax needs to know of a step's keys, two by two.
-struct Constants {
-  float4 key[kStep / 2];   // scales, values at code 8, both times scale * log2 e
-  float4 value[kStep / 2]; // ValueRow: log_s, inv_s
-  float2 at_8[kStep / 2];
-};
+// The first number of two in 16 bits, widened again.
+template <class T>
+__device__ __forceinline__ float rounded(float x) {
+  return T::up(T::down(x, 0.f)).x;
+}
 
-// Arguments of the weights of keys 2i and 2i + 1 of a step, from their products.
-__device__ __forceinline__ F2 arguments(const Constants& k, int i, uint32_t s0, uint32_t s1, F2 sumq) {
-  const float4 ks = k.key[i], vs = k.value[i];
-  return fma2(pack2(ks.x, ks.y), pack2(__uint_as_float(s0), __uint_as_float(s1)),
-              fma2(pack2(ks.z, ks.w), sumq, pack2(vs.x, vs.y)));
+// The 16 more channels, as 16-bit pairs: of a row of Q and of a key their
+// product is z sum(q) + log.  Halves in two terms each, and `log` in either of
+// two sizes; bf16 in three.
+template <class T>
+__device__ __forceinline__ void query_terms(float sum, uint4 (&x)[2]) {
+  const float h = rounded<T>(sum), m = rounded<T>(sum - h);
+  if constexpr (T::kBf16) {
+    x[0] = make_uint4(T::down(h, h), T::down(m, m), T::down(h, sum - h - m), T::down(1.f, 1.f));
+    x[1] = make_uint4(T::down(1.f, 0.f), 0u, 0u, 0u);
+  } else {
+    x[0] = make_uint4(T::down(h, m), T::down(h, 1.f), T::down(1.f, 16384.f), T::down(16384.f, 0.f));
+    x[1] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+template <class T>
+__device__ __forceinline__ void key_terms(float z, float log, uint4 (&x)[2]) {
+  const float zh = rounded<T>(z), zm = rounded<T>(z - zh);
+  if constexpr (T::kBf16) {
+    const float a = rounded<T>(log), b = rounded<T>(log - a);
+    x[0] = make_uint4(T::down(zh, zm), T::down(zh, zm), T::down(z - zh - zm, zh), T::down(a, b));
+    x[1] = make_uint4(T::down(log - a - b, 0.f), 0u, 0u, 0u);
+  } else {
+    const bool large = fabsf(log) > 60000.f;
+    const float y = large ? log * (1.f / 16384.f) : log;
+    const float a = rounded<T>(y), b = y - a;
+    x[0] = make_uint4(T::down(zh, zh), T::down(zm, large ? 0.f : a), T::down(large ? 0.f : b, large ? a : 0.f),
+                      T::down(large ? b : 0.f, 0.f));
+    x[1] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+// ... and what they hold: false for NaN too.
+template <class T>
+__device__ __forceinline__ bool terms_hold(float z, float log) {
+  return T::kBf16 ? fabsf(z) < 1e30f && fabsf(log) < 1e30f : fabsf(z) < 60000.f && fabsf(log) < 1e9f;
+}
+// The values' two numbers go into halves, a quarter of inv_s in 2^-9..2^15.
+__device__ __forceinline__ bool sums_hold(const ValueRow& v) {
+  return v.inv_s >= 0x1p-7f && v.inv_s <= 0x1p17f && fabsf(v.at_8) < 60000.f;
 }
 
 template <class T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     kv4_prompt_kernel(const __grid_constant__ PromptParams p) {
   using Cfg = PromptCfg<D>;
-  constexpr int kBytes = tile_bytes(D);
+  constexpr int kBytes = tile_bytes(D), kStep = Cfg::kStep, kTiles = Cfg::kTiles, kN = Cfg::kN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  Constants* constants = reinterpret_cast<Constants*>(smem + Cfg::kOffPairs);
+  Numbers* numbers = reinterpret_cast<Numbers*>(smem + Cfg::kOffNumbers);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffMisc);
   const uint32_t bar = smem_addr(bars);
   // barriers
-  const uint32_t q_ready = bar, k_full = bar + 16, k_empty = bar + 32, v_full = bar + 48,
-                 v_empty = bar + 64, s_full = bar + 80, p_ready = bar + 96, o_done = bar + 112,
-                 c_full = bar + 128 /* four */, finished = bar + 160;
+  // `spent`, for step t in [0, steps]: result t - 1 and scores t are done with
+  const uint32_t q_ready = bar, k_full = bar + 16, v_full = bar + 32, spent = bar + 48,
+                 s_full = bar + 64, p_ready = bar + 80, c_full = bar + 96 /* four */,
+                 second = bar + 128, finished = bar + 136;
   uint64_t* tile_at = bars + 24;                                        // keys' and values' [4][8]
-  uint32_t* valid = reinterpret_cast<uint32_t*>(bars + 88);             // [4][4]
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 96);
+  uint32_t* valid = reinterpret_cast<uint32_t*>(bars + 88);             // [4][4] keys that are there
+  uint32_t* plain_k = valid + 16;                                       // ... whose numbers the terms hold
+  uint32_t* plain_v = valid + 32;
+  int* range = reinterpret_cast<int*>(valid + 48);                      // [4][2][4] exponents of value scales
+  int* fine = range + 32;                                               // [4][4] all that are there are plain
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 140);
   volatile int* drain_flag = abort_flag + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 97);
-  int* sums = reinterpret_cast<int*>(bars + 98);                        // [20]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 141);
+  int* sums = reinterpret_cast<int*>(bars + 142);                       // [20]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.y;
 
@@ -288,14 +368,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_ready + 8 * i, 4);
       mbar_init(k_full + 8 * i, 4);
-      mbar_init(k_empty + 8 * i, tiles_q);
       mbar_init(v_full + 8 * i, 4);
-      mbar_init(v_empty + 8 * i, tiles_q);
+      mbar_init(spent + 8 * i, tiles_q);
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_ready + 8 * i, 4);
-      mbar_init(o_done + 8 * i, 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(c_full + 8 * i, 4);
+    mbar_init(second, 4);
     mbar_init(finished, tiles_q);
     *abort_flag = *drain_flag = 0;
     fence_mbar_init();
@@ -350,79 +429,110 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                             prmt(x.y, x.w, 0x7632)));
         }
       }
+      // a sum that the terms cannot hold is left to the careful form
+      const bool big = !T::kBf16 && !(fabsf(sumq) < 60000.f);
+      {
+        uint4 x[2];
+        query_terms<T>(big ? 0.f : sumq, x);
+        const uint32_t dst = smem_addr(smem) + Cfg::kOffQx + qi * Cfg::kQx + row * 32;
+        sts128(dst + ((row >> 2 & 1) << 4), x[0]);
+        sts128(dst + ((row >> 2 & 1 ^ 1) << 4), x[1]);
+      }
       fence_proxy_async_smem();
       __syncwarp();
+      const bool usual = !__any_sync(0xffffffffu, big);
       if (lane == 0) mbar_arrive(q_ready + 8 * qi);
 
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + lanes + Cfg::kColS + 128 * qi;
-      const uint32_t o_at = tmem + lanes + Cfg::kColO + D * qi;
+      const uint32_t s_at = tmem + lanes + Cfg::kColS + kStep * qi;
+      const uint32_t o_at = tmem + lanes + Cfg::kColO + kN * qi;
       const int pos = before + token;
-      const int tile_lo = before + (tile * 256 + qi * 128) / p.group;
-      const int tile_hi = before + (tile * 256 + min(rows, qi * 128 + 128) - 1) / p.group;
+      // positions of this warp's first and last row
+      const int w0 = qi * 128 + (warp & 3) * 32;
+      const int lo = before + (tile * 256 + w0) / p.group;
+      const int hi = before + (tile * 256 + max(w0, min(rows, w0 + 32) - 1)) / p.group;
       float top = kLowest, l = 0.f, off = 0.f;
+      int largest = -1000;  // exponent of a value scale up to here
       for (int it = 0; it < steps; ++it) {
         const int buf = it & 3;
         if (!wait_warp(c_full + 8 * buf, it >> 2) || !wait_warp(s_full + 8 * qi, it)) break;
         tc_fence_after();
-        const Constants& k = constants[buf];
+        const Numbers& k = numbers[buf];
         const int j0 = (step0 + it) * kStep;
-        const bool whole = j0 + kStep <= tile_lo + 1 && (p.window == 0 || tile_hi - j0 < p.window) &&
-                           (valid[4 * buf] & valid[4 * buf + 1] & valid[4 * buf + 2] & valid[4 * buf + 3]) ==
-                               0xffffffffu;
-        const F2 q2 = pack2(sumq, sumq);
         bool done = false;
-        if (whole && it > 0) {
+        const uint32_t* in_k = plain_k + 4 * buf;
+        const uint32_t* in_v = plain_v + 4 * buf;
+        const int4 up = *reinterpret_cast<const int4*>(range + 8 * buf);
+        const int4 down = *reinterpret_cast<const int4*>(range + 8 * buf + 4);
+        largest = max(largest, max(max(up.x, up.y), max(up.z, up.w)));
+        const int smallest = min(min(down.x, down.y), min(down.z, down.w));
+        const int4 all_fine = *reinterpret_cast<const int4*>(fine + 4 * buf);
+        const bool plain = usual && largest - smallest <= 6 && (all_fine.x & all_fine.y & all_fine.z & all_fine.w);
+        if (plain && it > 0 && j0 + kStep <= lo + 1 && (p.window == 0 || hi - j0 < p.window)) {
           // the step with the maximum as it is
-          uint32_t weights[64];
+          uint32_t weights[kStep / 2];
           float mx[2] = {kLowest, kLowest};
-          F2 l2[2] = {0, 0}, off2[2] = {0, 0};
           const F2 top2 = pack2(-top, -top);
+          uint32_t s[2][16];
+          tmem_load_16(s_at, s[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tmem_ld32(s_at + 32 * c, s);
+          for (int c = 0; c < kStep / 16; ++c) {
+            tmem_loaded(s[c & 1]);
+            if (c + 1 < kStep / 16) tmem_load_16(s_at + 16 * (c + 1), s[(c + 1) & 1]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 y = unpack2(add2(arguments(k, 16 * c + i, s[2 * i], s[2 * i + 1], q2), top2));
-              mx[i & 1] = max3(mx[i & 1], y.x, y.y);
-              const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-              const F2 w2 = pack2(w.x, w.y);
-              const float4 vs = k.value[16 * c + i];
-              const float2 z = k.at_8[16 * c + i];
-              l2[i & 1] = fma2(w2, pack2(vs.z, vs.w), l2[i & 1]);
-              off2[i & 1] = fma2(w2, pack2(z.x, z.y), off2[i & 1]);
-              weights[16 * c + i] = Half::down(w.x, w.y);
+            for (int i = 0; i < 16; i += 4) {
+              const float4 ks = *reinterpret_cast<const float4*>(k.scale + 16 * c + i);
+              const uint32_t* x = s[c & 1] + i;
+              const float2 y0 = unpack2(fma2(pack2(ks.x, ks.y), pack2(__uint_as_float(x[0]), __uint_as_float(x[1])), top2));
+              const float2 y1 = unpack2(fma2(pack2(ks.z, ks.w), pack2(__uint_as_float(x[2]), __uint_as_float(x[3])), top2));
+              mx[0] = max3(mx[0], y0.x, y0.y);
+              mx[1] = max3(mx[1], y1.x, y1.y);
+              weights[8 * c + i / 2] = Half::down(exp2_approx(y0.x), exp2_approx(y0.y));
+              weights[8 * c + i / 2 + 1] = Half::down(exp2_approx(y1.x), exp2_approx(y1.y));
             }
           }
           done = !__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) > 8.f);
           if (done) {
-            const float2 la = unpack2(add2(l2[0], l2[1])), oa = unpack2(add2(off2[0], off2[1]));
-            l += la.x + la.y;
-            off += oa.x + oa.y;
-            tmem_store_32(s_at, weights);
-            tmem_store_32(s_at + 32, weights + 32);
+#pragma unroll
+            for (int c = 0; c < kStep / 32; ++c) tmem_store_16(s_at + 16 * c, weights + 16 * c);
+            if constexpr (kStep % 32 != 0) tmem_store_8(s_at + kStep / 32 * 16, weights + kStep / 32 * 16);
           }
         }
         if (!done) {
           // With the maximum of the step first.  What a row does not see has no
           // weight, whatever lies in its place.
-          const int back = p.window ? p.window : 0x7fffffff;  // a query sees less far than this
-          auto unseen = [&](int j, uint32_t there) {
-            return j > pos || pos - j >= back || !(there >> (j & 31) & 1);
+          const int oldest = p.window && pos >= p.window ? pos - p.window + 1 : 0;
+          const uint32_t seen = pos < 0 ? 0 : pos - oldest;          // keys before the last one
+          const int first_key = pos < 0 ? -1000 : j0 - oldest;       // a row before all keys sees none
+          auto argument = [&](int i, uint32_t s) {  // of key i of the step
+            if (static_cast<uint32_t>(first_key + i) > seen ||
+                !(valid[4 * buf + (i >> 5)] >> (i & 31) & 1))
+              return -CUDART_INF_F;
+            float x = __uint_as_float(s);
+            const bool held = in_k[i >> 5] >> (i & 31) & 1;
+            if (!held || big) x = fmaf(k.z[i], sumq, x);
+            return fmaf(k.scale[i], x, held ? 0.f : k.log_s[i]);
+          };
+          auto plain_argument = [&](int i, uint32_t s, float scale) {
+            const float x = __uint_as_float(s) * scale;
+            return static_cast<uint32_t>(first_key + i) > seen ? -CUDART_INF_F : x;
           };
           float mx = kLowest;
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tmem_ld32(s_at + 32 * c, s);
-            const uint32_t there = valid[4 * buf + c];
+          for (int c = 0; c < kStep / 16; ++c) {
+            uint32_t s[16];
+            tmem_load_16(s_at + 16 * c, s);
+            tmem_loaded(s);
+            if (plain) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 x = unpack2(arguments(k, 16 * c + i, s[2 * i], s[2 * i + 1], q2));
-              const int j = j0 + 32 * c + 2 * i;
-              if (!unseen(j, there)) mx = fmaxf(mx, x.x);
-              if (!unseen(j + 1, there)) mx = fmaxf(mx, x.y);
+              for (int i = 0; i < 16; i += 4) {
+                const float4 ks = *reinterpret_cast<const float4*>(k.scale + 16 * c + i);
+                mx = max3(mx, plain_argument(16 * c + i, s[i], ks.x), plain_argument(16 * c + i + 1, s[i + 1], ks.y));
+                mx = max3(mx, plain_argument(16 * c + i + 2, s[i + 2], ks.z), plain_argument(16 * c + i + 3, s[i + 3], ks.w));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) mx = fmaxf(mx, argument(16 * c + i, s[i]));
             }
           }
           if (__any_sync(0xffffffffu, mx > top + 8.f)) {
@@ -431,65 +541,88 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             l *= f;
             off *= f;
             if (it > 0) {
-              if (!wait_warp(o_done + 8 * qi, it - 1)) break;
+              if (!wait_warp(spent + 8 * (it & 1), it >> 1)) break;
               tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32(o_at + 32 * c, o);
+              for (int c = 0; c < kN / 16; ++c) {
+                uint32_t o[16];
+                tmem_load_16(o_at + 16 * c, o);
+                tmem_loaded(o);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_store_32(o_at + 32 * c, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_store_16(o_at + 16 * c, o);
               }
             }
           }
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tmem_ld32(s_at + 32 * c, s);
-            const uint32_t there = valid[4 * buf + c];
+          for (int c = 0; c < kStep / 16; ++c) {
+            uint32_t s[16];
+            tmem_load_16(s_at + 16 * c, s);
+            tmem_loaded(s);
+            uint32_t weights[8];
+            if (plain) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 x = unpack2(arguments(k, 16 * c + i, s[2 * i], s[2 * i + 1], q2));
-              const float4 vs = k.value[16 * c + i];
-              const float2 z = k.at_8[16 * c + i];
-              const int j = j0 + 32 * c + 2 * i;
-              float2 w = make_float2(exp2_approx(x.x - top), exp2_approx(x.y - top));
-              float2 lw = make_float2(w.x * vs.z, w.y * vs.w), zw = make_float2(w.x * z.x, w.y * z.y);
-              if (unseen(j, there)) w.x = lw.x = zw.x = 0.f;
-              if (unseen(j + 1, there)) w.y = lw.y = zw.y = 0.f;
-              l += lw.x + lw.y;
-              off += zw.x + zw.y;
-              s[i] = Half::down(w.x, w.y);
+              for (int i = 0; i < 16; i += 4) {
+                const float4 ks = *reinterpret_cast<const float4*>(k.scale + 16 * c + i);
+                weights[i / 2] = Half::down(exp2_approx(plain_argument(16 * c + i, s[i], ks.x) - top),
+                                            exp2_approx(plain_argument(16 * c + i + 1, s[i + 1], ks.y) - top));
+                weights[i / 2 + 1] = Half::down(exp2_approx(plain_argument(16 * c + i + 2, s[i + 2], ks.z) - top),
+                                                exp2_approx(plain_argument(16 * c + i + 3, s[i + 3], ks.w) - top));
+              }
+            } else
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float x0 = argument(16 * c + i, s[i]), x1 = argument(16 * c + i + 1, s[i + 1]);
+              const float w0 = exp2_approx(x0 - top), w1 = exp2_approx(x1 - top);
+              weights[i / 2] = Half::down(w0, w1);
+              const float2 w = Half::up(weights[i / 2]);
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const int at = 16 * c + i + z;
+                const float r = (z ? w1 : w0) - (in_v[at >> 5] >> (at & 31) & 1 ? z ? w.y : w.x : 0.f);
+                if ((z ? x1 : x0) != -CUDART_INF_F) {
+                  l = fmaf(r, k.inv_s[at], l);
+                  off = fmaf(r, k.at_8[at], off);
+                }
+              }
             }
-            // its place is that of products already read
-            tmem_store_16(s_at + 16 * c, s);
+            tmem_store_8(s_at + 8 * c, weights);  // in the place of products already read
           }
         }
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + 8 * qi);
+        if (lane == 0) {
+          mbar_arrive(p_ready + 8 * qi);
+          if (it == 0 && qi == 0) mbar_arrive(second);
+        }
       }
-      if (steps > 0 && wait_warp(o_done + 8 * qi, steps - 1)) tc_fence_after();
+      if (steps > 0 && wait_warp(spent + 8 * (steps & 1), steps >> 1)) {
+        tc_fence_after();
+        uint32_t o[16];
+        tmem_load_16(o_at + D, o);
+        tmem_loaded(o);
+        l += 4.f * (__uint_as_float(o[0]) + __uint_as_float(o[1]));
+        off += __uint_as_float(o[2]) + __uint_as_float(o[3]);
+      }
       const float over = l == 0.f ? 0.f : 1.f / l;
       uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(first + token) * p.q_heads + h) * D);
       if (ok) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          if (steps > 0) tmem_ld32(o_at + 32 * c, o);
-          if (!live) continue;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float a = __uint_as_float(o[8 * i + 2 * x]), d = __uint_as_float(o[8 * i + 2 * x + 1]);
-              w[x] = l == 0.f || steps == 0 ? 0u : T::down((a + off) * over, (d + off) * over);
-            }
-            *reinterpret_cast<uint4*>(dst + 64 * c + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16] = {};
+          if (steps > 0) {
+            tmem_load_16(o_at + 16 * c, o);
+            tmem_loaded(o);
           }
+          if (!live) continue;
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            w[i] = l == 0.f ? 0u
+                            : T::down((__uint_as_float(o[2 * i]) + off) * over, (__uint_as_float(o[2 * i + 1]) + off) * over);
+          *reinterpret_cast<uint4*>(dst + 32 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(dst + 32 * c + 16) = make_uint4(w[4], w[5], w[6], w[7]);
         }
       }
     }
@@ -505,9 +638,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const int dw = warp & 3, id = dw * 32 + lane, meet = keys ? 1 : 2;
     const int per_page = p.cache.page_size / kTile;
     uint64_t* tiles = tile_at + (keys ? 0 : 32);
-    auto look_up = [&](int it) {  // where the step's eight cache tiles are
-      if (dw == 0 && lane < 8 && it < steps) {
-        const int t = (step0 + it) * 8 + lane;
+    auto look_up = [&](int it) {  // where the step's cache tiles are
+      if (dw == 0 && lane < kTiles && it < steps) {
+        const int t = (step0 + it) * kTiles + lane;
         uint64_t at = 0;
         if (static_cast<int64_t>(t) * kTile < len) {
           const int page = p.tables[p.table_stride * b + t / per_page];
@@ -532,11 +665,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
           const int rest = (u * 128 + id) >> 3, chunk = rest % kUnits, half = rest / kUnits;
-          const uint8_t* src = tile_of(it, half >> 1);
+          const uint8_t* src = half < 2 * kTiles ? tile_of(it, half >> 1) : nullptr;
           codes[u] = src ? *reinterpret_cast<const uint4*>(src + off_k(D, (half & 1) * 8 + (lane & 7)) + 16 * chunk)
                          : make_uint4(0, 0, 0, 0);
         }
-        const uint8_t* src = tile_of(it, id >> 4);
+        const uint8_t* src = id < kStep ? tile_of(it, id >> 4) : nullptr;
         here = src != nullptr && (step0 + it) * kStep + id < len;
         kp = here ? *reinterpret_cast<const uint32_t*>(src + off_k_pair(D, id & 15)) : 0u;
         vp = here ? *reinterpret_cast<const uint32_t*>(src + off_v_pair(D, id & 15)) : 0u;
@@ -545,27 +678,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int it = 0; it < steps; ++it) {
         const int stage = it & 1, buf = it & 3;
         look_up(it + 2);
-        if (it >= 2) wait_warp(k_empty + 8 * stage, (it >> 1) - 1);
+        if (it >= 2) wait_warp(spent + 8 * stage, (it >> 1) - 1);
         {
+          // A row without a scale has all codes 0: any scale tells the same.
           const float2 ks = T::up(kp);
+          const float s = ks.x > 0.f ? ks.x : fmaxf(fabsf(ks.y) * 0x1p-10f, 0x1p-10f);
+          const float z = __fdividef(ks.y, s) + 8.f, scale = s * c2;
           const ValueRow v = value_row(T::up(vp));
-          Constants& c = constants[buf];
-          float* kf = reinterpret_cast<float*>(&c.key[id >> 1]) + (id & 1);
-          kf[0] = ks.x * c2;
-          kf[2] = fmaf(ks.x, 8.f, ks.y) * c2;
-          float* vf = reinterpret_cast<float*>(&c.value[id >> 1]) + (id & 1);
-          vf[0] = v.log_s;
-          vf[2] = v.inv_s;
-          reinterpret_cast<float*>(&c.at_8[id >> 1])[id & 1] = v.at_8;
+          const float log = __fdividef(v.log_s, scale);
+          const bool held = here && terms_hold<T>(z, log);
+          Numbers& k = numbers[buf];
+          k.scale[id] = scale;
+          k.z[id] = z;
+          k.log_s[id] = v.log_s;
+          k.inv_s[id] = v.inv_s;
+          k.at_8[id] = v.at_8;
           const uint32_t mask = __ballot_sync(0xffffffffu, here);
-          if (lane == 0) valid[4 * buf + dw] = mask;
+          const uint32_t mask_k = __ballot_sync(0xffffffffu, held);
+          const uint32_t mask_v = __ballot_sync(0xffffffffu, here && sums_hold(v));
+          const bool beyond = id >= kStep || (step0 + it) * kStep + id >= len;
+          const int all_fine = __all_sync(0xffffffffu, beyond || (held && sums_hold(v)));
+          const int e = static_cast<int>(__float_as_uint(v.inv_s) >> 23);  // 254 less the scale's
+          const int up = __reduce_max_sync(0xffffffffu, here ? 254 - e : -1000);
+          const int down = __reduce_min_sync(0xffffffffu, here ? 254 - e : 1000);
+          if (lane == 0) {
+            fine[4 * buf + dw] = all_fine;
+            range[8 * buf + dw] = up;
+            range[8 * buf + 4 + dw] = down;
+            valid[4 * buf + dw] = mask;
+            plain_k[4 * buf + dw] = mask_k;
+            plain_v[4 * buf + dw] = mask_v;
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(c_full + 8 * buf);
+          if (id < kStep) {
+            uint4 x[2];
+            key_terms<T>(held ? z : 0.f, held ? log : 0.f, x);
+            const uint32_t dst = smem_addr(smem) + Cfg::kOffKx + stage * Cfg::kKx + id * 32;
+            sts128(dst + ((id >> 2 & 1) << 4), x[0]);
+            sts128(dst + ((id >> 2 & 1 ^ 1) << 4), x[1]);
+          }
         }
         const uint32_t dst = smem_addr(smem) + Cfg::kOffK + stage * Cfg::kK;
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
           const int rest = (u * 128 + id) >> 3, chunk = rest % kUnits, half = rest / kUnits;
+          if (half >= 2 * kTiles) continue;
           const int key = half * 8 + (lane & 7);
           const uint32_t w[4] = {codes[u].x, codes[u].y, codes[u].z, codes[u].w};
 #pragma unroll
@@ -584,10 +742,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     } else {
       constexpr int kWordsV = D / 64;  // words of codes per token a thread
       const int half = (lane & 7) + 8 * (dw & 1), piece = (lane >> 3) + 4 * (dw >> 1);
+      const bool serves = half < 2 * kTiles;
+      uint32_t vp = 0;                 // of value `id`
+      bool here = false;
+      // the columns after the sums' are nothing
+      for (int i = id; i < 2 * 2 * 12 * 8; i += 128) {
+        const int chunk = i & 7, r = (i >> 3) % 12, atom = i / 96 & 1, stage = i / 192;
+        sts128(smem_addr(smem) + Cfg::kOffV + stage * Cfg::kV + atom * (kN * 128) + (D + 4 + r) * 128 + 16 * chunk,
+               make_uint4(0, 0, 0, 0));
+      }
       uint32_t w[8 * kWordsV];         // of the eight tokens of a half tile: [token][kWordsV]
       auto load = [&](int it) {
         if (it >= steps) return;
-        const uint8_t* src = tile_of(it, half >> 1);
+        const uint8_t* pair = id < kStep ? tile_of(it, id >> 4) : nullptr;
+        here = pair != nullptr && (step0 + it) * kStep + id < len;
+        vp = here ? *reinterpret_cast<const uint32_t*>(pair + off_v_pair(D, id & 15)) : 0u;
+        const uint8_t* src = serves ? tile_of(it, half >> 1) : nullptr;
 #pragma unroll
         for (int u = 0; u < 2 * kWordsV; ++u) {
           const uint4 x = src ? *reinterpret_cast<const uint4*>(src + off_v(D, (half & 1) * 8, piece) + 16 * u)
@@ -599,8 +769,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int it = 0; it < steps; ++it) {
         const int stage = it & 1;
         look_up(it + 2);
-        if (it >= 2) wait_warp(v_empty + 8 * stage, (it >> 1) - 1);
-        const uint32_t dst = smem_addr(smem) + Cfg::kOffV + stage * Cfg::kK;
+        if (it >= 2) wait_warp(spent + 8 * (stage ^ 1), (it - 1) >> 1);
+        const uint32_t dst = smem_addr(smem) + Cfg::kOffV + stage * Cfg::kV;
+        if (id < kStep) {
+          const ValueRow v = value_row(T::up(vp));
+          const bool held = here && sums_hold(v);
+          const float inv = held ? 0.25f * v.inv_s : 0.f, z = held ? v.at_8 : 0.f;
+          const float h = rounded<Half>(inv), zh = rounded<Half>(z);
+          const uint32_t x = Half::down(h, inv - h), y = Half::down(zh, z - zh);
+          const uint32_t at = dst + (id >> 6) * (kN * 128) + 2 * (id & 7);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint16_t number = static_cast<uint16_t>((r < 2 ? x : y) >> (16 * (r & 1)));
+            asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + (D + r) * 128 + (((id >> 3 & 7) ^ ((D + r) & 7)) << 4)),
+                         "h"(number)
+                         : "memory");
+          }
+        }
+        if (serves)
 #pragma unroll
         for (int o = 0; o < kWordsV; ++o) {
 #pragma unroll
@@ -615,7 +801,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             for (int x = 0; x < 2; ++x) {
               const int d = piece * (D / 8) + 8 * o + 2 * part + x;
               const half2* z = x ? odd : even;
-              sts128(dst + (half >> 3) * (D * 128) + d * 128 + (((half & 7) ^ (d & 7)) << 4),
+              sts128(dst + (half >> 3) * (kN * 128) + d * 128 + (((half & 7) ^ (d & 7)) << 4),
                      make_uint4(*reinterpret_cast<const uint32_t*>(&z[0]), *reinterpret_cast<const uint32_t*>(&z[1]),
                                 *reinterpret_cast<const uint32_t*>(&z[2]), *reinterpret_cast<const uint32_t*>(&z[3])));
             }
@@ -634,36 +820,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (lane == 0 && qi < tiles_q && steps > 0) {
       // ---------------------------------------------------------- products
       constexpr uint32_t types = T::kBf16 ? (1u << 7) | (1u << 10) : 0u;
-      constexpr uint32_t id_s = umma_idesc_f16_f32(kStep) | types, id_o = umma_idesc_f16_f32(D);
+      constexpr uint32_t id_s = umma_idesc_f16_f32(kStep) | types, id_o = umma_idesc_f16_f32(kN);
       const uint32_t base = smem_addr(smem);
-      const uint32_t s_at = tmem + Cfg::kColS + 128 * qi, o_at = tmem + Cfg::kColO + D * qi;
+      const uint32_t s_at = tmem + Cfg::kColS + kStep * qi, o_at = tmem + Cfg::kColO + kN * qi;
       auto scores = [&](int stage) {
         const uint64_t a = umma_desc_sw128_k(base + qi * Cfg::kQ);
         const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffK + stage * Cfg::kK);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
-          umma_f16(s_at, a + (at >> 4), bd + (at >> 4), id_s, k > 0);
+          umma_f16(s_at, a + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
+                   bd + (((k >> 2) * (kStep * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
         }
+        umma_f16(s_at, umma_desc_sw32_k(base + Cfg::kOffQx + qi * Cfg::kQx),
+                 umma_desc_sw32_k(base + Cfg::kOffKx + stage * Cfg::kKx), id_s, 1);
         umma_commit(s_full + 8 * qi);
-        umma_commit(k_empty + 8 * stage);
+        umma_commit(spent + 8 * stage);
       };
-      if (wait(q_ready + 8 * qi, 0) && wait(k_full, 0)) {
+      if (wait(q_ready + 8 * qi, 0) && wait(k_full, 0) && (qi == 0 || wait(second, 0))) {
         tc_fence_after();
         scores(0);
         for (int it = 0; it < steps; ++it) {
           const int stage = it & 1, next = (it + 1) & 1;
           if (!wait(v_full + 8 * stage, it >> 1) || !wait(p_ready + 8 * qi, it)) break;
           tc_fence_after();
-          const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kK);
+          const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kV);
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k) {
-            const uint32_t at = (k >> 2) * (D * 128) + (k & 3) * 32;
+            const uint32_t at = (k >> 2) * (kN * 128) + (k & 3) * 32;
             umma_f16_ts(o_at, s_at + 8 * k, bd + (at >> 4), id_o, it > 0 || k > 0);
           }
-          umma_commit(o_done + 8 * qi);
-          umma_commit(v_empty + 8 * stage);
-          if (it + 1 < steps) {
+          if (it + 1 == steps) {
+            umma_commit(spent + 8 * next);
+          } else {
             if (!wait(k_full + 8 * next, (it + 1) >> 1)) break;
             tc_fence_after();
             scores(next);
