@@ -455,8 +455,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       int largest = -1000;  // exponent of a value scale up to here
       for (int it = 0; it < steps; ++it) {
         const int buf = it & 3;
-        if (!wait_warp(c_full + 8 * buf, it >> 2) || !wait_warp(s_full + 8 * qi, it)) break;
-        tc_fence_after();
+        if (!wait_warp(c_full + 8 * buf, it >> 2)) break;
         const Numbers& k = numbers[buf];
         const int j0 = (step0 + it) * kStep;
         bool done = false;
@@ -468,6 +467,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int smallest = min(min(down.x, down.y), min(down.z, down.w));
         const int4 all_fine = *reinterpret_cast<const int4*>(fine + 4 * buf);
         const bool plain = usual && largest - smallest <= 6 && (all_fine.x & all_fine.y & all_fine.z & all_fine.w);
+        if (!wait_warp(s_full + 8 * qi, it)) break;
+        tc_fence_after();
         if (plain && it > 0 && j0 + kStep <= lo + 1 && (p.window == 0 || hi - j0 < p.window)) {
           // the step with the maximum as it is
           uint32_t weights[kStep / 2];
@@ -841,7 +842,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         scores(0);
         for (int it = 0; it < steps; ++it) {
           const int stage = it & 1, next = (it + 1) & 1;
-          if (!wait(v_full + 8 * stage, it >> 1) || !wait(p_ready + 8 * qi, it)) break;
+          const bool more = it + 1 < steps;
+          if (!wait(v_full + 8 * stage, it >> 1) || (more && !wait(k_full + 8 * next, (it + 1) >> 1)) ||
+              !wait(p_ready + 8 * qi, it))
+            break;
           tc_fence_after();
           const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kV);
 #pragma unroll
@@ -849,12 +853,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const uint32_t at = (k >> 2) * (kN * 128) + (k & 3) * 32;
             umma_f16_ts(o_at, s_at + 8 * k, bd + (at >> 4), id_o, it > 0 || k > 0);
           }
-          if (it + 1 == steps) {
-            umma_commit(spent + 8 * next);
-          } else {
-            if (!wait(k_full + 8 * next, (it + 1) >> 1)) break;
-            tc_fence_after();
+          if (more) {
             scores(next);
+          } else {
+            umma_commit(spent + 8 * next);
           }
         }
       }
