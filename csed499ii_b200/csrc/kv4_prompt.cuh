@@ -35,9 +35,8 @@
 // (a factor of 256), which is rare after the first steps.
 //
 // Four warps each turn key and value codes into operand tiles (two stages of
-// each), a thread per query tile issues its products (one thread issues one
-// every ~90 cycles, the tensor core could take one every 64), and four warps
-// per query tile do the softmax, one row a thread.  The second query tile starts
+// each), a warp per query tile issues its products, and four warps per query
+// tile do the softmax, one row a thread.  The second query tile starts
 // when the first one's first softmax is done, so that the products of one run
 // while the other is in its softmax.
 #pragma once
@@ -116,12 +115,31 @@ __device__ __forceinline__ uint64_t umma_desc_sw32_k(uint32_t saddr) {
   return d;
 }
 
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
-                                            uint32_t idesc, uint32_t accumulate) {
+// Products issued by a whole warp, of which one thread does it: where the code
+// around them does not diverge their operands stay in uniform registers (a
+// product of 128 x 144 x 16 every 74 cycles; issued from a branch of one lane,
+// every 160).
+__device__ __forceinline__ void warp_umma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void warp_umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same thread's: arrives on `bar` once all its products so far are done.
+__device__ __forceinline__ void warp_umma_commit(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
       : "memory");
 }
 
@@ -385,10 +403,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
-  auto wait = [&](uint32_t at, int phase) {  // one thread
-    ok = ok && mbar_wait_spin_sleep_bounded(at, phase & 1, abort_flag);
-    return ok;
-  };
   auto wait_warp = [&](uint32_t at, int phase) {
     ok = __all_sync(0xffffffffu, ok && mbar_wait_spin_sleep_bounded(at, phase & 1, abort_flag));
     return ok;
@@ -817,50 +831,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else {
     give_registers<kIssueRegs>();
-    const int qi = warp - 16;
-    if (lane == 0 && qi < tiles_q && steps > 0) {
+    const int qi = __shfl_sync(0xffffffffu, warp, 0) - 16;
+    if (qi < tiles_q && steps > 0) {
       // ---------------------------------------------------------- products
       constexpr uint32_t types = T::kBf16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t id_s = umma_idesc_f16_f32(kStep) | types, id_o = umma_idesc_f16_f32(kN);
-      const uint32_t base = smem_addr(smem);
-      const uint32_t s_at = tmem + Cfg::kColS + kStep * qi, o_at = tmem + Cfg::kColO + kN * qi;
+      const uint32_t base = smem_addr(smem), t0 = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t s_at = t0 + Cfg::kColS + kStep * qi, o_at = t0 + Cfg::kColO + kN * qi;
+      const uint64_t q_desc = umma_desc_sw128_k(base + qi * Cfg::kQ);
+      const uint64_t qx_desc = umma_desc_sw32_k(base + Cfg::kOffQx + qi * Cfg::kQx);
       auto scores = [&](int stage) {
-        const uint64_t a = umma_desc_sw128_k(base + qi * Cfg::kQ);
-        const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffK + stage * Cfg::kK);
+        const uint64_t k_desc = umma_desc_sw128_k(base + Cfg::kOffK + stage * Cfg::kK);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          umma_f16(s_at, a + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
-                   bd + (((k >> 2) * (kStep * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
-        }
-        umma_f16(s_at, umma_desc_sw32_k(base + Cfg::kOffQx + qi * Cfg::kQx),
-                 umma_desc_sw32_k(base + Cfg::kOffKx + stage * Cfg::kKx), id_s, 1);
-        umma_commit(s_full + 8 * qi);
-        umma_commit(spent + 8 * stage);
+        for (int k = 0; k < D / 16; ++k)
+          warp_umma_ss(s_at, q_desc + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
+                       k_desc + (((k >> 2) * (kStep * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
+        warp_umma_ss(s_at, qx_desc, umma_desc_sw32_k(base + Cfg::kOffKx + stage * Cfg::kKx), id_s, 1);
+        warp_umma_commit(s_full + 8 * qi);
+        warp_umma_commit(spent + 8 * stage);
       };
-      if (wait(q_ready + 8 * qi, 0) && wait(k_full, 0) && (qi == 0 || wait(second, 0))) {
+      if (wait_warp(q_ready + 8 * qi, 0) && wait_warp(k_full, 0) && (qi == 0 || wait_warp(second, 0))) {
         tc_fence_after();
         scores(0);
         for (int it = 0; it < steps; ++it) {
           const int stage = it & 1, next = (it + 1) & 1;
           const bool more = it + 1 < steps;
-          if (!wait(v_full + 8 * stage, it >> 1) || (more && !wait(k_full + 8 * next, (it + 1) >> 1)) ||
-              !wait(p_ready + 8 * qi, it))
+          if (!wait_warp(v_full + 8 * stage, it >> 1) || (more && !wait_warp(k_full + 8 * next, (it + 1) >> 1)) ||
+              !wait_warp(p_ready + 8 * qi, it))
             break;
           tc_fence_after();
-          const uint64_t bd = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kV);
+          const uint64_t v_desc = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kV);
 #pragma unroll
-          for (int k = 0; k < kStep / 16; ++k) {
-            const uint32_t at = (k >> 2) * (kN * 128) + (k & 3) * 32;
-            umma_f16_ts(o_at, s_at + 8 * k, bd + (at >> 4), id_o, it > 0 || k > 0);
-          }
+          for (int k = 0; k < kStep / 16; ++k)
+            warp_umma_ts(o_at, s_at + 8 * k, v_desc + (((k >> 2) * (kN * 128) + (k & 3) * 32) >> 4), id_o,
+                         it > 0 || k > 0);
           if (more) {
             scores(next);
           } else {
-            umma_commit(spent + 8 * next);
+            warp_umma_commit(spent + 8 * next);
           }
         }
       }
-      umma_commit(finished);
+      warp_umma_commit(finished);
       mbar_wait_bounded(finished, 0, drain_flag);
     }
   }
