@@ -25,6 +25,12 @@
 // figure below).  They are why a step is 112 keys: two tiles of scores and two
 // of 144 channels are all of tensor memory.
 //
+// What is left to bound it is shared memory: a product of 128 x 112 x 16 reads
+// 120 bytes a cycle.  So the scores are read in the fragment form of 16 lanes x
+// 8 columns, in which a thread has two neighbouring keys of four rows: one
+// 8-byte read of the keys' scales serves 8 products, where one row a thread
+// would take a broadcast for every key.
+//
 // Numbers that the terms cannot hold (a key's or value's scale out of the usual
 // range, a row of NaN) are added in 32 bits by a careful form of the step.  So
 // is what the weights lose in rounding to half where the values' scales differ
@@ -35,10 +41,9 @@
 // (a factor of 256), which is rare after the first steps.
 //
 // Four warps each turn key and value codes into operand tiles (two stages of
-// each), a warp per query tile issues its products, and four warps per query
-// tile do the softmax, one row a thread.  The second query tile starts
-// when the first one's first softmax is done, so that the products of one run
-// while the other is in its softmax.
+// each), four warps per query tile do the softmax, and one warp issues the
+// products, the first query tile's result and next scores before the second
+// one's: so each runs while the other is in its softmax.
 #pragma once
 
 #include <math_constants.h>
@@ -118,22 +123,59 @@ __device__ __forceinline__ uint64_t umma_desc_sw32_k(uint32_t saddr) {
 // Products issued by a whole warp, of which one thread does it: where the code
 // around them does not diverge their operands stay in uniform registers (a
 // product of 128 x 144 x 16 every 74 cycles; issued from a branch of one lane,
-// every 160).
+// every 160).  N products along 64 channels or keys, 32 bytes apart in both
+// operands (8 columns in tensor memory).
+template <int N>
 __device__ __forceinline__ void warp_umma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                              uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+  static_assert(N == 1 || N == 4, "products");
+  if constexpr (N == 1) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, q, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
+        "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
 }
+template <int N>
 __device__ __forceinline__ void warp_umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                              uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+  static_assert(N == 3 || N == 4, "products");
+  if constexpr (N == 3) {
+    asm volatile(
+        "{\n\t.reg .pred p, q, t;\n\t.reg .b64 b1, b2;\n\t.reg .b32 a1, a2;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "add.s32 a1, %1, 8;\n\tadd.s64 b1, %2, 2;\n\tadd.s32 a2, %1, 16;\n\tadd.s64 b2, %2, 4;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, q, t;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "add.s32 a1, %1, 8;\n\tadd.s64 b1, %2, 2;\n\tadd.s32 a2, %1, 16;\n\tadd.s64 b2, %2, 4;\n\t"
+        "add.s32 a3, %1, 24;\n\tadd.s64 b3, %2, 6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
 }
 // The same thread's: arrives on `bar` once all its products so far are done.
 __device__ __forceinline__ void warp_umma_commit(uint32_t bar) {
@@ -171,10 +213,33 @@ __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* v)
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
-               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
+// Fragments of 16 lanes: N groups of 8 columns as 32-bit numbers (a thread has
+// columns 2 (lane % 4) and the next of rows lane / 4 and lane / 4 + 8), and N
+// groups of 4 columns (column lane % 4 of the same rows).
+__device__ __forceinline__ void tmem_load_fragment(uint32_t taddr, uint32_t* r) {  // 16 columns
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+template <int N>
+__device__ __forceinline__ void tmem_store_fragment(uint32_t taddr, const uint32_t* v) {
+  if constexpr (N == 2) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3])
+                 : "memory");
+  } else if constexpr (N == 4) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    static_assert(N == 8, "groups");
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+  }
 }
 
 __device__ __forceinline__ void tmem_store_wait() {
@@ -328,7 +393,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   // `spent`, for step t in [0, steps]: result t - 1 and scores t are done with
   const uint32_t q_ready = bar, k_full = bar + 16, v_full = bar + 32, spent = bar + 48,
                  s_full = bar + 64, p_ready = bar + 80, c_full = bar + 96 /* four */,
-                 second = bar + 128, finished = bar + 136;
+                 finished = bar + 128;
   uint64_t* tile_at = bars + 24;                                        // keys' and values' [4][8]
   uint32_t* valid = reinterpret_cast<uint32_t*>(bars + 88);             // [4][4] keys that are there
   uint32_t* plain_k = valid + 16;                                       // ... whose numbers the terms hold
@@ -387,13 +452,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(q_ready + 8 * i, 4);
       mbar_init(k_full + 8 * i, 4);
       mbar_init(v_full + 8 * i, 4);
-      mbar_init(spent + 8 * i, tiles_q);
+      mbar_init(spent + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_ready + 8 * i, 4);
     }
     for (int i = 0; i < 4; ++i) mbar_init(c_full + 8 * i, 4);
-    mbar_init(second, 4);
-    mbar_init(finished, tiles_q);
+    mbar_init(finished, 1);
     *abort_flag = *drain_flag = 0;
     fence_mbar_init();
   }
@@ -404,7 +468,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
   auto wait_warp = [&](uint32_t at, int phase) {
-    ok = __all_sync(0xffffffffu, ok && mbar_wait_spin_sleep_bounded(at, phase & 1, abort_flag));
+    ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(at, phase & 1, abort_flag));
     return ok;
   };
 
@@ -460,12 +524,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t s_at = tmem + lanes + Cfg::kColS + kStep * qi;
       const uint32_t o_at = tmem + lanes + Cfg::kColO + kN * qi;
-      const int pos = before + token;
+      // this thread's rows of the scores: 8 i + lane / 4 of the warp's, i < 4
+      const int w0 = qi * 128 + (warp & 3) * 32, t2 = 2 * (lane & 3);
       // positions of this warp's first and last row
-      const int w0 = qi * 128 + (warp & 3) * 32;
       const int lo = before + (tile * 256 + w0) / p.group;
       const int hi = before + (tile * 256 + max(w0, min(rows, w0 + 32) - 1)) / p.group;
-      float top = kLowest, l = 0.f, off = 0.f;
+      // from a number of each of those rows to that of row `lane`
+      auto of_lane = [&](const float (&x)[4]) {
+        float y = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float z = __shfl_sync(0xffffffffu, x[i], (lane & 7) * 4);
+          if (lane >> 3 == i) y = z;
+        }
+        return y;
+      };
+      float top[4], l[4], off[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[i] = kLowest, l[i] = off[i] = 0.f;
       int largest = -1000;  // exponent of a value scale up to here
       for (int it = 0; it < steps; ++it) {
         const int buf = it & 3;
@@ -473,8 +549,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const Numbers& k = numbers[buf];
         const int j0 = (step0 + it) * kStep;
         bool done = false;
-        const uint32_t* in_k = plain_k + 4 * buf;
-        const uint32_t* in_v = plain_v + 4 * buf;
         const int4 up = *reinterpret_cast<const int4*>(range + 8 * buf);
         const int4 down = *reinterpret_cast<const int4*>(range + 8 * buf + 4);
         largest = max(largest, max(max(up.x, up.y), max(up.z, up.w)));
@@ -485,77 +559,121 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         tc_fence_after();
         if (plain && it > 0 && j0 + kStep <= lo + 1 && (p.window == 0 || hi - j0 < p.window)) {
           // the step with the maximum as it is
-          uint32_t weights[kStep / 2];
+          uint32_t weights[2][kStep / 4];  // of either 16 lanes
           float mx[2] = {kLowest, kLowest};
-          const F2 top2 = pack2(-top, -top);
+          F2 top2[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top2[i] = pack2(-top[i], -top[i]);
           uint32_t s[2][16];
-          tmem_load_16(s_at, s[0]);
+          tmem_load_fragment(s_at, s[0]);
+          tmem_load_fragment(s_at + (16u << 16), s[0] + 8);
 #pragma unroll
           for (int c = 0; c < kStep / 16; ++c) {
             tmem_loaded(s[c & 1]);
-            if (c + 1 < kStep / 16) tmem_load_16(s_at + 16 * (c + 1), s[(c + 1) & 1]);
+            if (c + 1 < kStep / 16) {
+              tmem_load_fragment(s_at + 16 * (c + 1), s[(c + 1) & 1]);
+              tmem_load_fragment(s_at + (16u << 16) + 16 * (c + 1), s[(c + 1) & 1] + 8);
+            }
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const float4 ks = *reinterpret_cast<const float4*>(k.scale + 16 * c + i);
-              const uint32_t* x = s[c & 1] + i;
-              const float2 y0 = unpack2(fma2(pack2(ks.x, ks.y), pack2(__uint_as_float(x[0]), __uint_as_float(x[1])), top2));
-              const float2 y1 = unpack2(fma2(pack2(ks.z, ks.w), pack2(__uint_as_float(x[2]), __uint_as_float(x[3])), top2));
-              mx[0] = max3(mx[0], y0.x, y0.y);
-              mx[1] = max3(mx[1], y1.x, y1.y);
-              weights[8 * c + i / 2] = Half::down(exp2_approx(y0.x), exp2_approx(y0.y));
-              weights[8 * c + i / 2 + 1] = Half::down(exp2_approx(y1.x), exp2_approx(y1.y));
+            for (int j = 0; j < 2; ++j) {
+              const float2 ks = *reinterpret_cast<const float2*>(k.scale + 16 * c + 8 * j + t2);
+              const F2 ks2 = pack2(ks.x, ks.y);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t* x = s[c & 1] + 8 * (i >> 1) + 4 * j + 2 * (i & 1);
+                const float2 y = unpack2(fma2(ks2, pack2(__uint_as_float(x[0]), __uint_as_float(x[1])), top2[i]));
+                mx[j] = max3(mx[j], y.x, y.y);
+                weights[i >> 1][4 * c + 2 * j + (i & 1)] = Half::down(exp2_approx(y.x), exp2_approx(y.y));
+              }
             }
           }
           done = !__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) > 8.f);
           if (done) {
 #pragma unroll
-            for (int c = 0; c < kStep / 32; ++c) tmem_store_16(s_at + 16 * c, weights + 16 * c);
-            if constexpr (kStep % 32 != 0) tmem_store_8(s_at + kStep / 32 * 16, weights + kStep / 32 * 16);
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t at = s_at + (i ? 16u << 16 : 0u);
+              tmem_store_fragment<8>(at, weights[i]);
+              if constexpr (kStep == 128) {
+                tmem_store_fragment<8>(at + 32, weights[i] + 16);
+              } else {
+                tmem_store_fragment<4>(at + 32, weights[i] + 16);
+                tmem_store_fragment<2>(at + 48, weights[i] + 24);
+              }
+            }
           }
         }
         if (!done) {
           // With the maximum of the step first.  What a row does not see has no
           // weight, whatever lies in its place.
-          const int oldest = p.window && pos >= p.window ? pos - p.window + 1 : 0;
-          const uint32_t seen = pos < 0 ? 0 : pos - oldest;          // keys before the last one
-          const int first_key = pos < 0 ? -1000 : j0 - oldest;       // a row before all keys sees none
-          auto argument = [&](int i, uint32_t s) {  // of key i of the step
-            if (static_cast<uint32_t>(first_key + i) > seen ||
-                !(valid[4 * buf + (i >> 5)] >> (i & 31) & 1))
-              return -CUDART_INF_F;
+          uint32_t seen[4];  // keys before the row's last one
+          int first_key[4];  // the step's, counted from the row's first one
+          float sums[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int pos = before + (tile * 256 + w0 + 8 * i + (lane >> 2)) / p.group;
+            const int oldest = p.window && pos >= p.window ? pos - p.window + 1 : 0;
+            seen[i] = pos < 0 ? 0 : pos - oldest;
+            first_key[i] = pos < 0 ? -1000 : j0 - oldest;  // a row before all keys sees none
+            sums[i] = __shfl_sync(0xffffffffu, sumq, 8 * i + (lane >> 2));
+          }
+          const uint32_t* in_k = plain_k + 4 * buf;
+          const uint32_t* in_v = plain_v + 4 * buf;
+          auto bit = [&](const uint32_t* mask, int i) { return mask[i >> 5] >> (i & 31) & 1; };
+          auto argument = [&](int r, int i, uint32_t s) {  // of key i of the step for row r
+            if (static_cast<uint32_t>(first_key[r] + i) > seen[r]) return -CUDART_INF_F;
             float x = __uint_as_float(s);
-            const bool held = in_k[i >> 5] >> (i & 31) & 1;
-            if (!held || big) x = fmaf(k.z[i], sumq, x);
+            if (!bit(valid + 4 * buf, i)) return -CUDART_INF_F;
+            const bool held = bit(in_k, i);
+            if (!held || !T::kBf16 && !(fabsf(sums[r]) < 60000.f)) x = fmaf(k.z[i], sums[r], x);
             return fmaf(k.scale[i], x, held ? 0.f : k.log_s[i]);
           };
-          auto plain_argument = [&](int i, uint32_t s, float scale) {
+          auto plain_argument = [&](int r, int i, uint32_t s, float scale) {
             const float x = __uint_as_float(s) * scale;
-            return static_cast<uint32_t>(first_key + i) > seen ? -CUDART_INF_F : x;
+            return static_cast<uint32_t>(first_key[r] + i) > seen[r] ? -CUDART_INF_F : x;
           };
-          float mx = kLowest;
+          float mx[4] = {kLowest, kLowest, kLowest, kLowest};
 #pragma unroll 1
           for (int c = 0; c < kStep / 16; ++c) {
             uint32_t s[16];
-            tmem_load_16(s_at + 16 * c, s);
+            tmem_load_fragment(s_at + 16 * c, s);
+            tmem_load_fragment(s_at + (16u << 16) + 16 * c, s + 8);
             tmem_loaded(s);
             if (plain) {
 #pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                const float4 ks = *reinterpret_cast<const float4*>(k.scale + 16 * c + i);
-                mx = max3(mx, plain_argument(16 * c + i, s[i], ks.x), plain_argument(16 * c + i + 1, s[i + 1], ks.y));
-                mx = max3(mx, plain_argument(16 * c + i + 2, s[i + 2], ks.z), plain_argument(16 * c + i + 3, s[i + 3], ks.w));
-              }
-            } else {
+              for (int j = 0; j < 2; ++j) {
+                const int at = 16 * c + 8 * j + t2;
+                const float2 ks = *reinterpret_cast<const float2*>(k.scale + at);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) mx = fmaxf(mx, argument(16 * c + i, s[i]));
+                for (int r = 0; r < 4; ++r) {
+                  const uint32_t* x = s + 8 * (r >> 1) + 4 * j + 2 * (r & 1);
+                  mx[r] = max3(mx[r], plain_argument(r, at, x[0], ks.x), plain_argument(r, at + 1, x[1], ks.y));
+                }
+              }
+            } else
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int r = 2 * (i >> 3) + (i >> 1 & 1);
+              mx[r] = fmaxf(mx[r], argument(r, 16 * c + 8 * (i >> 2 & 1) + t2 + (i & 1), s[i]));
             }
           }
-          if (__any_sync(0xffffffffu, mx > top + 8.f)) {
-            const float f = exp2_approx(top - fmaxf(top, mx));
-            top = fmaxf(top, mx);
-            l *= f;
-            off *= f;
+          bool moves = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+            moves |= mx[i] > top[i] + 8.f;
+          }
+          if (__any_sync(0xffffffffu, moves)) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f[i] = exp2_approx(top[i] - fmaxf(top[i], mx[i]));
+              top[i] = fmaxf(top[i], mx[i]);
+              l[i] *= f[i];
+              off[i] *= f[i];
+            }
             if (it > 0) {
+              const float fl = of_lane(f);
               if (!wait_warp(spent + 8 * (it & 1), it >> 1)) break;
               tc_fence_after();
 #pragma unroll 1
@@ -564,7 +682,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 tmem_load_16(o_at + 16 * c, o);
                 tmem_loaded(o);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fl);
                 tmem_store_16(o_at + 16 * c, o);
               }
             }
@@ -572,55 +690,72 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll 1
           for (int c = 0; c < kStep / 16; ++c) {
             uint32_t s[16];
-            tmem_load_16(s_at + 16 * c, s);
+            tmem_load_fragment(s_at + 16 * c, s);
+            tmem_load_fragment(s_at + (16u << 16) + 16 * c, s + 8);
             tmem_loaded(s);
             uint32_t weights[8];
             if (plain) {
 #pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                const float4 ks = *reinterpret_cast<const float4*>(k.scale + 16 * c + i);
-                weights[i / 2] = Half::down(exp2_approx(plain_argument(16 * c + i, s[i], ks.x) - top),
-                                            exp2_approx(plain_argument(16 * c + i + 1, s[i + 1], ks.y) - top));
-                weights[i / 2 + 1] = Half::down(exp2_approx(plain_argument(16 * c + i + 2, s[i + 2], ks.z) - top),
-                                                exp2_approx(plain_argument(16 * c + i + 3, s[i + 3], ks.w) - top));
+              for (int j = 0; j < 2; ++j) {
+                const int at = 16 * c + 8 * j + t2;
+                const float2 ks = *reinterpret_cast<const float2*>(k.scale + at);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const uint32_t* x = s + 8 * (r >> 1) + 4 * j + 2 * (r & 1);
+                  weights[4 * (r >> 1) + 2 * j + (r & 1)] =
+                      Half::down(exp2_approx(plain_argument(r, at, x[0], ks.x) - top[r]),
+                                 exp2_approx(plain_argument(r, at + 1, x[1], ks.y) - top[r]));
+                }
               }
             } else
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float x0 = argument(16 * c + i, s[i]), x1 = argument(16 * c + i + 1, s[i + 1]);
-              const float w0 = exp2_approx(x0 - top), w1 = exp2_approx(x1 - top);
-              weights[i / 2] = Half::down(w0, w1);
-              const float2 w = Half::up(weights[i / 2]);
+            for (int i = 0; i < 8; ++i) {
+              const int r = 2 * (i >> 2) + (i & 1), at = 16 * c + 8 * (i >> 1 & 1) + t2;
+              const float x0 = argument(r, at, s[2 * i]), x1 = argument(r, at + 1, s[2 * i + 1]);
+              const float w0 = exp2_approx(x0 - top[r]), w1 = exp2_approx(x1 - top[r]);
+              weights[4 * (i >> 2) + (i & 3)] = Half::down(w0, w1);
+              // what the sums' columns do not hold, or what the weights lose
+              const float2 w = Half::up(weights[4 * (i >> 2) + (i & 3)]);
 #pragma unroll
               for (int z = 0; z < 2; ++z) {
-                const int at = 16 * c + i + z;
-                const float r = (z ? w1 : w0) - (in_v[at >> 5] >> (at & 31) & 1 ? z ? w.y : w.x : 0.f);
+                const float rest = (z ? w1 : w0) - (bit(in_v, at + z) ? z ? w.y : w.x : 0.f);
                 if ((z ? x1 : x0) != -CUDART_INF_F) {
-                  l = fmaf(r, k.inv_s[at], l);
-                  off = fmaf(r, k.at_8[at], off);
+                  l[r] = fmaf(rest, k.inv_s[at + z], l[r]);
+                  off[r] = fmaf(rest, k.at_8[at + z], off[r]);
                 }
               }
             }
-            tmem_store_8(s_at + 8 * c, weights);  // in the place of products already read
+            // in the place of products already read
+            tmem_store_fragment<2>(s_at + 8 * c, weights);
+            tmem_store_fragment<2>(s_at + (16u << 16) + 8 * c, weights + 4);
           }
         }
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(p_ready + 8 * qi);
-          if (it == 0 && qi == 0) mbar_arrive(second);
-        }
+        if (lane == 0) mbar_arrive(p_ready + 8 * qi);
       }
-      if (steps > 0 && wait_warp(spent + 8 * (steps & 1), steps >> 1)) {
+      // from here on one row a thread
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int z = 1; z < 4; z <<= 1) {
+          l[i] += __shfl_xor_sync(0xffffffffu, l[i], z);
+          off[i] += __shfl_xor_sync(0xffffffffu, off[i], z);
+        }
+      float sum = of_lane(l), rest = of_lane(off);
+      // (the last phase of a `spent` can only be told from the one before the one
+      // before it once that one is over)
+      if (steps > 0 && wait_warp(spent + 8 * (steps - 1 & 1), (steps - 1) >> 1) &&
+          wait_warp(spent + 8 * (steps & 1), steps >> 1)) {
         tc_fence_after();
         uint32_t o[16];
         tmem_load_16(o_at + D, o);
         tmem_loaded(o);
-        l += 4.f * (__uint_as_float(o[0]) + __uint_as_float(o[1]));
-        off += __uint_as_float(o[2]) + __uint_as_float(o[3]);
+        sum += 4.f * (__uint_as_float(o[0]) + __uint_as_float(o[1]));
+        rest += __uint_as_float(o[2]) + __uint_as_float(o[3]);
       }
-      const float over = l == 0.f ? 0.f : 1.f / l;
+      const float over = sum == 0.f ? 0.f : 1.f / sum;
       uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(first + token) * p.q_heads + h) * D);
       if (ok) {
 #pragma unroll 1
@@ -634,8 +769,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            w[i] = l == 0.f ? 0u
-                            : T::down((__uint_as_float(o[2 * i]) + off) * over, (__uint_as_float(o[2 * i + 1]) + off) * over);
+            w[i] = sum == 0.f ? 0u
+                              : T::down((__uint_as_float(o[2 * i]) + rest) * over,
+                                        (__uint_as_float(o[2 * i + 1]) + rest) * over);
           *reinterpret_cast<uint4*>(dst + 32 * c) = make_uint4(w[0], w[1], w[2], w[3]);
           *reinterpret_cast<uint4*>(dst + 32 * c + 16) = make_uint4(w[4], w[5], w[6], w[7]);
         }
@@ -831,46 +967,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else {
     give_registers<kIssueRegs>();
-    const int qi = __shfl_sync(0xffffffffu, warp, 0) - 16;
-    if (qi < tiles_q && steps > 0) {
+    if (__shfl_sync(0xffffffffu, warp, 0) == 16 && steps > 0) {
       // ---------------------------------------------------------- products
       constexpr uint32_t types = T::kBf16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t id_s = umma_idesc_f16_f32(kStep) | types, id_o = umma_idesc_f16_f32(kN);
       const uint32_t base = smem_addr(smem), t0 = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint32_t s_at = t0 + Cfg::kColS + kStep * qi, o_at = t0 + Cfg::kColO + kN * qi;
-      const uint64_t q_desc = umma_desc_sw128_k(base + qi * Cfg::kQ);
-      const uint64_t qx_desc = umma_desc_sw32_k(base + Cfg::kOffQx + qi * Cfg::kQx);
-      auto scores = [&](int stage) {
+      auto scores = [&](int qi, int stage) {
+        const uint64_t q_desc = umma_desc_sw128_k(base + qi * Cfg::kQ);
         const uint64_t k_desc = umma_desc_sw128_k(base + Cfg::kOffK + stage * Cfg::kK);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          warp_umma_ss(s_at, q_desc + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
-                       k_desc + (((k >> 2) * (kStep * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
-        warp_umma_ss(s_at, qx_desc, umma_desc_sw32_k(base + Cfg::kOffKx + stage * Cfg::kKx), id_s, 1);
+        const uint32_t s_at = t0 + Cfg::kColS + kStep * qi;
+        warp_umma_ss<4>(s_at, q_desc, k_desc, id_s, 0);
+        if constexpr (D == 128) warp_umma_ss<4>(s_at, q_desc + (128 * 128 >> 4), k_desc + (kStep * 128 >> 4), id_s, 1);
+        warp_umma_ss<1>(s_at, umma_desc_sw32_k(base + Cfg::kOffQx + qi * Cfg::kQx),
+                     umma_desc_sw32_k(base + Cfg::kOffKx + stage * Cfg::kKx), id_s, 1);
         warp_umma_commit(s_full + 8 * qi);
-        warp_umma_commit(spent + 8 * stage);
       };
-      if (wait_warp(q_ready + 8 * qi, 0) && wait_warp(k_full, 0) && (qi == 0 || wait_warp(second, 0))) {
+      bool go = wait_warp(k_full, 0);
+      for (int qi = 0; qi < tiles_q && go; ++qi) {
+        go = wait_warp(q_ready + 8 * qi, 0);
+        if (!go) break;
         tc_fence_after();
-        scores(0);
-        for (int it = 0; it < steps; ++it) {
-          const int stage = it & 1, next = (it + 1) & 1;
-          const bool more = it + 1 < steps;
-          if (!wait_warp(v_full + 8 * stage, it >> 1) || (more && !wait_warp(k_full + 8 * next, (it + 1) >> 1)) ||
-              !wait_warp(p_ready + 8 * qi, it))
-            break;
+        scores(qi, 0);
+      }
+      warp_umma_commit(spent);
+      for (int it = 0; it < steps && go; ++it) {
+        const int stage = it & 1, next = (it + 1) & 1;
+        const bool more = it + 1 < steps;
+        go = wait_warp(v_full + 8 * stage, it >> 1) && (!more || wait_warp(k_full + 8 * next, (it + 1) >> 1));
+        for (int qi = 0; qi < tiles_q && go; ++qi) {
+          go = wait_warp(p_ready + 8 * qi, it);
+          if (!go) break;
           tc_fence_after();
           const uint64_t v_desc = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kV);
-#pragma unroll
-          for (int k = 0; k < kStep / 16; ++k)
-            warp_umma_ts(o_at, s_at + 8 * k, v_desc + (((k >> 2) * (kN * 128) + (k & 3) * 32) >> 4), id_o,
-                         it > 0 || k > 0);
-          if (more) {
-            scores(next);
-          } else {
-            warp_umma_commit(spent + 8 * next);
-          }
+          const uint32_t s_at = t0 + Cfg::kColS + kStep * qi, o_at = t0 + Cfg::kColO + kN * qi;
+          warp_umma_ts<4>(o_at, s_at, v_desc, id_o, it > 0);
+          warp_umma_ts<kStep / 16 - 4>(o_at, s_at + 32, v_desc + (kN * 128 >> 4), id_o, 1);
+          if (more) scores(qi, next);
         }
+        warp_umma_commit(spent + 8 * next);
       }
       warp_umma_commit(finished);
       mbar_wait_bounded(finished, 0, drain_flag);
