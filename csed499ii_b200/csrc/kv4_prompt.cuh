@@ -41,8 +41,9 @@
 // (a factor of 256), which is rare after the first steps.
 //
 // Four warps each turn key and value codes into operand tiles (two stages of
-// each), four warps per query tile do the softmax, and one warp issues the
-// products, the first query tile's result and next scores before the second
+// each), eight warps per query tile do the softmax (two for 32 rows: one has
+// the first 64 keys of a step, one the others, and they agree on whether the
+// maximum moves), and one warp issues the products, the first query tile's result and next scores before the second
 // one's: so each runs while the other is in its softmax.
 #pragma once
 
@@ -55,9 +56,9 @@ namespace sm100 {
 namespace kv4 {
 
 constexpr int kPromptBatch = 8192;  // requests of a launch
-constexpr int kPromptThreads = 20 * 32;
-// Registers a thread: 96 at launch, then as below (256 * 168 + 256 * 56 + 128 * 32 = 640 * 96).
-constexpr int kSoftmaxRegs = 168, kOperandRegs = 56, kIssueRegs = 32;
+constexpr int kPromptThreads = 28 * 32;
+// Registers a thread: 72 at launch, then as below (512 * 88 + 256 * 56 + 128 * 40 = 896 * 72).
+constexpr int kSoftmaxRegs = 88, kOperandRegs = 56, kIssueRegs = 40;
 
 struct PromptParams {
   Cache cache;
@@ -102,7 +103,8 @@ struct PromptCfg {
   static constexpr int kOffQx = kOffV + 2 * kV;
   static constexpr int kOffKx = kOffQx + 2 * kQx;
   static constexpr int kOffNumbers = kOffKx + 2 * kKx;  // four stages
-  static constexpr int kOffMisc = kOffNumbers + 4 * sizeof(Numbers);
+  static constexpr int kOffRows = kOffNumbers + 4 * sizeof(Numbers);  // [tile][half][row] of two numbers
+  static constexpr int kOffMisc = kOffRows + 2 * 2 * 128 * 8;
   static constexpr int kSmem = kOffMisc + 1280 + 1024;  // and room to align
   static_assert(kSmem <= kPrefillSmemBudget && kK % 1024 == 0 && kV % 1024 == 0 && kKx % 256 == 0, "tiles");
   static constexpr uint32_t kColS = 0, kColO = 2 * kStep, kCols = 512;
@@ -299,6 +301,18 @@ __device__ __forceinline__ void give_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// Whether any thread of the barrier's says so.
+__device__ __forceinline__ bool named_bar_any(int id, int threads, bool x) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<int>(x)), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -403,7 +417,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 140);
   volatile int* drain_flag = abort_flag + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 141);
-  int* sums = reinterpret_cast<int*>(bars + 142);                       // [20]
+  int* sums = reinterpret_cast<int*>(bars + 142);                       // [28]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.y;
 
@@ -449,19 +463,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_ready + 8 * i, 4);
+      mbar_init(q_ready + 8 * i, 8);
       mbar_init(k_full + 8 * i, 4);
       mbar_init(v_full + 8 * i, 4);
       mbar_init(spent + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_ready + 8 * i, 4);
+      mbar_init(p_ready + 8 * i, 8);
     }
     for (int i = 0; i < 4; ++i) mbar_init(c_full + 8 * i, 4);
     mbar_init(finished, 1);
     *abort_flag = *drain_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 16) tmem_alloc(smem_addr(tmem_slot), Cfg::kCols);
+  if (warp == 24) tmem_alloc(smem_addr(tmem_slot), Cfg::kCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -472,22 +486,32 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     return ok;
   };
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ------------------------------------------------------------- softmax
     take_registers<kSoftmaxRegs>();
-    const int qi = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int qi = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
     if (qi < tiles_q) {
       const int r = tile * 256 + qi * 128 + row;
       const int token = r / p.group, h = head * p.group + r % p.group;
       const bool live = qi * 128 + row < rows;
-      // this row of Q, its channels in the order that `centred` gives the codes
+      // the two warps of 32 rows meet here, and leave each other numbers there
+      const int meet = 1 + 4 * qi + (warp & 3);
+      float2* mine = reinterpret_cast<float2*>(smem + Cfg::kOffRows) + (2 * qi + half) * 128;
+      const float2* other = mine + (half ? -128 : 128);
+      // A wait that gave up ends both warps' work: neither may miss the other's barriers.
+      auto gave_up = [&]() {
+        ok = !named_bar_any(meet, 64, !ok);
+        return !ok;
+      };
+      // half of this row of Q, its channels in the order that `centred` gives the codes
       float sumq = 0.f;
       {
         const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) +
                               p.q_row * (first + token) + p.q_head * h;
         const uint32_t dst = smem_addr(smem) + qi * Cfg::kQ + row * 128;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
+        for (int i = 0; i < D / 16; ++i) {
+          const int c = half * (D / 16) + i;
           uint4 x = make_uint4(0, 0, 0, 0);
           if (live) {
             if (p.q_aligned) {
@@ -506,10 +530,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                  make_uint4(prmt(x.x, x.z, 0x5410), prmt(x.x, x.z, 0x7632), prmt(x.y, x.w, 0x5410),
                             prmt(x.y, x.w, 0x7632)));
         }
+        mine[row].x = sumq;
+        named_bar_sync(meet, 64);
+        sumq = half ? other[row].x + sumq : sumq + other[row].x;
       }
       // a sum that the terms cannot hold is left to the careful form
       const bool big = !T::kBf16 && !(fabsf(sumq) < 60000.f);
-      {
+      if (half == 0) {
         uint4 x[2];
         query_terms<T>(big ? 0.f : sumq, x);
         const uint32_t dst = smem_addr(smem) + Cfg::kOffQx + qi * Cfg::kQx + row * 32;
@@ -522,7 +549,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (lane == 0) mbar_arrive(q_ready + 8 * qi);
 
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + lanes + Cfg::kColS + kStep * qi;
+      constexpr int kRest = kStep / 16 - 4;  // chunks of 16 keys that the second half has; the first has four
+      const int chunks = half ? kRest : 4, key0 = 64 * half;
+      const uint32_t s_at = tmem + lanes + Cfg::kColS + kStep * qi + key0;
       const uint32_t o_at = tmem + lanes + Cfg::kColO + kN * qi;
       // this thread's rows of the scores: 8 i + lane / 4 of the warp's, i < 4
       const int w0 = qi * 128 + (warp & 3) * 32, t2 = 2 * (lane & 3);
@@ -545,7 +574,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       int largest = -1000;  // exponent of a value scale up to here
       for (int it = 0; it < steps; ++it) {
         const int buf = it & 3;
-        if (!wait_warp(c_full + 8 * buf, it >> 2)) break;
+        wait_warp(c_full + 8 * buf, it >> 2);
         const Numbers& k = numbers[buf];
         const int j0 = (step0 + it) * kStep;
         bool done = false;
@@ -555,49 +584,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int smallest = min(min(down.x, down.y), min(down.z, down.w));
         const int4 all_fine = *reinterpret_cast<const int4*>(fine + 4 * buf);
         const bool plain = usual && largest - smallest <= 6 && (all_fine.x & all_fine.y & all_fine.z & all_fine.w);
-        if (!wait_warp(s_full + 8 * qi, it)) break;
+        wait_warp(s_full + 8 * qi, it);
+        if (gave_up()) break;
         tc_fence_after();
         if (plain && it > 0 && j0 + kStep <= lo + 1 && (p.window == 0 || hi - j0 < p.window)) {
           // the step with the maximum as it is
-          uint32_t weights[2][kStep / 4];  // of either 16 lanes
+          uint32_t weights[2][16];  // of either 16 lanes
           float mx[2] = {kLowest, kLowest};
           F2 top2[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) top2[i] = pack2(-top[i], -top[i]);
-          uint32_t s[2][16];
-          tmem_load_fragment(s_at, s[0]);
-          tmem_load_fragment(s_at + (16u << 16), s[0] + 8);
 #pragma unroll
-          for (int c = 0; c < kStep / 16; ++c) {
-            tmem_loaded(s[c & 1]);
-            if (c + 1 < kStep / 16) {
-              tmem_load_fragment(s_at + 16 * (c + 1), s[(c + 1) & 1]);
-              tmem_load_fragment(s_at + (16u << 16) + 16 * (c + 1), s[(c + 1) & 1] + 8);
-            }
+          for (int c = 0; c < 4; ++c) {
+            if (c >= kRest && c >= chunks) break;
+            uint32_t s[16];
+            tmem_load_fragment(s_at + 16 * c, s);
+            tmem_load_fragment(s_at + (16u << 16) + 16 * c, s + 8);
+            tmem_loaded(s);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float2 ks = *reinterpret_cast<const float2*>(k.scale + 16 * c + 8 * j + t2);
+              const float2 ks = *reinterpret_cast<const float2*>(k.scale + key0 + 16 * c + 8 * j + t2);
               const F2 ks2 = pack2(ks.x, ks.y);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const uint32_t* x = s[c & 1] + 8 * (i >> 1) + 4 * j + 2 * (i & 1);
+                const uint32_t* x = s + 8 * (i >> 1) + 4 * j + 2 * (i & 1);
                 const float2 y = unpack2(fma2(ks2, pack2(__uint_as_float(x[0]), __uint_as_float(x[1])), top2[i]));
                 mx[j] = max3(mx[j], y.x, y.y);
                 weights[i >> 1][4 * c + 2 * j + (i & 1)] = Half::down(exp2_approx(y.x), exp2_approx(y.y));
               }
             }
           }
-          done = !__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) > 8.f);
+          done = !named_bar_any(meet, 64, fmaxf(mx[0], mx[1]) > 8.f);
           if (done) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t at = s_at + (i ? 16u << 16 : 0u);
-              tmem_store_fragment<8>(at, weights[i]);
-              if constexpr (kStep == 128) {
-                tmem_store_fragment<8>(at + 32, weights[i] + 16);
+              if (kRest == 4 || half == 0) {
+                tmem_store_fragment<8>(at, weights[i]);
               } else {
-                tmem_store_fragment<4>(at + 32, weights[i] + 16);
-                tmem_store_fragment<2>(at + 48, weights[i] + 24);
+                tmem_store_fragment<4>(at, weights[i]);
+                tmem_store_fragment<2>(at + 16, weights[i] + 8);
               }
             }
           }
@@ -633,7 +659,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           };
           float mx[4] = {kLowest, kLowest, kLowest, kLowest};
 #pragma unroll 1
-          for (int c = 0; c < kStep / 16; ++c) {
+          for (int c = 0; c < chunks; ++c) {
             uint32_t s[16];
             tmem_load_fragment(s_at + 16 * c, s);
             tmem_load_fragment(s_at + (16u << 16) + 16 * c, s + 8);
@@ -641,7 +667,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (plain) {
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                const int at = 16 * c + 8 * j + t2;
+                const int at = key0 + 16 * c + 8 * j + t2;
                 const float2 ks = *reinterpret_cast<const float2*>(k.scale + at);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -653,14 +679,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int r = 2 * (i >> 3) + (i >> 1 & 1);
-              mx[r] = fmaxf(mx[r], argument(r, 16 * c + 8 * (i >> 2 & 1) + t2 + (i & 1), s[i]));
+              mx[r] = fmaxf(mx[r], argument(r, key0 + 16 * c + 8 * (i >> 2 & 1) + t2 + (i & 1), s[i]));
             }
           }
           bool moves = false;
+          const int row0 = (warp & 3) * 32 + (lane >> 2);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+            if ((lane & 3) == 0) mine[row0 + 8 * i].y = mx[i];
+          }
+          named_bar_sync(meet, 64);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            mx[i] = fmaxf(mx[i], other[row0 + 8 * i].y);
             moves |= mx[i] > top[i] + 8.f;
           }
           if (__any_sync(0xffffffffu, moves)) {
@@ -674,10 +707,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             if (it > 0) {
               const float fl = of_lane(f);
-              if (!wait_warp(spent + 8 * (it & 1), it >> 1)) break;
+              wait_warp(spent + 8 * (it & 1), it >> 1);
+              if (gave_up()) break;
               tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < kN / 16; ++c) {
+              for (int c = half; c < kN / 16; c += 2) {
                 uint32_t o[16];
                 tmem_load_16(o_at + 16 * c, o);
                 tmem_loaded(o);
@@ -688,7 +722,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
           }
 #pragma unroll 1
-          for (int c = 0; c < kStep / 16; ++c) {
+          for (int c = 0; c < chunks; ++c) {
             uint32_t s[16];
             tmem_load_fragment(s_at + 16 * c, s);
             tmem_load_fragment(s_at + (16u << 16) + 16 * c, s + 8);
@@ -697,7 +731,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (plain) {
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                const int at = 16 * c + 8 * j + t2;
+                const int at = key0 + 16 * c + 8 * j + t2;
                 const float2 ks = *reinterpret_cast<const float2*>(k.scale + at);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -710,7 +744,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             } else
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const int r = 2 * (i >> 2) + (i & 1), at = 16 * c + 8 * (i >> 1 & 1) + t2;
+              const int r = 2 * (i >> 2) + (i & 1), at = key0 + 16 * c + 8 * (i >> 1 & 1) + t2;
               const float x0 = argument(r, at, s[2 * i]), x1 = argument(r, at + 1, s[2 * i + 1]);
               const float w0 = exp2_approx(x0 - top[r]), w1 = exp2_approx(x1 - top[r]);
               weights[4 * (i >> 2) + (i & 3)] = Half::down(w0, w1);
@@ -744,6 +778,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           off[i] += __shfl_xor_sync(0xffffffffu, off[i], z);
         }
       float sum = of_lane(l), rest = of_lane(off);
+      named_bar_sync(meet, 64);  // the other has read what is there
+      mine[row] = make_float2(sum, rest);
+      named_bar_sync(meet, 64);
+      sum = half ? other[row].x + sum : sum + other[row].x;
+      rest = half ? other[row].y + rest : rest + other[row].y;
       // (the last phase of a `spent` can only be told from the one before the one
       // before it once that one is over)
       if (steps > 0 && wait_warp(spent + 8 * (steps - 1 & 1), (steps - 1) >> 1) &&
@@ -759,7 +798,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(first + token) * p.q_heads + h) * D);
       if (ok) {
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
+        for (int c = half; c < D / 16; c += 2) {
           uint32_t o[16] = {};
           if (steps > 0) {
             tmem_load_16(o_at + 16 * c, o);
@@ -777,16 +816,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       }
     }
-  } else if (warp < 16) {
+  } else if (warp < 24) {
     // ------------------------------------------- codes to operand tiles
-    // Warps 8-11 the keys' (and what the softmax needs to know), 12-15 the
+    // Warps 16-19 the keys' (and what the softmax needs to know), 20-23 the
     // values'.  Codes are in registers a step ahead; where a step's tiles lie is
     // looked up two steps ahead.  Once a wait has given up these warps run on
     // without waiting: they meet at a barrier every step, which none of them
     // may leave alone.
     give_registers<kOperandRegs>();
-    const bool keys = warp < 12;
-    const int dw = warp & 3, id = dw * 32 + lane, meet = keys ? 1 : 2;
+    const bool keys = warp < 20;
+    const int dw = warp & 3, id = dw * 32 + lane, meet = keys ? 9 : 10;
     const int per_page = p.cache.page_size / kTile;
     uint64_t* tiles = tile_at + (keys ? 0 : 32);
     auto look_up = [&](int it) {  // where the step's cache tiles are
@@ -967,7 +1006,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else {
     give_registers<kIssueRegs>();
-    if (__shfl_sync(0xffffffffu, warp, 0) == 16 && steps > 0) {
+    if (__shfl_sync(0xffffffffu, warp, 0) == 24 && steps > 0) {
       // ---------------------------------------------------------- products
       constexpr uint32_t types = T::kBf16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t id_s = umma_idesc_f16_f32(kStep) | types, id_o = umma_idesc_f16_f32(kN);
@@ -1001,7 +1040,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const uint64_t v_desc = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kV);
           const uint32_t s_at = t0 + Cfg::kColS + kStep * qi, o_at = t0 + Cfg::kColO + kN * qi;
           warp_umma_ts<4>(o_at, s_at, v_desc, id_o, it > 0);
-          warp_umma_ts<kStep / 16 - 4>(o_at, s_at + 32, v_desc + (kN * 128 >> 4), id_o, 1);
+          warp_umma_ts<kStep / 16 - 4>(o_at, s_at + 64, v_desc + (kN * 128 >> 4), id_o, 1);
           if (more) scores(qi, next);
         }
         warp_umma_commit(spent + 8 * next);
@@ -1013,7 +1052,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (!ok && lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 24) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::kCols);
   }
