@@ -15,6 +15,7 @@ namespace sm100 {
 int cuda_fail(cudaError_t e);
 int kernel_status(int dev, int** out);  // device address of the status word
 int sm_count(int dev, int* sms);
+bool overlap_enabled();                 // programmatic launches (sm100_marlin_set_overlap)
 
 namespace {
 
@@ -36,9 +37,26 @@ struct OnDevice {
   }
 };
 
-int launched() {
-  const cudaError_t e = cudaGetLastError();
+int launched(cudaError_t e) {
+  if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? SM100_MARLIN_OK : cuda_fail(e);
+}
+
+// A launch that may begin while the kernel before it on the stream ends: every
+// kernel here waits for that one before it touches global memory.
+template <class Params>
+cudaError_t launch(void (*kernel)(Params), dim3 grid, int threads, int smem, cudaStream_t stream, const Params& p) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = overlap_enabled() ? 1 : 0;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, p);
 }
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -91,14 +109,15 @@ int launch_decode(DecodeParams p, int64_t most, int sms, int dev, cudaStream_t s
     const int n = batch - done < slice ? batch - done : slice;
     p.batch = n;
     p.pad = done + n == batch;
-    kv4_decode_kernel<T, D, NT><<<sms, Cfg::kThreads, Cfg::kSmem, stream>>>(p);
+    const cudaError_t e = launch(kv4_decode_kernel<T, D, NT>, dim3(sms), Cfg::kThreads, Cfg::kSmem, stream, p);
+    if (e != cudaSuccess) return cuda_fail(e);
     p.lens += n;
     p.tables += n * p.table_stride;
     p.row0 += n;
     if (p.starts) p.starts += n;
     done += n;
   } while (done < batch);
-  return launched();
+  return launched(cudaSuccess);
 }
 
 template <class T, int D>
@@ -112,14 +131,16 @@ int launch_prompt(PromptParams p, int dev, cudaStream_t stream) {
     p.batch = batch - done < kPromptBatch ? batch - done : kPromptBatch;
     const int64_t rests = rows / (p.most + 1);
     const int64_t items = rows / 256 + (rests < p.batch ? rests : p.batch);
-    if (items > 0)
-      kv4_prompt_kernel<T, D><<<dim3(static_cast<unsigned>(items), p.cache.heads), kPromptThreads,
-                                PromptCfg<D>::kSmem, stream>>>(p);
+    if (items > 0) {
+      const cudaError_t e = launch(kv4_prompt_kernel<T, D>, dim3(static_cast<unsigned>(items), p.cache.heads),
+                                   kPromptThreads, PromptCfg<D>::kSmem, stream, p);
+      if (e != cudaSuccess) return cuda_fail(e);
+    }
     p.lens += p.batch;
     p.tables += p.batch * p.table_stride;
     p.starts += p.batch;
   }
-  return launched();
+  return launched(cudaSuccess);
 }
 
 // f(T{}, std::integral_constant-like D) for the cache's type and head size.
@@ -167,9 +188,8 @@ int sm100_marlin_kv4_schedule(const int* new_lens, const int* lens, int* block_t
   // would read them while it writes.
   const bool in_place = lens_out == lens || free_count_out == free_count;
   const int ctas = in_place ? 1 : 1 + (rows > batch ? rows : batch) / 2048;
-  kv4_schedule_kernel<<<ctas < 148 ? ctas : 148, kScheduleThreads, smem,
-                        static_cast<cudaStream_t>(stream)>>>(p);
-  return launched();
+  return launched(launch(kv4_schedule_kernel, dim3(ctas < 148 ? ctas : 148), kScheduleThreads, smem,
+                         static_cast<cudaStream_t>(stream), p));
 }
 
 int sm100_marlin_kv4_append(const void* k, int64_t k_row, int64_t k_head, const void* v,
@@ -178,7 +198,7 @@ int sm100_marlin_kv4_append(const void* k, int64_t k_row, int64_t k_head, const 
                             int dev, void* stream) {
   const int bad = check_cache(cache, pages, kv_heads, page_size, head_dim, dtype);
   if (bad) return bad;
-  if (tokens < 0) return SM100_MARLIN_ERR_PROB_SHAPE;
+  if (tokens < 0 || static_cast<int64_t>(tokens) * kv_heads > 0x7fffffffll) return SM100_MARLIN_ERR_PROB_SHAPE;
   if (tokens == 0) return SM100_MARLIN_OK;
   if (!k || !v || !slots) return SM100_MARLIN_ERR_ARGUMENT;
   if (!aligned(k, 2) || !aligned(v, 2)) return SM100_MARLIN_ERR_ALIGNMENT;
@@ -188,11 +208,11 @@ int sm100_marlin_kv4_append(const void* k, int64_t k_row, int64_t k_head, const 
   const AppendParams p{{static_cast<uint8_t*>(cache), pages, kv_heads, page_size},
                        static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_row, k_head,
                        v_row, v_head, slots, tokens, vector};
-  const int64_t threads = 2ll * tokens * kv_heads * (head_dim / 8);
+  const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * (head_dim / 8);
   return dispatch(dtype, head_dim, [&](auto type, auto dim) {
-    kv4_append_kernel<decltype(type), decltype(dim)::value>
-        <<<static_cast<unsigned>((threads + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    return launched();
+    return launched(launch(kv4_append_kernel<decltype(type), decltype(dim)::value>,
+                           dim3(static_cast<unsigned>((threads + 255) / 256)), 256, 0,
+                           static_cast<cudaStream_t>(stream), p));
   });
 }
 
@@ -201,7 +221,7 @@ int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_s
                           void* stream) {
   const int bad = check_cache(cache, pages, kv_heads, page_size, head_dim, dtype);
   if (bad) return bad;
-  if (tokens < 0) return SM100_MARLIN_ERR_PROB_SHAPE;
+  if (tokens < 0 || static_cast<int64_t>(tokens) * kv_heads > 0x7fffffffll) return SM100_MARLIN_ERR_PROB_SHAPE;
   if (tokens == 0) return SM100_MARLIN_OK;
   if (!k || !v || !slots) return SM100_MARLIN_ERR_ARGUMENT;
   if (!aligned(k, 16) || !aligned(v, 16)) return SM100_MARLIN_ERR_ALIGNMENT;
@@ -209,11 +229,11 @@ int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_s
   if (on.error != cudaSuccess) return cuda_fail(on.error);
   const ReadParams p{{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, kv_heads, page_size},
                      static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), slots, tokens};
-  const int64_t threads = 2ll * tokens * kv_heads * (head_dim / 8);
+  const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * (head_dim / 8);
   return dispatch(dtype, head_dim, [&](auto type, auto dim) {
-    kv4_read_kernel<decltype(type), decltype(dim)::value>
-        <<<static_cast<unsigned>((threads + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    return launched();
+    return launched(launch(kv4_read_kernel<decltype(type), decltype(dim)::value>,
+                           dim3(static_cast<unsigned>((threads + 255) / 256)), 256, 0,
+                           static_cast<cudaStream_t>(stream), p));
   });
 }
 

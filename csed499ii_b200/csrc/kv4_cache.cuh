@@ -1,10 +1,11 @@
 // Writing keys and values into the 4-bit cache, and reading them back.
 // The layout and the rounding are those of kv4_format.cuh.
 //
-// Both are bound by memory.  A group of D/8 lanes owns one row (one token, one
-// head, keys or values): each lane holds 8 channels, 16 bytes, so a warp reads
-// 512 contiguous bytes an instruction; the row's range is a shuffle reduction,
-// and every lane's 8 codes are one 32-bit word of the tile.
+// Both are bound by memory: 4 D bytes of a token and head one way and D + 8 the
+// other.  A group of D/8 lanes owns one token and head, its key and its value
+// row: each lane holds 8 channels of both, so a warp has 1 KB of loads under
+// way; the rows' ranges are shuffle reductions, and a lane's 8 codes of a row
+// are one 32-bit word of the tile.
 #pragma once
 
 #include <math_constants.h>
@@ -34,7 +35,7 @@ struct ReadParams {
 
 // 8 channels as 4 words of two.
 __device__ __forceinline__ uint4 load_8(const uint8_t* p, bool aligned) {
-  if (aligned) return *reinterpret_cast<const uint4*>(p);
+  if (aligned) return __ldg(reinterpret_cast<const uint4*>(p));
   const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
   uint4 x;
   x.x = e[0] | static_cast<uint32_t>(e[1]) << 16;
@@ -44,101 +45,142 @@ __device__ __forceinline__ uint4 load_8(const uint8_t* p, bool aligned) {
   return x;
 }
 
+// The codes of this lane's 8 channels of a row of D/8 lanes, and the row's pair.
 template <class T, int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int kLanes = D / 8;  // of a row
-  const int lane = threadIdx.x & 31;
-  const int sub = lane % kLanes;
-  const int64_t rows = 2ll * p.tokens * p.cache.heads;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
-  // a warp's rows are adjacent; rows past the end repeat the last one without storing it
-  const bool live = row < rows;
-  const int64_t r = live ? row : rows - 1;
-  const bool is_v = r & 1;
-  const int token = static_cast<int>((r >> 1) / p.cache.heads);
-  const int head = static_cast<int>((r >> 1) - static_cast<int64_t>(token) * p.cache.heads);
-  const uint8_t* src = is_v ? p.v + 2 * (p.v_row * token + p.v_head * head)
-                            : p.k + 2 * (p.k_row * token + p.k_head * head);
-  const int slot = p.slots[token];
-  const uint4 raw = load_8(src + 16 * sub, p.aligned);
-  float x[8];
+__device__ __forceinline__ void quantise(const uint4& raw, uint32_t& codes, uint32_t& pair) {
+  constexpr int kLanes = D / 8;
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = T::up(w[i]);
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
   }
-  float lo = x[0], hi = x[0];
-  bool odd = false;  // an infinity or a NaN
+  float lo = x[0], hi = x[0], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
-    odd |= !(fabsf(x[i]) <= 3.402823466e38f);
+    sum = fmaf(x[i], 0.f, sum);  // 0, or a NaN for an infinity or a NaN
   }
 #pragma unroll
   for (int s = kLanes / 2; s > 0; s >>= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
   }
-  const uint32_t group = ((kLanes == 32 ? 0u : (1u << kLanes)) - 1u) << (lane - sub);
-  odd = (__ballot_sync(0xffffffffu, odd) & group) != 0;
-  const uint32_t pair_of_scale = T::down(__fdiv_rn(__fsub_rn(hi, lo), 15.f), lo);
-  const float scale = T::up(pair_of_scale).x;
+  const int lane = threadIdx.x & 31;
+  const uint32_t group = ((1u << kLanes) - 1u) << (lane / kLanes * kLanes);
+  bool odd = (__ballot_sync(0xffffffffu, !(sum == 0.f)) & group) != 0;
+  pair = T::down(__fdiv_rn(__fsub_rn(hi, lo), 15.f), lo);
+  const float scale = T::up(pair).x;
   odd |= !(scale <= 3.402823466e38f);
-  uint32_t codes = 0;
-  if (!odd && scale > 0.f) {
+  codes = 0;
+  if (odd) {
+    pair = T::down(CUDART_NAN_F, CUDART_NAN_F);
+  } else if (scale > 0.f) {
+    // The quotient rounded to binary32 decides a code.  Times the reciprocal it
+    // is within 2^-21 of 15; where that leaves the nearest integer open, and
+    // where the reciprocal is not a normal number, it is divided.
+    const float inv = __fdividef(1.f, scale);
+    bool near = !(inv < 1e37f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float c = rintf(__fdiv_rn(__fsub_rn(x[i], lo), scale));
+      const float q = __fmul_rn(__fsub_rn(x[i], lo), inv);
+      const float c = rintf(q);
+      near |= fabsf(fabsf(q - c) - 0.5f) < 1e-4f;
       codes |= static_cast<uint32_t>(fminf(c, 15.f)) << (4 * i);  // c >= 0: lo is the least x
     }
+    if (near) {
+      codes = 0;
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = T::up(i < 4 ? i < 2 ? raw.x : raw.y : i < 6 ? raw.z : raw.w);
+        const float c = rintf(__fdiv_rn(__fsub_rn(i & 1 ? f.y : f.x, lo), scale));
+        codes |= static_cast<uint32_t>(fminf(c, 15.f)) << (4 * i);
+      }
+    }
   }
-  const uint32_t pair = odd ? T::down(CUDART_NAN_F, CUDART_NAN_F) : pair_of_scale;
-  if (!live || static_cast<uint32_t>(slot) >= static_cast<uint32_t>(p.cache.pages) * p.cache.page_size)
+}
+
+// Where a lane's codes and a row's pair of a slot lie.
+template <int D>
+struct Place {
+  uint8_t* tile;
+  int k, v, at;
+
+  __device__ __forceinline__ Place(const Cache& cache, int slot, int head, int sub) {
+    const int page = slot / cache.page_size, place = slot - page * cache.page_size;
+    tile = cache.page_tiles<D>(page, head) + (place / kTile) * tile_bytes(D);
+    at = place % kTile;
+    k = off_k(D, at) + 4 * sub;
+    v = off_v(D, at, sub * 64 / D) + (D == 128 ? (sub & 1) * 4 : 0);
+  }
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kLanes = D / 8;  // of a row
+  grid_dependency_launch();
+  const int sub = threadIdx.x % kLanes;
+  const uint32_t rows = static_cast<uint32_t>(p.tokens) * p.cache.heads;
+  const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  // a warp's rows are adjacent; rows past the end repeat the last one without storing it
+  const uint32_t r = min(row, rows - 1);
+  const int token = r / p.cache.heads, head = r - token * p.cache.heads;
+  grid_dependency_wait();
+  const uint4 k = load_8(p.k + 2 * (p.k_row * token + p.k_head * head) + 16 * sub, p.aligned);
+  const uint4 v = load_8(p.v + 2 * (p.v_row * token + p.v_head * head) + 16 * sub, p.aligned);
+  const int slot = p.slots[token];
+  uint32_t k_codes, k_pair, v_codes, v_pair;
+  quantise<T, D>(k, k_codes, k_pair);
+  quantise<T, D>(v, v_codes, v_pair);
+  if (row >= rows || static_cast<uint32_t>(slot) >= static_cast<uint32_t>(p.cache.pages) * p.cache.page_size)
     return;
-  const int page = slot / p.cache.page_size, place = slot - page * p.cache.page_size;
-  uint8_t* tile = p.cache.page_tiles<D>(page, head) + (place / kTile) * tile_bytes(D);
-  const int at = place % kTile;
-  const int off = is_v ? off_v(D, at, sub * 8 / kLanes) + (D == 128 ? (sub & 1) * 4 : 0)
-                       : off_k(D, at) + 4 * sub;
-  *reinterpret_cast<uint32_t*>(tile + off) = codes;
-  if (sub == 0)
-    *reinterpret_cast<uint32_t*>(tile + (is_v ? off_v_pair(D, at) : off_k_pair(D, at))) = pair;
+  const Place<D> to(p.cache, slot, head, sub);
+  *reinterpret_cast<uint32_t*>(to.tile + to.k) = k_codes;
+  *reinterpret_cast<uint32_t*>(to.tile + to.v) = v_codes;
+  if (sub < 2)
+    *reinterpret_cast<uint32_t*>(to.tile + (sub ? off_v_pair(D, to.at) : off_k_pair(D, to.at))) =
+        sub ? v_pair : k_pair;
+}
+
+// What 8 codes stand for, in the model's type.
+template <class T>
+__device__ __forceinline__ uint4 values_of(uint32_t codes, uint32_t pair) {
+  const float2 so = T::up(pair);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = T::down(fmaf(static_cast<float>((codes >> (8 * i)) & 15u), so.x, so.y),
+                   fmaf(static_cast<float>((codes >> (8 * i + 4)) & 15u), so.x, so.y));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <class T, int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ ReadParams p) {
   constexpr int kLanes = D / 8;
+  grid_dependency_launch();
   const int sub = threadIdx.x % kLanes;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
-  if (row >= 2ll * p.tokens * p.cache.heads) return;
-  const bool is_v = row & 1;
-  const int64_t r = row >> 1;
-  const int token = static_cast<int>(r / p.cache.heads);
-  const int head = static_cast<int>(r - static_cast<int64_t>(token) * p.cache.heads);
+  const uint32_t rows = static_cast<uint32_t>(p.tokens) * p.cache.heads;
+  const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int token = row / p.cache.heads, head = row - token * p.cache.heads;
+  grid_dependency_wait();
+  if (row >= rows) return;
   const int slot = p.slots[token];
-  uint4 out = make_uint4(0, 0, 0, 0);
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
   if (static_cast<uint32_t>(slot) < static_cast<uint32_t>(p.cache.pages) * p.cache.page_size) {
-    const int page = slot / p.cache.page_size, place = slot - page * p.cache.page_size;
-    const uint8_t* tile = p.cache.page_tiles<D>(page, head) + (place / kTile) * tile_bytes(D);
-    const int at = place % kTile;
-    const int off = is_v ? off_v(D, at, sub * 8 / kLanes) + (D == 128 ? (sub & 1) * 4 : 0)
-                         : off_k(D, at) + 4 * sub;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(tile + off);
-    const float2 so = T::up(*reinterpret_cast<const uint32_t*>(
-        tile + (is_v ? off_v_pair(D, at) : off_k_pair(D, at))));
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = static_cast<float>((codes >> (8 * i)) & 15u);
-      const float b = static_cast<float>((codes >> (8 * i + 4)) & 15u);
-      w[i] = T::down(fmaf(a, so.x, so.y), fmaf(b, so.x, so.y));
-    }
-    out = make_uint4(w[0], w[1], w[2], w[3]);
+    const Place<D> at(p.cache, slot, head, sub);
+    const uint32_t k_codes = *reinterpret_cast<const uint32_t*>(at.tile + at.k);
+    const uint32_t v_codes = *reinterpret_cast<const uint32_t*>(at.tile + at.v);
+    const uint32_t k_pair = *reinterpret_cast<const uint32_t*>(at.tile + off_k_pair(D, at.at));
+    const uint32_t v_pair = *reinterpret_cast<const uint32_t*>(at.tile + off_v_pair(D, at.at));
+    k = values_of<T>(k_codes, k_pair);
+    v = values_of<T>(v_codes, v_pair);
   }
-  *reinterpret_cast<uint4*>((is_v ? p.v : p.k) + 2 * D * r + 16 * sub) = out;
+  const int64_t to = 2ll * D * row + 16 * sub;
+  __stcs(reinterpret_cast<uint4*>(p.k + to), k);
+  __stcs(reinterpret_cast<uint4*>(p.v + to), v);
 }
 
 }  // namespace kv4

@@ -325,6 +325,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
   if (threadIdx.x == 0) *abort_flag = *drain_flag = 0;
   fence_mbar_init();
 
+  grid_dependency_launch();
+  grid_dependency_wait();
+
   // --- the row of all steps: where each request's end is -------------------
   int total = 0;  // the host keeps it below 2^30
   int longest = 0, shortest = 0x7fffffff;  // items

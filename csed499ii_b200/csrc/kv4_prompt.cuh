@@ -421,6 +421,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.y;
 
+  grid_dependency_launch();
+  grid_dependency_wait();
+
   // --- which rows -------------------------------------------------------------
   int* pre = reinterpret_cast<int*>(smem);  // where the tiles will be
   int total = 0;

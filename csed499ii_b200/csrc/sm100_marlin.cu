@@ -206,6 +206,7 @@ int device_status_ptr(int dev, int** out) {
 
 int kernel_status(int dev, int** out) { return device_status_ptr(dev, out); }
 int sm_count(int dev, int* sms) { return device_sms(dev, sms); }
+bool overlap_enabled() { return pdl_enabled(); }
 
 namespace {
 
