@@ -105,6 +105,26 @@ def fast():
     return _fast
 
 
+_torch_fast = None
+_torch_fast_tried = False
+
+
+def torch_fast():
+    """The binding of the kv4 entry points that takes torch tensors
+    (``_torchfast``, built by ``build.build_torchfast``), or None when it has
+    not been built: callers then check and allocate in Python."""
+    global _torch_fast, _torch_fast_tried
+    if not _torch_fast_tried:
+        _torch_fast_tried = True
+        load()
+        try:
+            from . import _torchfast
+            _torch_fast = _torchfast
+        except ImportError:
+            _torch_fast = None
+    return _torch_fast
+
+
 def load(path: str = LIB_PATH):
     """Load (once) and return the library; raise if it is not built."""
     global _lib

@@ -147,6 +147,43 @@ def build_fastcall(force: bool = False) -> str:
     return FAST_PATH
 
 
+TORCH_FAST_NAME = "_torchfast" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so")
+TORCH_FAST_PATH = os.path.join(HERE, TORCH_FAST_NAME)
+
+
+def build_torchfast(force: bool = False) -> str:
+    """Compile the binding that takes torch tensors (csrc/torch_fast.cpp) next
+    to the package; like the CPython binding it links the library from _lib/."""
+    src = os.path.join(CSRC, "torch_fast.cpp")
+    hdr = os.path.join(ROOT, "include", "sm100_marlin.h")
+    if (not force and os.path.exists(TORCH_FAST_PATH)
+            and os.path.getmtime(TORCH_FAST_PATH) >= max(os.path.getmtime(src), os.path.getmtime(hdr),
+                                                         os.path.getmtime(LIB_PATH))):
+        return TORCH_FAST_PATH
+    import torch
+    from torch.utils import cpp_extension
+
+    cc = shutil.which("g++") or shutil.which("c++")
+    if cc is None:
+        raise RuntimeError("no C++ compiler for the torch binding")
+    tmp = TORCH_FAST_PATH + ".tmp"
+    cmd = [cc, "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", sysconfig.get_paths()["include"]]
+    for d in cpp_extension.include_paths("cuda"):
+        cmd += ["-isystem", d]
+    cmd += [src, "-o", tmp, "-L", LIB_DIR, "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN/_lib"]
+    for d in cpp_extension.library_paths():
+        cmd += ["-L", d]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("building the torch binding failed:\n" + res.stdout + res.stderr)
+    os.replace(tmp, TORCH_FAST_PATH)
+    return TORCH_FAST_PATH
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose=True, ptxas_info="--ptxas" in sys.argv)
     build_fastcall(force="--force" in sys.argv)
+    build_torchfast(force="--force" in sys.argv)

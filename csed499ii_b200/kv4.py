@@ -40,10 +40,7 @@ def _raise(name, err):
 
 
 def _entry(name):
-    """The C entry sm100_marlin_<name>: through the CPython binding, or through
-    ctypes where that has not been built."""
-    fast = _ext._fast if _ext._fast_tried else _ext.fast()
-    return getattr(_ext.load(), "sm100_marlin_" + name) if fast is None else getattr(fast, name)
+    return getattr(_ext.load(), "sm100_marlin_" + name)
 
 
 def _check_ints(name, t, dev, numel=None):
@@ -136,6 +133,14 @@ def kv4_schedule(new_lens, lens, block_tables, free_pages, free_count, rows, pag
         and ``free_count`` themselves are allowed (a step that is replayed from
         a CUDA graph updates them in place)
     """
+    fast = _ext._torch_fast if _ext._torch_fast_tried else _ext.torch_fast()
+    if fast is not None:
+        done = fast.kv4_schedule(new_lens, lens, block_tables, free_pages, free_count, rows, page_size,
+                                 lens_out, free_count_out)
+        if done is not None:
+            if done[0]:
+                _raise("kv4_schedule", done[0])
+            return KV4Step(*done[1:])
     dev = new_lens.get_device()
     batch, tables_shape = new_lens.numel(), block_tables.shape
     # one combined test; the checks with their messages only run when it fails
@@ -199,6 +204,13 @@ def kv4_append(k, v, cache, slots):
     @slots: ``torch.int`` ``(tokens,)``, no slot twice; rows whose slot is
         outside the cache (-1) are skipped
     """
+    fast = _ext._torch_fast if _ext._torch_fast_tried else _ext.torch_fast()
+    if fast is not None:
+        err = fast.kv4_append(k, v, cache, slots)
+        if err == 0:
+            return
+        if err is not None:
+            _raise("kv4_append", err)
     pages, heads, page_size, dim, dtype, dev = _cache_shape(cache)
     shape, k_at, v_at, kind = k.shape, k.stride(), v.stride(), cache.dtype
     tokens = shape[0] if shape else 0
@@ -221,6 +233,13 @@ def kv4_append(k, v, cache, slots):
 def kv4_read(cache, slots):
     """Keys and values at ``slots``, each ``(tokens, kv_heads, head_dim)`` in the
     cache's type; zeros where a slot is outside the cache."""
+    fast = _ext._torch_fast if _ext._torch_fast_tried else _ext.torch_fast()
+    if fast is not None:
+        done = fast.kv4_read(cache, slots)
+        if done is not None:
+            if done[0]:
+                _raise("kv4_read", done[0])
+            return done[1], done[2]
     pages, heads, page_size, dim, dtype, dev = _cache_shape(cache)
     _check_ints("slots", slots, dev)
     tokens = slots.numel()
@@ -254,6 +273,13 @@ def _workspace(dev, stream):
     return found
 
 
+def _attention_error(err, dev):
+    if err == _ext.ERR_SCRATCH:
+        need = _ext.load().sm100_marlin_kv4_workspace_bytes(dev) // 4
+        raise RuntimeError(f"workspace must be of size at least {need}.")
+    _raise("kv4_attention", err)
+
+
 def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, window=0, scale=None,
                   out=None, workspace=None):
     """Attention of each request's last tokens over what it has in the cache.
@@ -272,6 +298,17 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
     @workspace: :func:`kv4_workspace`; None: one that the module keeps for the
         current stream
     """
+    fast = _ext._torch_fast if _ext._torch_fast_tried else _ext.torch_fast()
+    if fast is not None and out is None and cache.is_cuda:
+        space = workspace
+        if space is None:
+            dev = cache.get_device()
+            space = _workspace(dev, _stream_ptr(dev))
+        done = fast.kv4_attention(q, cache, block_tables, lens, starts, max_new, window, scale, space)
+        if done is not None:
+            if done[0]:
+                _attention_error(done[0], cache.get_device())
+            return done[1]
     pages, heads, page_size, dim, dtype, dev = _cache_shape(cache)
     shape, at, tables_shape, batch = q.shape, q.stride(), block_tables.shape, lens.numel()
     if not (q.dtype is cache.dtype and q.get_device() == dev and len(shape) == 3 and shape[2] == dim
@@ -309,9 +346,6 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
         block_tables.data_ptr(), block_tables.stride(0), tables_shape[1], lens.data_ptr(), starts_at,
         batch, rows, q_heads, max_new, window, dim**-0.5 if scale is None else scale, out.data_ptr(),
         workspace.data_ptr(), 4 * workspace.numel(), dev, stream)
-    if err == _ext.ERR_SCRATCH:
-        need = _ext.load().sm100_marlin_kv4_workspace_bytes(dev) // 4
-        raise RuntimeError(f"workspace must be of size at least {need}.")
     if err:
-        _raise("kv4_attention", err)
+        _attention_error(err, dev)
     return out
