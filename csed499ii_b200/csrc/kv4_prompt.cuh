@@ -78,8 +78,15 @@ struct PromptParams {
   int window;            // 0: none
   int most;              // requests with at most this many query rows a group are left alone
   float scale;
+  int split;             // CTAs of a head that the keys of its items may be shared out over; 0: they are not
+  float* partials;       // [CTAs] parts of items that are
   int* status;
 };
+
+constexpr int kSplitBatch = 1024;  // requests of a launch that shares out keys
+// Steps of a CTA where keys are shared out: an item costs a CTA about as much as
+// four steps before and after its own.
+constexpr int kLeastPromptSteps = 4;
 
 // What the careful form of a step needs to know of its keys (the usual one
 // reads the scales alone).
@@ -392,6 +399,69 @@ __device__ __forceinline__ bool sums_hold(const ValueRow& v) {
   return v.inv_s >= 0x1p-7f && v.inv_s <= 0x1p17f && fabsf(v.at_8) < 60000.f;
 }
 
+// Inclusive prefix sums of the requests' items in `pre`, and their total.
+template <int Threads>
+__device__ __forceinline__ int prompt_prefix(const PromptParams& p, int* pre, int* sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int total = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += Threads) {
+    const int b = b0 + threadIdx.x;
+    int x = b < p.batch ? prompt_items(p, b) : 0;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, i);
+      if (lane >= i) x += y;
+    }
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    int all = 0;
+    for (int i = 0; i < Threads / 32; ++i) {
+      if (i == warp) x += all;
+      all += sums[i];
+    }
+    if (b < p.batch) pre[b] = total + x;
+    total += all;
+    __syncthreads();
+  }
+  return total;
+}
+
+// 256 query rows of a request, and the keys that any of them sees.
+struct PromptItem {
+  int b, tile;
+  int first, n, len;     // the request's rows and tokens
+  int rows;              // of the item
+  int before;            // position of the request's row 0
+  int step0, steps;
+};
+template <int Step>
+__device__ __forceinline__ PromptItem prompt_item(const PromptParams& p, const int* pre, int item) {
+  PromptItem x;
+  x.b = first_above(pre, p.batch, item);
+  x.tile = item - (x.b ? pre[x.b - 1] : 0);
+  x.first = min(max(p.starts[x.b], 0), p.rows);
+  x.n = min(p.starts[x.b + 1], p.rows) - x.first;
+  const int64_t room = static_cast<int64_t>(p.width) * p.cache.page_size;
+  x.len = static_cast<int>(min(static_cast<int64_t>(p.lens[x.b]), room));
+  x.rows = min(256, x.n * p.group - x.tile * 256);
+  x.before = x.len - x.n;
+  const int lo = x.before + x.tile * 256 / p.group, hi = x.before + (x.tile * 256 + x.rows - 1) / p.group;
+  const int from = p.window && lo >= p.window ? lo - p.window + 1 : 0;
+  const int to = min(x.len, hi + 1);
+  x.step0 = from / Step;
+  x.steps = to > from ? (to + Step - 1) / Step - x.step0 : 0;
+  return x;
+}
+
+// How an item's steps are shared out over at most `most` CTAs.
+struct Shares {
+  int parts, steps;  // of a part
+  __device__ __forceinline__ Shares(int all, int most) {
+    steps = max((all + most - 1) / most, min(all, kLeastPromptSteps));
+    parts = steps ? (all + steps - 1) / steps : 1;
+  }
+};
+
 template <class T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     kv4_prompt_kernel(const __grid_constant__ PromptParams p) {
@@ -417,7 +487,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 140);
   volatile int* drain_flag = abort_flag + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 141);
-  int* sums = reinterpret_cast<int*>(bars + 142);                       // [28]
+  volatile int* after = reinterpret_cast<volatile int*>(bars + 142);    // [4]
+  int* sums = reinterpret_cast<int*>(bars + 144);                       // [28]
+  static_assert((144 + 14) * 8 <= 1280, "shared memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.y;
 
@@ -426,42 +498,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   // --- which rows -------------------------------------------------------------
   int* pre = reinterpret_cast<int*>(smem);  // where the tiles will be
-  int total = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kPromptThreads) {
-    const int b = b0 + threadIdx.x;
-    int x = b < p.batch ? prompt_items(p, b) : 0;
-#pragma unroll
-    for (int i = 1; i < 32; i <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, i);
-      if (lane >= i) x += y;
-    }
-    if (lane == 31) sums[warp] = x;
-    __syncthreads();
-    int all = 0;
-    for (int i = 0; i < kPromptThreads / 32; ++i) {
-      if (i == warp) x += all;
-      all += sums[i];
-    }
-    if (b < p.batch) pre[b] = total + x;
-    total += all;
-    __syncthreads();
-  }
+  const int total = prompt_prefix<kPromptThreads>(p, pre, sums);
+  const int most = p.split && total ? max(gridDim.x / total, 1u) : 1;  // CTAs of an item
   // the last items first: within a request they have the most keys
-  const int item = total - 1 - static_cast<int>(blockIdx.x);
+  const int item = total - 1 - static_cast<int>(blockIdx.x) / most, share = blockIdx.x % most;
   if (item < 0) return;
-  const int b = first_above(pre, p.batch, item);
-  const int tile = item - (b ? pre[b - 1] : 0);
-  const int first = min(max(p.starts[b], 0), p.rows), n = min(p.starts[b + 1], p.rows) - first;
-  const int64_t room = static_cast<int64_t>(p.width) * p.cache.page_size;
-  const int len = static_cast<int>(min(static_cast<int64_t>(p.lens[b]), room));
-  const int rows = min(256, n * p.group - tile * 256);
+  const PromptItem x = prompt_item<kStep>(p, pre, item);
+  const int b = x.b, tile = x.tile, first = x.first, len = x.len, rows = x.rows, before = x.before;
   const int tiles_q = rows > 128 ? 2 : 1;
-  const int before = len - n;  // position of the request's row 0
-  const int lo_pos = before + tile * 256 / p.group, hi_pos = before + (tile * 256 + rows - 1) / p.group;
-  const int from = p.window && lo_pos >= p.window ? lo_pos - p.window + 1 : 0;
-  const int to = min(len, hi_pos + 1);
-  const int step0 = from / kStep;
-  const int steps = to > from ? (to + kStep - 1) / kStep - step0 : 0;
+  const Shares shares(x.steps, most);
+  if (share >= shares.parts) return;
+  const int step0 = x.step0 + share * shares.steps, steps = min(shares.steps, x.steps - share * shares.steps);
   __syncthreads();  // `pre` is read
 
   if (threadIdx.x == 0) {
@@ -476,6 +523,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int i = 0; i < 4; ++i) mbar_init(c_full + 8 * i, 4);
     mbar_init(finished, 1);
     *abort_flag = *drain_flag = 0;
+    // for the end of the softmax warps, whose registers are few
+    after[0] = shares.parts, after[1] = first, after[2] = tile * 256, after[3] = rows;
     fence_mbar_init();
   }
   if (warp == 24) tmem_alloc(smem_addr(tmem_slot), Cfg::kCols);
@@ -798,7 +847,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         rest += __uint_as_float(o[2]) + __uint_as_float(o[3]);
       }
       const float over = sum == 0.f ? 0.f : 1.f / sum;
-      uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(first + token) * p.q_heads + h) * D);
+      const bool whole = after[0] == 1, there = qi * 128 + row < after[3];
+      const int at = after[2] + qi * 128 + row, at_token = at / p.group;
+      uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(after[1] + at_token) * p.q_heads + head * p.group + at -
+                                   at_token * p.group) * D);
+      // a part: [16 channels][row][16] results, the rows' maxima and sums
+      float* part = p.partials + (blockIdx.y * gridDim.x + blockIdx.x) * (256 * (D + 2)) + qi * 128 + row;
+      const float highest = of_lane(top);
+      if (!whole && half == 0) {
+        part[256 * D] = highest;
+        part[256 * (D + 1)] = sum;
+      }
+      part += 15 * (qi * 128 + row);
       if (ok) {
 #pragma unroll 1
         for (int c = half; c < D / 16; c += 2) {
@@ -807,7 +867,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             tmem_load_16(o_at + 16 * c, o);
             tmem_loaded(o);
           }
-          if (!live) continue;
+          if (!there) continue;
+          if (!whole) {
+            float4* to = reinterpret_cast<float4*>(part + c * (256 * 16));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (sum != 0.f)
+                y = make_float4((__uint_as_float(o[4 * i]) + rest) * over, (__uint_as_float(o[4 * i + 1]) + rest) * over,
+                                (__uint_as_float(o[4 * i + 2]) + rest) * over,
+                                (__uint_as_float(o[4 * i + 3]) + rest) * over);
+              to[i] = y;
+            }
+            continue;
+          }
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i)
@@ -1059,6 +1132,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::kCols);
   }
+}
+
+// The parts of items whose keys were shared out: a thread joins 16 channels of a
+// row, a CTA 32 rows.
+template <class T, int D>
+__global__ void __launch_bounds__(2 * D) kv4_prompt_join_kernel(const __grid_constant__ PromptParams p) {
+  __shared__ int pre[kSplitBatch], sums[2 * D / 32];
+  grid_dependency_launch();
+  grid_dependency_wait();
+  const int total = prompt_prefix<2 * D>(p, pre, sums);
+  const int item = total - 1 - static_cast<int>(blockIdx.x / 8);
+  if (item < 0) return;
+  // gridDim.x is 8 times the most items there can be; the other kernel's is p.split
+  const int most = max(p.split / total, 1);
+  const PromptItem x = prompt_item<PromptCfg<D>::kStep>(p, pre, item);
+  const Shares shares(x.steps, most);
+  const int row = blockIdx.x % 8 * 32 + threadIdx.x % 32, c = threadIdx.x / 32;
+  if (shares.parts < 2 || row >= x.rows) return;
+  constexpr int kPart = 256 * (D + 2);
+  const float* part = p.partials + (static_cast<int>(blockIdx.y) * p.split + (total - 1 - item) * most) * kPart;
+  float top = kLowest;
+#pragma unroll 8
+  for (int i = 0; i < shares.parts; ++i) top = fmaxf(top, __ldcg(part + i * kPart + 256 * D + row));
+  float y[16] = {}, sum = 0.f;
+#pragma unroll 2
+  for (int i = 0; i < shares.parts; ++i) {
+    const float* at = part + i * kPart;
+    const float w = __ldcg(at + 256 * (D + 1) + row) * exp2_approx(__ldcg(at + 256 * D + row) - top);
+    sum += w;
+    const float4* from = reinterpret_cast<const float4*>(at + (c * 256 + row) * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = __ldcg(from + j);
+      y[4 * j] = fmaf(w, v.x, y[4 * j]), y[4 * j + 1] = fmaf(w, v.y, y[4 * j + 1]);
+      y[4 * j + 2] = fmaf(w, v.z, y[4 * j + 2]), y[4 * j + 3] = fmaf(w, v.w, y[4 * j + 3]);
+    }
+  }
+  const float over = sum == 0.f ? 0.f : 1.f / sum;
+  const int r = x.tile * 256 + row, token = r / p.group, h = blockIdx.y * p.group + r % p.group;
+  uint4* dst = reinterpret_cast<uint4*>(
+      p.out + 2 * ((static_cast<int64_t>(x.first + token) * p.q_heads + h) * D + 16 * c));
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    dst[j] = make_uint4(T::down(y[8 * j] * over, y[8 * j + 1] * over), T::down(y[8 * j + 2] * over, y[8 * j + 3] * over),
+                        T::down(y[8 * j + 4] * over, y[8 * j + 5] * over),
+                        T::down(y[8 * j + 6] * over, y[8 * j + 7] * over));
 }
 
 }  // namespace kv4

@@ -338,6 +338,19 @@ def test_whole_prompts(m, dim, heads, group):
     p.check(m.kv4_attention(p.q, p.cache, p.tables, ints(lens), starts=ints(p.starts), max_new=1000))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,new,heads,group,window", [
+    ([20000], [9], 1, 8, 0), ([5000, 0, 3, 9000], [100, 0, 3, 40], 2, 4, 0),
+    ([5000, 1200, 3, 9000], [100, 300, 3, 40], 2, 4, 2500), ([7001, 6000], [1, 130], 3, 5, 1000)])
+def test_few_rows_of_many_keys(m, dtype, dim, lens, new, heads, group, window):
+    p = Problem(m, lens, new, heads, group, dim, 32, dtype, seed=sum(new), pad=2)
+    for most in (max(new), None):
+        out = m.kv4_attention(p.q, p.cache, p.tables, ints(lens), starts=ints(p.starts), max_new=most,
+                              window=window)
+        p.check(out, window)
+
+
 @pytest.mark.parametrize("lens", [[20000], [1, 30000, 5], [4097] * 3, [100] * 200])
 @pytest.mark.parametrize("heads,group", [(1, 1), (2, 8)])
 def test_work_of_uneven_lengths(m, lens, heads, group):
