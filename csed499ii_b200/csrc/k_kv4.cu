@@ -201,7 +201,7 @@ int sm100_marlin_kv4_schedule(const int* new_lens, const int* lens, int* block_t
   // One CTA where the lengths or the count are updated in place: the others
   // would read them while it writes.
   const bool in_place = lens_out == lens || free_count_out == free_count;
-  const int ctas = in_place ? 1 : 1 + (rows > batch ? rows : batch) / 2048;
+  const int ctas = in_place ? 1 : 1 + (rows > batch ? rows : batch) / kScheduleThreads;
   return launched(launch(kv4_schedule_kernel, dim3(ctas < 148 ? ctas : 148), kScheduleThreads, smem,
                          static_cast<cudaStream_t>(stream), p));
 }
@@ -222,10 +222,10 @@ int sm100_marlin_kv4_append(const void* k, int64_t k_row, int64_t k_head, const 
   const AppendParams p{{static_cast<uint8_t*>(cache), pages, kv_heads, page_size},
                        static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_row, k_head,
                        v_row, v_head, slots, tokens, vector};
-  const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * (head_dim / 8);
+  const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * kRowLanes;
   return dispatch(dtype, head_dim, [&](auto type, auto dim) {
     return launched(launch(kv4_append_kernel<decltype(type), decltype(dim)::value>,
-                           dim3(static_cast<unsigned>((threads + 255) / 256)), 256, 0,
+                           dim3(static_cast<unsigned>((threads + kCacheThreads - 1) / kCacheThreads)), kCacheThreads, 0,
                            static_cast<cudaStream_t>(stream), p));
   });
 }
@@ -243,10 +243,10 @@ int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_s
   if (on.error != cudaSuccess) return cuda_fail(on.error);
   const ReadParams p{{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, kv_heads, page_size},
                      static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), slots, tokens};
-  const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * (head_dim / 8);
+  const int64_t threads = static_cast<int64_t>(tokens) * kv_heads * kRowLanes;
   return dispatch(dtype, head_dim, [&](auto type, auto dim) {
     return launched(launch(kv4_read_kernel<decltype(type), decltype(dim)::value>,
-                           dim3(static_cast<unsigned>((threads + 255) / 256)), 256, 0,
+                           dim3(static_cast<unsigned>((threads + kCacheThreads - 1) / kCacheThreads)), kCacheThreads, 0,
                            static_cast<cudaStream_t>(stream), p));
   });
 }

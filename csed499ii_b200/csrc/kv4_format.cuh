@@ -62,9 +62,42 @@ struct Cache {
   }
 };
 
+// Two floats in one register pair, for the two-wide instructions.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(F2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // The two 16-bit types of a model.
 struct Half {
   static constexpr bool kBf16 = false;
+  // of two pairs; NaN where either is
+  static __device__ __forceinline__ uint32_t least(uint32_t x, uint32_t y) {
+    const half2 h = __hmin2_nan(*reinterpret_cast<const half2*>(&x), *reinterpret_cast<const half2*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t most(uint32_t x, uint32_t y) {
+    const half2 h = __hmax2_nan(*reinterpret_cast<const half2*>(&x), *reinterpret_cast<const half2*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
   static __device__ __forceinline__ float2 up(uint32_t x) {
     return __half22float2(*reinterpret_cast<const half2*>(&x));
   }
@@ -76,6 +109,16 @@ struct Half {
 
 struct Bf16 {
   static constexpr bool kBf16 = true;
+  static __device__ __forceinline__ uint32_t least(uint32_t x, uint32_t y) {
+    const __nv_bfloat162 h =
+        __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t most(uint32_t x, uint32_t y) {
+    const __nv_bfloat162 h =
+        __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
   static __device__ __forceinline__ float2 up(uint32_t x) {
     return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
   }

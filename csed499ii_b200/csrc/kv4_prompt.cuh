@@ -255,24 +255,6 @@ __device__ __forceinline__ void tmem_store_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// Two floats in one register pair, for the two-wide instructions.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pack2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(F2 x) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // Eight codes (nibbles 0..7 of `w`) less 8 as 16-bit numbers, in the order
 // 0, 4, 1, 5, 2, 6, 3, 7.
 template <bool BF16>
@@ -318,12 +300,6 @@ __device__ __forceinline__ bool named_bar_any(int id, int threads, bool x) {
       : "r"(static_cast<int>(x)), "r"(id), "r"(threads)
       : "memory");
   return r != 0;
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 __device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {

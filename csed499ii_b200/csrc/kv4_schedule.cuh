@@ -42,20 +42,37 @@ struct ScheduleParams {
 
 enum : int { kFateOk = 0, kFateNoPages = 1, kFateTable = 2, kFateRows = 3 };
 
-// Inclusive prefix sums of `x` over the block, in thread order.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* warp_sums) {
+// Inclusive prefix sums of `x` over the block, in thread order, and its sums.
+// `warp_sums` is another buffer than the last call's.
+template <int N>
+__device__ __forceinline__ void block_scan(int64_t (&x)[N], int64_t (&total)[N],
+                                           int64_t (*warp_sums)[kScheduleThreads / 32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int s = 1; s < 32; s <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, s);
-    if (lane >= s) x += y;
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x[n], s);
+      if (lane >= s) x[n] += y;
+    }
+    if (lane == 31) warp_sums[n][warp] = x[n];
   }
-  if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  int64_t before = 0;
-  for (int w = 0; w < warp; ++w) before += warp_sums[w];
-  __syncthreads();
-  return x + before;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    total[n] = 0;
+#pragma unroll
+    for (int w = 0; w < kScheduleThreads / 32; ++w) {
+      if (w == warp) x[n] += total[n];
+      total[n] += warp_sums[n][w];
+    }
+  }
+}
+
+// Pages of `tokens` tokens.
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t page) {
+  const uint32_t n = tokens / page;
+  return n + (n * page != tokens);
 }
 
 // First index whose (ascending) entry is above `x`; n if there is none.
@@ -80,7 +97,8 @@ __device__ __forceinline__ int clamp_int(int64_t x) {
 __global__ void __launch_bounds__(kScheduleThreads)
     kv4_schedule_kernel(const __grid_constant__ ScheduleParams p) {
   extern __shared__ int schedule_smem[];
-  __shared__ int64_t warp_sums[kScheduleThreads / 32];
+  __shared__ int64_t warp_sums[2][2][kScheduleThreads / 32];
+  __shared__ int granted;
   int* ends = schedule_smem;       // new tokens up to and with the request
   int* backs = ends + p.batch;     // pages given back up to and with it
   int* needs = backs + p.batch;    // pages needed by the requests before it
@@ -89,56 +107,59 @@ __global__ void __launch_bounds__(kScheduleThreads)
   grid_dependency_launch();
   grid_dependency_wait();
   const int count = min(max(*p.free_count, 0), p.capacity);
-  const int64_t page = p.page_size;
+  const uint32_t page = p.page_size;
+  if (threadIdx.x == 0) granted = 0;
 
   int64_t end0 = 0, back0 = 0;
+  int turn = 0;
   for (int b0 = 0; b0 < p.batch; b0 += kScheduleThreads) {
     const int b = b0 + threadIdx.x;
-    int64_t fresh = 0, back = 0;
+    int64_t x[2] = {0, 0}, all[2];
     if (b < p.batch) {
       const int asked = p.new_lens[b];
       const int len = lens[b] = max(p.lens[b], 0);
-      fresh = max(asked, 0);
-      if (asked < 0) back = min((len + page - 1) / page, static_cast<int64_t>(p.width));
+      x[0] = max(asked, 0);
+      if (asked < 0) x[1] = min(pages_of(len, page), static_cast<uint32_t>(p.width));
+      grants[b] = asked;
     }
-    const int64_t end = end0 + block_scan(fresh, warp_sums);
-    const int64_t given = back0 + block_scan(back, warp_sums);
+    block_scan(x, all, warp_sums[turn ^= 1]);
     if (b < p.batch) {
-      ends[b] = clamp_int(end);
-      backs[b] = clamp_int(given);
+      ends[b] = clamp_int(end0 + x[0]);
+      backs[b] = clamp_int(back0 + x[1]);
       if (blockIdx.x == 0) p.starts[b + 1] = ends[b];
     }
-    __shared__ int64_t carry[2];
-    if (threadIdx.x == kScheduleThreads - 1) carry[0] = end, carry[1] = given;
-    __syncthreads();
-    end0 = carry[0];
-    back0 = carry[1];
-    __syncthreads();
+    end0 += all[0];
+    back0 += all[1];
   }
   const int64_t full = count + back0;  // free pages once the ended requests' are back
 
-  int64_t need0 = 0, granted = 0;
+  // A request that comes too late for its pages leaves those after it none: the
+  // sum of all needs before it only grows, and what is granted is the largest
+  // that the pages reach.
+  int64_t need0 = 0;
   for (int b0 = 0; b0 < p.batch; b0 += kScheduleThreads) {
     const int b = b0 + threadIdx.x;
     int64_t need = 0;
     int fate = kFateOk, asked = 0, len = 0;
     if (b < p.batch) {
-      asked = p.new_lens[b];
+      asked = grants[b];
       len = lens[b];
       if (asked > 0) {
-        const int64_t wanted = (static_cast<int64_t>(len) + asked + page - 1) / page;
+        const uint32_t wanted = pages_of(static_cast<uint32_t>(len) + asked, page);
         if (ends[b] > p.rows) {
           fate = kFateRows;
-        } else if (wanted > p.width) {
+        } else if (wanted > static_cast<uint32_t>(p.width)) {
           fate = kFateTable;
         } else {
-          need = wanted - (len + page - 1) / page;
+          need = wanted - pages_of(len, page);
         }
       }
     }
-    const int64_t upto = need0 + block_scan(need, warp_sums);
+    int64_t x[1] = {need}, all[1];
+    block_scan(x, all, warp_sums[turn ^= 1]);
+    const int64_t upto = need0 + x[0];
+    need0 += all[0];
     if (need > 0 && upto > full) fate = kFateNoPages;
-    const int64_t mine = fate == kFateOk ? need : 0;
     if (b < p.batch) {
       needs[b] = clamp_int(upto - need);
       grants[b] = fate == kFateOk ? static_cast<int>(need) : -1 - fate;
@@ -147,14 +168,10 @@ __global__ void __launch_bounds__(kScheduleThreads)
         p.lens_out[b] = asked < 0 ? 0 : fate == kFateOk ? clamp_int(static_cast<int64_t>(len) + asked) : len;
       }
     }
-    const int64_t got = block_scan(mine, warp_sums);
-    __shared__ int64_t carry[2];
-    if (threadIdx.x == kScheduleThreads - 1) carry[0] = upto, carry[1] = granted + got;
-    __syncthreads();
-    need0 = carry[0];
-    granted = carry[1];
-    __syncthreads();
+    const int most = __reduce_max_sync(0xffffffffu, upto <= full ? clamp_int(upto) : 0);
+    if (blockIdx.x == 0 && (threadIdx.x & 31) == 0) atomicMax(&granted, most);
   }
+  __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     p.starts[0] = 0;
     *p.free_count_out = clamp_int(full - granted);
@@ -173,16 +190,15 @@ __global__ void __launch_bounds__(kScheduleThreads)
   for (int r = thread; r < p.rows; r += threads) {
     const int b = upper_bound(ends, p.batch, r);
     int slot = -1;
-    int64_t position = 0;
+    uint32_t position = 0;
     if (b < p.batch) {
       const int len = lens[b];
-      position = static_cast<int64_t>(len) + r - (b ? ends[b - 1] : 0);
+      position = static_cast<uint32_t>(len) + (r - (b ? ends[b - 1] : 0));
       if (grants[b] >= 0) {
-        const int entry = static_cast<int>(position / page);
-        const int used = static_cast<int>((len + page - 1) / page);
+        const int entry = position / page, used = pages_of(len, page);
         const int id = entry < used ? p.tables[p.table_stride * b + entry]
                                     : stack(full - 1 - needs[b] - (entry - used));
-        slot = static_cast<int>(id * page + position - entry * page);
+        slot = id * page + position - entry * page;
       }
     }
     p.slots[r] = slot;
@@ -196,7 +212,7 @@ __global__ void __launch_bounds__(kScheduleThreads)
       if (at < p.capacity) p.free_pages[at] = p.tables[p.table_stride * b + i];
     }
     if (grants[b] <= 0) continue;
-    const int used = static_cast<int>((lens[b] + page - 1) / page);
+    const int used = pages_of(lens[b], page);
     for (int i = lane; i < grants[b]; i += 32)
       p.tables[p.table_stride * b + used + i] = stack(full - 1 - needs[b] - i);
   }
