@@ -54,6 +54,14 @@ struct Cache {
   }
 };
 
+// Entries from `from` on of a tensor in one dimension, as a tensor of these sizes.
+at::Tensor part_of(const at::Tensor& t, int64_t from, at::IntArrayRef sizes) {
+  at::Tensor x = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+  x.unsafeGetTensorImpl()->set_storage_offset(from);
+  x.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return x;
+}
+
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 
 PyObject* none() { Py_RETURN_NONE; }
@@ -79,8 +87,8 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 2 || !c.from(args[0])) return none();
   const at::Tensor* slots = tensor_of(args[1]);
   if (!ints_on(slots, c.dev) || slots->numel() > INT_MAX) return none();
-  const at::Tensor k = at::empty({slots->numel(), c.heads, c.dim}, c.t->options());
-  const at::Tensor v = at::empty({slots->numel(), c.heads, c.dim}, c.t->options());
+  const int64_t sizes[] = {slots->numel(), c.heads, c.dim}, of_k = sizes[0] * sizes[1] * sizes[2];
+  const at::Tensor both = at::empty({2 * of_k}, c.t->options()), k = part_of(both, 0, sizes), v = part_of(both, of_k, sizes);
   const int rc = sm100_marlin_kv4_read(c.t->const_data_ptr(), c.pages, c.heads, c.page_size, c.dim, c.dtype,
                                        static_cast<const int*>(slots->const_data_ptr()),
                                        static_cast<int>(slots->numel()), k.mutable_data_ptr(),
@@ -151,13 +159,18 @@ PyObject* schedule(PyObject*, PyObject* const* args, Py_ssize_t n) {
       (args[7] != Py_None && (!ints_on(lens_out, dev) || lens_out->numel() != batch)) ||
       (args[8] != Py_None && (!ints_on(count_out, dev) || count_out->numel() != 1)))
     return none();
+  // What only this step needs shares one allocation; lengths and count, which
+  // stay, have their own.
   const auto options = t[0]->options();
+  const int64_t at_slots = (batch + 64) / 64 * 64, at_positions = at_slots + (rows + 63) / 64 * 64,
+                at_fate = at_positions + (rows + 63) / 64 * 64;
+  const at::Tensor step = at::empty({at_fate + batch}, options);
   const at::Tensor out[6] = {lens_out ? *lens_out : at::empty({batch}, options),
                              count_out ? *count_out : at::empty({1}, options),
-                             at::empty({batch + 1}, options),
-                             at::empty({rows}, options),
-                             at::empty({rows}, options),
-                             at::empty({batch}, options)};
+                             part_of(step, 0, {batch + 1}),
+                             part_of(step, at_slots, {rows}),
+                             part_of(step, at_positions, {rows}),
+                             part_of(step, at_fate, {batch})};
   int* to[6];
   for (int i = 0; i < 6; ++i) to[i] = static_cast<int*>(out[i].mutable_data_ptr());
   const int rc = sm100_marlin_kv4_schedule(
