@@ -87,6 +87,7 @@ struct DecodeCfg {
   static constexpr int kSmem = kOffMisc + 1280;
   // a warp's last part takes the place of its ring
   static_assert(kPart * 4 <= kDepth * kSlot, "part does not fit the ring");
+  static_assert((kWarps + kRows) * (2 * D + 8) * 4 <= kRing, "sheets do not fit the rings");
 };
 
 // What a launch knows about one request.
@@ -828,22 +829,25 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
   __syncthreads();
   if (!last_flag[0] && !last_flag[1]) return;
   __threadfence();
-  int rows_of[2];
+  // A warp a row, or several, each over some of the CTAs.  How many is the item's
+  // alone: the order of the sums must not depend on which CTA is last for what.
+  int rows_of[2], split_of[2];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     rows_of[side] = 0;
+    split_of[side] = 1;
     if (last_flag[side]) {
       const Segment& seg = segments[side ? open1 : open0];
       rows_of[side] = min(kRows, span_of<kRows>(p, seg.b).n * p.group - seg.chunk * kRows);
+      split_of[side] = max(kWarps / rows_of[side], 1);
     }
   }
-  // a warp a row of either item, or several, each over some of the CTAs
-  const int units = rows_of[0] + rows_of[1];
-  const int split = units <= kWarps / 2 ? kWarps / units : 1;
-  float* sheets = reinterpret_cast<float*>(smem);  // [warps][D + 4]: the rings are done with
+  const int units0 = rows_of[0] * split_of[0], units = units0 + rows_of[1] * split_of[1];
+  float* sheets = reinterpret_cast<float*>(smem);  // [units][D + 4]: the rings are done with
 #pragma unroll 1
-  for (int unit = warp / split; unit < units; unit += kWarps / split) {
-    const int side = unit >= rows_of[0], r = side ? unit - rows_of[0] : unit, sub = warp % split;
+  for (int unit = warp; unit < units; unit += kWarps) {
+    const int side = unit >= units0, split = split_of[side], at = side ? unit - units0 : unit;
+    const int r = at / split, sub = at - r * split;
     const Segment seg = segments[side ? open1 : open0];
     const int c0 = first_cta(seg.begin), parts = last_cta(seg.begin, seg.end) - c0 + 1;
     auto from = [&](int c) -> const float* {
@@ -876,23 +880,25 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
 #pragma unroll
     for (int y = 0; y < D / 32; ++y) x.x[y] *= over;
     if (split > 1) {
-      x.put(sheets + warp * (D + 4), lane);
-      if (lane == 0) sheets[warp * (D + 4) + D] = top_all, sheets[warp * (D + 4) + D + 1] = sum;
+      x.put(sheets + unit * (D + 4), lane);
+      if (lane == 0) sheets[unit * (D + 4) + D] = top_all, sheets[unit * (D + 4) + D + 1] = sum;
     } else {
       store(seg, span_of<kRows>(p, seg.b), r, x);
     }
   }
-  if (split == 1) return;
+  if (split_of[0] == 1 && split_of[1] == 1) return;
   __syncthreads();
-  if (warp < units) {
-    const int side = warp >= rows_of[0], r = side ? warp - rows_of[0] : warp;
+#pragma unroll 1
+  for (int row = warp; row < rows_of[0] + rows_of[1]; row += kWarps) {
+    const int side = row >= rows_of[0], split = split_of[side], r = side ? row - rows_of[0] : row;
+    if (split == 1) continue;
+    const float* sheet = sheets + ((side ? units0 : 0) + r * split) * (D + 4);
     float top_all = kLowest, sum = 0.f;
     Row x = {};
 #pragma unroll 1
-    for (int y = 0; y < split; ++y) top_all = fmaxf(top_all, sheets[(warp * split + y) * (D + 4) + D]);
+    for (int y = 0; y < split; ++y) top_all = fmaxf(top_all, sheet[y * (D + 4) + D]);
 #pragma unroll 1
-    for (int y = 0; y < split; ++y) {
-      const float* sheet = sheets + (warp * split + y) * (D + 4);
+    for (int y = 0; y < split; ++y, sheet += D + 4) {
       const float f = exp2_approx(sheet[D] - top_all);
       sum = fmaf(sheet[D + 1], f, sum);
       x.add_shared(f, sheet, lane);

@@ -456,6 +456,23 @@ def test_results_do_not_change_from_call_to_call(m):
         assert torch.equal(first, m.kv4_attention(*args, starts=ints(p.starts), max_new=260))
 
 
+@pytest.mark.parametrize("lens,heads,group", [([9000, 40], 2, 8), ([9000, 8000, 7000], 3, 3), ([30000] * 5, 1, 1)])
+def test_results_do_not_depend_on_timing(m, lens, heads, group):
+    """Joins over CTAs while calls on other streams come between."""
+    p = Problem(m, lens, [1] * len(lens), heads, group, 128, 64, torch.half, seed=20)
+    args = (p.q, p.cache, p.tables, ints(lens))
+    want = m.kv4_attention(*args)
+    p.check(want)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        outs = []
+        for s in [torch.cuda.Stream(DEV) for _ in range(3)]:
+            with torch.cuda.stream(s):
+                outs += [m.kv4_attention(*args) for _ in range(10)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
 def test_streams_and_workspaces(m):
     p = Problem(m, [9000, 40], [1, 1], 2, 8, 128, 64, torch.half, seed=19)
     lens = ints(p.lens)
