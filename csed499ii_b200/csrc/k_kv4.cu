@@ -42,8 +42,10 @@ int launched(cudaError_t e) {
   return e == cudaSuccess ? SM100_MARLIN_OK : cuda_fail(e);
 }
 
-// A launch that may begin while the kernel before it on the stream ends: every
-// kernel here waits for that one before it touches global memory.
+// A launch that may begin while the kernel before it on the stream ends.  Every
+// kernel here waits for that one before it touches global memory, and only then
+// lets the next one begin: a GEMM fetches its weights before it waits, and a
+// kernel before this one may be writing them.
 template <class Params>
 cudaError_t launch(void (*kernel)(Params), dim3 grid, int threads, int smem, cudaStream_t stream, const Params& p) {
   cudaLaunchAttribute attr;

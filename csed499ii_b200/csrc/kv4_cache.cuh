@@ -142,7 +142,6 @@ struct Place {
 template <class T, int D>
 __global__ void __launch_bounds__(kCacheThreads) kv4_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int N = D / 64;
-  grid_dependency_launch();
   const int sub = threadIdx.x % kRowLanes;
   const uint32_t rows = static_cast<uint32_t>(p.tokens) * p.cache.heads;
   const uint32_t row = blockIdx.x * (kCacheThreads / kRowLanes) + threadIdx.x / kRowLanes;
@@ -152,6 +151,7 @@ __global__ void __launch_bounds__(kCacheThreads) kv4_append_kernel(const __grid_
   const uint8_t* k_from = p.k + 2 * (p.k_row * token + p.k_head * head) + 16 * sub;
   const uint8_t* v_from = p.v + 2 * (p.v_row * token + p.v_head * head) + 16 * sub;
   grid_dependency_wait();
+  grid_dependency_launch();
   uint4 k[N], v[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) k[n] = load_8(k_from + 128 * n, p.aligned), v[n] = load_8(v_from + 128 * n, p.aligned);
@@ -182,12 +182,12 @@ __device__ __forceinline__ uint4 values_of(uint32_t codes, uint32_t pair) {
 template <class T, int D>
 __global__ void __launch_bounds__(kCacheThreads) kv4_read_kernel(const __grid_constant__ ReadParams p) {
   constexpr int N = D / 64;
-  grid_dependency_launch();
   const int sub = threadIdx.x % kRowLanes;
   const uint32_t rows = static_cast<uint32_t>(p.tokens) * p.cache.heads;
   const uint32_t row = blockIdx.x * (kCacheThreads / kRowLanes) + threadIdx.x / kRowLanes;
   const int token = row / p.cache.heads, head = row - token * p.cache.heads;
   grid_dependency_wait();
+  grid_dependency_launch();
   if (row >= rows) return;
   const int slot = p.slots[token];
   uint4 k[N], v[N];

@@ -469,8 +469,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.y;
 
-  grid_dependency_launch();
   grid_dependency_wait();
+  grid_dependency_launch();
 
   // --- which rows -------------------------------------------------------------
   int* pre = reinterpret_cast<int*>(smem);  // where the tiles will be
@@ -1115,8 +1115,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 template <class T, int D>
 __global__ void __launch_bounds__(2 * D) kv4_prompt_join_kernel(const __grid_constant__ PromptParams p) {
   __shared__ int pre[kSplitBatch], sums[2 * D / 32];
-  grid_dependency_launch();
   grid_dependency_wait();
+  grid_dependency_launch();
   const int total = prompt_prefix<2 * D>(p, pre, sums);
   const int item = total - 1 - static_cast<int>(blockIdx.x / 8);
   if (item < 0) return;

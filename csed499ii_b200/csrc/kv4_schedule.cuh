@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(kScheduleThreads)
   int* needs = backs + p.batch;    // pages needed by the requests before it
   int* grants = needs + p.batch;   // pages it gets, or -1 - fate where it is refused
   int* lens = grants + p.batch;    // tokens in the cache (lens_out may be the same array as lens)
-  grid_dependency_launch();
   grid_dependency_wait();
+  grid_dependency_launch();
   const int count = min(max(*p.free_count, 0), p.capacity);
   const uint32_t page = p.page_size;
   if (threadIdx.x == 0) granted = 0;

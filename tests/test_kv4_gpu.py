@@ -529,6 +529,39 @@ def test_a_step_in_a_graph(m):
     assert lens.tolist() == [50] * batch and count.item() == 40 - batch * 4
 
 
+def test_a_layer_that_serves(m):
+    """The demo's layer: prompts, single tokens, a request that ends and one that takes its place,
+    against plain attention over what its cache holds."""
+    from csed499ii_b200.kv4_demo import CachedAttention
+
+    heads, kv, dim, hidden = 8, 2, 64, 512
+    layer = CachedAttention(hidden, heads, kv, dim, batch=3, pages=12, page_size=32, most=160, seed=5)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    held = [[], [], []]  # (k, v) of each token, as the projection gives them
+    for new in ([70, 0, 33], [1, 5, 1], [1, 1, -1], [1, 1, 40], [1, 1, 1]):
+        rows = sum(max(n, 0) for n in new)
+        x = torch.randn(rows, hidden, generator=g, device=DEV).half()
+        y, step = layer.step(x, ints(new), max(new))
+        assert step.fate.tolist() == [0, 0, 0]
+        q, k, v = layer.qkv(x).view(rows, -1, dim).split([heads, kv, kv], 1)
+        out = torch.zeros(rows, heads, dim, dtype=torch.double, device=DEV)
+        slack, at = torch.zeros_like(out), 0
+        for b, n in enumerate(new):
+            if n < 0:
+                held[b] = []
+                continue
+            held[b] += [(k[i], v[i]) for i in range(at, at + n)]
+            if n:
+                ks, vs = (torch.stack([t[j] for t in held[b]]) for j in (0, 1))
+                out[at:at + n], slack[at:at + n] = R.attention(q[at:at + n], ks, vs, n)
+            at += n
+        assert step.lens.tolist() == [len(h) for h in held]
+        got = m.kv4_attention(q, layer.cache, layer.tables, step.lens, starts=step.starts, max_new=max(new))
+        assert ((got.double() - out).abs() <= slack + 2.0**-24).all()
+        assert torch.equal(y, layer.proj(got.flatten(1)))
+    assert layer.count.item() == 12 - sum(-(-len(h) // 32) for h in held)
+
+
 def test_offsets_past_32_bits(m):
     """A cache of more than 4 GB, its pages used at both ends."""
     heads, dim, page = 8, 128, 64
@@ -602,3 +635,36 @@ def test_refusals(m):
         with pytest.raises(ValueError):
             call()
     torch.cuda.synchronize()
+
+
+def test_weights_written_before_a_cache_call(m):
+    """A GEMM prefetches its weights while the call before it ends: not while the copy before that runs."""
+    k, n = 4096, 22016
+    g = torch.Generator(device=DEV).manual_seed(21)
+    layer = m.Layer_2_4(k, n, groupsize=128).to(DEV)
+    sets = []
+    for _ in range(2):
+        w = torch.randn(k, n, generator=g, device=DEV).half() * 0.02
+        layer.pack(type("W", (), {"weight": w, "bias": None})(), (w.view(k // 128, 128, n).abs().amax(1) / 7).half())
+        sets.append([t.clone() for t in (layer.B, layer.meta, layer.s)])
+    x = torch.randn(16, k, generator=g, device=DEV).half()
+    want = []
+    for s in sets:
+        for t, u in zip((layer.B, layer.meta, layer.s), s):
+            t.copy_(u)
+        torch.cuda.synchronize()
+        want.append(layer(x))
+    cache = m.kv4_cache(4, 2, 64, 16, torch.half, DEV)
+    rows = torch.randn(3, 2, 64, generator=g, device=DEV).half()
+    q, tables, lens = rows.repeat(1, 2, 1), ints([[0], [1], [2]]), ints([3, 2, 1])
+    calls = [lambda: m.kv4_append(rows, rows, cache, ints_of_three),
+             lambda: m.kv4_read(cache, ints_of_three),
+             lambda: m.kv4_attention(q, cache, tables, lens),
+             lambda: m.kv4_schedule(lens, lens, tables, lens, ints_of_three[:1], 6, 16)]
+    ints_of_three = ints([0, 1, 2])
+    for i in range(40):
+        torch.cuda.synchronize()
+        for t, u in zip((layer.s, layer.meta, layer.B), reversed(sets[i % 2])):
+            t.copy_(u)
+        calls[i // 2 % 4]()
+        assert torch.equal(layer(x), want[i % 2]), i
