@@ -8,6 +8,11 @@
 // handed from CTA to CTA and one launch does it all.  Pages that are given
 // back and handed out in the same step are looked up where they lie (in the
 // ended request's table row): no CTA reads what another writes.
+//
+// Latency bounds it: loads, two scans of the block, a search for a row's request
+// and a page's entry one after another.  A step of 8 requests takes 3.8 us on the
+// GPU (a launch alone about 2.2), 500 requests with 9000 rows 6.3 us: 14 us with a
+// CTA for 2048 rows, 64-bit divisions and twelve barriers instead of three.
 #pragma once
 
 #include <stdint.h>

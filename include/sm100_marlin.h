@@ -351,6 +351,9 @@ int sm100_marlin_set_trace_buffer(void* buf);
  *   slots, positions   [rows]; past the last request's rows -1 and 0
  *   fate           [batch], SM100_MARLIN_KV4_*
  * batch is at most 8192.
+ * Like all kv4 calls it is launched so that it may begin while the kernel before
+ * it on the stream ends (sm100_marlin_set_overlap), but touches no memory before
+ * that one is done.
  */
 int sm100_marlin_kv4_schedule(const int* new_lens, const int* lens, int* block_tables,
                               int64_t table_stride, int width, int batch, int* free_pages,
@@ -361,7 +364,7 @@ int sm100_marlin_kv4_schedule(const int* new_lens, const int* lens, int* block_t
 /* Quantises the rows of k and v (element (token, head, c) at token * *_row +
  * head * *_head + c, 16-bit aligned) into the cache at `slots[token]`; rows
  * whose slot is outside the cache are skipped.  Two rows of one call must not
- * have the same slot. */
+ * have the same slot.  tokens * kv_heads is below 2^31. */
 int sm100_marlin_kv4_append(const void* k, int64_t k_row, int64_t k_head, const void* v,
                             int64_t v_row, int64_t v_head, void* cache, int pages, int kv_heads,
                             int page_size, int head_dim, int dtype, const int* slots, int tokens,
@@ -387,8 +390,10 @@ int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_s
  *   max_new    no request has more rows than this (it picks the kernel: not
  *              more work, and no result, hangs on how close it is)
  *   workspace  sm100_marlin_kv4_workspace_bytes(dev) bytes, 16-byte aligned,
- *              all zero on entry and left so; calls that may overlap need
- *              their own
+ *              the first 4096 zero before the first call (and left so by every
+ *              one); calls that may overlap need their own
+ * SM100_MARLIN_ERR_PROB_SHAPE where one request alone could have 2^30 steps of 32
+ * tokens (table width * page_size * kv_heads * row chunks).
  */
 int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, const void* cache,
                                int pages, int kv_heads, int page_size, int head_dim, int dtype,
