@@ -34,7 +34,7 @@
 //
 // Measured at 8 key/value heads of 128 and 8 query heads each: one request of
 // 131072 tokens (142.8 MB) in 45 us, 64 of up to 8192 (256 MB, bf16) in 80 us, 3.2
-// TB/s of 6.55 measured for a copy.  Instructions bound it: 270 a warp and tile, half
+// TB/s of 6.55 measured for a copy.  Instructions bound it: 290 a warp and tile, half
 // of them on the integer pipe (each takes a scheduler two cycles there) to turn
 // codes into operands, which is 120 cycles a tile and SM at the 52% of issue slots
 // that 16 warps of 128 registers fill.  Launch, first bytes, and joins in the CTA
