@@ -237,16 +237,21 @@ __device__ __forceinline__ uint32_t key_odd(uint32_t w) {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What the weights need to know of a row of values: its scale's logarithm and
-// reciprocal, and its value at code 8 over the scale.  A row without a scale
-// has all codes 0, so any scale tells the same values; a small one rounds its
-// weights where nothing shows.
+// reciprocal, and its value at code 8 over the scale.
+//
+// The sum of the weights is kept as sum(w / s), so 1 / s has to leave room for a
+// long sum in 32 bits: a scale below 2^-90 (bf16 values below 2^-75) counts as
+// 2^-90.  One below 2^-30 of the offset changes no value that 32 bits hold.  A
+// row without a scale has all codes 0, so any scale tells the same values; its
+// weights are to outweigh nobody else's, who would lose theirs in the rounding to
+// half: 2^-10 of the offset is below what its own value adds to the result, and
+// 2^-60 for a row of zeros is in the middle of what scales can be.
 struct ValueRow {
   float log_s, inv_s, at_8;
 };
 __device__ __forceinline__ ValueRow value_row(float2 pair) {
-  const float s = pair.x >= 0x1p-60f  ? pair.x
-                  : pair.x > 0.f      ? 0x1p-60f
-                                      : fmaxf(fabsf(pair.y) * 0x1p-10f, 0x1p-17f);
+  const float s = pair.x > 0.f ? fmaxf(fmaxf(pair.x, fabsf(pair.y) * 0x1p-30f), 0x1p-90f)
+                               : fmaxf(fabsf(pair.y) * 0x1p-10f, 0x1p-60f);
   ValueRow r;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r.log_s) : "f"(s));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inv_s) : "f"(s));
