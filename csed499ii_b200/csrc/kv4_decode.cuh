@@ -13,10 +13,11 @@
 // the weights w = p s (to half, whatever the model's type).  The exponential
 // gives w itself, its argument is the score plus log2 s, and the running
 // maximum is that of these arguments: a half then holds the weights that
-// matter whatever sizes the values have, and p is w / s in 32 bits.  The offset
-// term takes the rounded weights too, so a rounding error meets the value that a
-// code stands for, as it would meet a dequantised value, and only sum(p) takes the
-// weights as they are.
+// matter whatever sizes the values have, and p is w / s in 32 bits.  sum(p) and the
+// offset term take the weights as they are, and the codes act as if centred on 8: a
+// rounding error meets at most 8 steps of its row's scale, never its offset, which
+// can be 2^15 scales (with rounded weights in the offset term one wide row among
+// 20000 narrow ones moved the result by 5 times what its rounding allows).
 //
 // mma.m16n8k16 takes 16 tokens (scores) or 16 channels (result) as its rows
 // and 8 query rows as its columns; the 8 query heads of a group fill it.  Codes
@@ -672,15 +673,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
             for (int c = 0; c < 4; ++c) {
               w[c] = exp2_approx(x[u][nt][c] - top[nt][c & 1]);
               l[nt][c & 1] = fmaf(w[c], c < 2 ? s0.x : s1.x, l[nt][c & 1]);
+              a1[nt][c & 1] = fmaf(w[c], c < 2 ? s0.y : s1.y, a1[nt][c & 1]);
             }
-            const uint32_t w01 = Half::down(w[0], w[1]), w23 = Half::down(w[2], w[3]);
-            const float2 r01 = Half::up(w01), r23 = Half::up(w23);
-            a1[nt][0] = fmaf(r01.x, s0.y, a1[nt][0]);
-            a1[nt][1] = fmaf(r01.y, s0.y, a1[nt][1]);
-            a1[nt][0] = fmaf(r23.x, s1.y, a1[nt][0]);
-            a1[nt][1] = fmaf(r23.y, s1.y, a1[nt][1]);
-            wb[nt][0] = transpose_8x8(w01);
-            wb[nt][1] = transpose_8x8(w23);
+            wb[nt][0] = transpose_8x8(Half::down(w[0], w[1]));
+            wb[nt][1] = transpose_8x8(Half::down(w[2], w[3]));
             if (u == 0) {
               mma_16816_z<false>(ones[nt], kOnes, kOnes, kOnes, kOnes, wb[nt][0], wb[nt][1]);
             } else {

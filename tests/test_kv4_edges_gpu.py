@@ -55,3 +55,29 @@ def test_rows_of_zeros_between_values_of_any_exponent(m, power):  # noqa: F811
     p.v[::3] = 0
     m.kv4_append(p.k, p.v * 2.0**power, p.cache, p.slots)
     p.check((attend(m, p, lens, new).double() * 2.0**-power).to(torch.bfloat16))
+
+
+# ---------------------------------------------------------------------------
+# weights of very different sizes
+# ---------------------------------------------------------------------------
+def attend_many(m, p, n, new, copies):  # noqa: F811
+    """Attention of one request, and of many at once that share its pages: enough
+    of them that a warp or a CTA goes over all keys of a request by itself."""
+    out = attend(m, p, [n], [new])
+    many = m.kv4_attention(p.q.repeat(copies, 1, 1), p.cache, p.tables.repeat(copies, 1), ints([n] * copies),
+                           starts=ints([new * i for i in range(copies + 1)]), max_new=new)
+    return [out, many[:new], many[-new:], many[copies // 2 * new:][:new]]
+
+
+@pytest.mark.parametrize("new,copies", [(1, 2600), (100, 80)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_wide_row_among_narrow_ones(m, dim, new, copies):  # noqa: F811
+    """Values next to 1 whose scales are 2^-14, one row whose scale is 64, equal weights."""
+    n = 20000
+    p = Problem(m, [n], [new], 1, 2, dim, 64, torch.half, seed=36, sharp=0.0)
+    g = torch.Generator(device=DEV).manual_seed(37)
+    p.v = (1 + 2.0**-10 * torch.randint(0, 4, p.v.shape, generator=g, device=DEV)).half()
+    p.v[77] = (960 * torch.rand(p.v[77].shape, generator=g, device=DEV) - 480).half()
+    m.kv4_append(p.k, p.v, p.cache, p.slots)
+    for out in attend_many(m, p, n, new, copies):
+        p.check(out)
