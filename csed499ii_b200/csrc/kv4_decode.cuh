@@ -261,13 +261,22 @@ __device__ __forceinline__ ValueRow value_row(float2 pair) {
 }
 
 // What there is of an item in one place: results (already divided by the sum),
-// the running maximum of the weights' arguments and the sum of the weights.
+// the running maximum of the weights' arguments (less kWeightTop) and the sum of
+// the weights over 2 to it.
 struct Segment {
   int begin, end;        // the item's place in the row of all steps; begin < 0: none
   int b, head, chunk;
 };
 
 constexpr float kLowest = -3.0e38f;
+
+// A weight in half is 2^kWeightTop where its argument is the maximum, which moves
+// once an argument passes it by kLag: weights reach 2^kMoveAt, and what lies 2^-31
+// below the largest is still held.  With 1 for the largest a half rounds below
+// 2^-14 and ends at 2^-24: 32767 keys that weigh 2^-20 of a first one, 2^-5
+// together, had errors of 1.4 times what the rounding of weights allows, and keys
+// that weigh 2^-26 were lost.
+constexpr float kWeightTop = 7.f, kLag = 8.f, kMoveAt = kWeightTop + kLag;
 
 __device__ __forceinline__ float warp_max(float x) {
 #pragma unroll
@@ -626,14 +635,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
                   x[u][nt][c] = -CUDART_INF_F;
               }
         }
-        // The maximum moves only where an argument passes it by more than 8 (a
-        // factor of 256, harmless in the sums), so most steps need no exchange.
+        // The maximum moves only where an argument passes it by more than kLag, so
+        // most steps need no exchange.
         bool moves = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c)
-            moves |= fmaxf(fmaxf(x[0][nt][c], x[0][nt][c + 2]), fmaxf(x[1][nt][c], x[1][nt][c + 2])) > top[nt][c] + 8.f;
+            moves |= fmaxf(fmaxf(x[0][nt][c], x[0][nt][c + 2]), fmaxf(x[1][nt][c], x[1][nt][c + 2])) >
+                     top[nt][c] + kMoveAt;
         if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -641,7 +651,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               float m = fmaxf(fmaxf(x[0][nt][c], x[0][nt][c + 2]), fmaxf(x[1][nt][c], x[1][nt][c + 2]));
-              m = fmaxf(top[nt][c], m);
+              m = fmaxf(top[nt][c], m - kWeightTop);
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));

@@ -35,11 +35,11 @@
 // Numbers that the terms cannot hold (a key's or value's scale out of the usual
 // range, a row of NaN) are added in 32 bits by a careful form of the step.  So
 // is what the weights lose in rounding to half where the values' scales differ
-// by more than a factor of 64: a weight p s_v below 2^-14 is rounded more
-// coarsely, which is nothing to the result but could be to sum(p).  A third form
+// by more than a factor of 64: a weight p s_v below 2^-21 of the largest is rounded
+// more coarsely, which is nothing to the result but could be to sum(p).  A third form
 // serves steps that some row does not see whole and steps that move the running
-// maximum: the maximum is only moved when an argument passes it by more than 8
-// (a factor of 256), which is rare after the first steps.
+// maximum: the maximum is only moved when an argument passes it by more than kLag,
+// which is rare after the first steps.
 //
 // Four warps each turn key and value codes into operand tiles (two stages of
 // each), eight warps per query tile do the softmax (two for 32 rows: one has
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               }
             }
           }
-          done = !named_bar_any(meet, 64, fmaxf(mx[0], mx[1]) > 8.f);
+          done = !named_bar_any(meet, 64, fmaxf(mx[0], mx[1]) > kMoveAt);
           if (done) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -734,14 +734,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             mx[i] = fmaxf(mx[i], other[row0 + 8 * i].y);
-            moves |= mx[i] > top[i] + 8.f;
+            moves |= mx[i] > top[i] + kMoveAt;
           }
           if (__any_sync(0xffffffffu, moves)) {
             float f[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              f[i] = exp2_approx(top[i] - fmaxf(top[i], mx[i]));
-              top[i] = fmaxf(top[i], mx[i]);
+              const float next = fmaxf(top[i], mx[i] - kWeightTop);
+              f[i] = exp2_approx(top[i] - next);
+              top[i] = next;
               l[i] *= f[i];
               off[i] *= f[i];
             }

@@ -81,3 +81,31 @@ def test_one_wide_row_among_narrow_ones(m, dim, new, copies):  # noqa: F811
     m.kv4_append(p.k, p.v, p.cache, p.slots)
     for out in attend_many(m, p, n, new, copies):
         p.check(out)
+
+
+@pytest.mark.parametrize("new,copies", [(1, 2600), (100, 80)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,power", [(32768, 18), (32768, 19), (32768, 20), (32768, 21), (32768, 22), (32768, 24)])
+def test_one_strong_key_before_many_weak_ones(m, dtype, n, power, new, copies):  # noqa: F811
+    """Keys that weigh 2^-power of the first each have their part in the result too."""
+    p = Problem(m, [n], [new], 1, 2, 128, 64, dtype, seed=34)
+    g = torch.Generator(device=DEV).manual_seed(35)
+    signs = torch.where(torch.rand(128, generator=g, device=DEV) < 0.5, -1.0, 1.0)
+    p.q = signs.expand(p.q.shape).contiguous().to(dtype)
+    p.k = torch.zeros_like(p.k)
+    p.k[0, 0] = (signs * (power * 0.6931 / 128**0.5)).to(dtype)
+    p.v[1:] = p.v[1]
+    m.kv4_append(p.k, p.v, p.cache, p.slots)
+    for out in attend_many(m, p, n, new, copies):
+        p.check(out)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_next_to_zero(m, dim):  # noqa: F811
+    """Keys whose scale is a subnormal of the type, or of 32 bits: they weigh as zeros do."""
+    lens, new = [200, 150], [1, 150]
+    p = Problem(m, lens, new, 2, 2, dim, 64, torch.bfloat16, seed=38)
+    tiny = torch.tensor([0.0, 2.0**-133, 2.0**-129, 2.0**-126, 2.0**-120, 2.0**-60], device=DEV)
+    p.k[::4] = (torch.rand(p.k[::4].shape, device=DEV) * tiny[torch.arange(88, device=DEV) % 6, None, None]).bfloat16()
+    m.kv4_append(p.k, p.v, p.cache, p.slots)
+    p.check(attend(m, p, lens, new))
