@@ -200,6 +200,15 @@ __device__ __forceinline__ void mma_16816_z(float (&c)[4], uint32_t a0, uint32_t
   }
 }
 
+// The same for halves, begun with (c0, c1, c2, c3).
+__device__ __forceinline__ void mma_16816_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
 // The 8x8 matrix of 16-bit values spread over the warp, transposed.
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
@@ -669,13 +678,13 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
             }
           }
         }
+        // Weights, and their sums.
         constexpr uint32_t kOnes = 0x3c003c00u;  // 1.0 twice
+        uint32_t wb[2][NT][2];
         float ones[NT][4];  // the step's sum of the rounded weights
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          // weights, and their sums
           const float2 s0 = token_sums[16 * u + g], s1 = token_sums[16 * u + g + 8];
-          uint32_t wb[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float w[4];
@@ -685,55 +694,68 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
               l[nt][c & 1] = fmaf(w[c], c < 2 ? s0.x : s1.x, l[nt][c & 1]);
               a1[nt][c & 1] = fmaf(w[c], c < 2 ? s0.y : s1.y, a1[nt][c & 1]);
             }
-            wb[nt][0] = transpose_8x8(Half::down(w[0], w[1]));
-            wb[nt][1] = transpose_8x8(Half::down(w[2], w[3]));
+            wb[u][nt][0] = transpose_8x8(Half::down(w[0], w[1]));
+            wb[u][nt][1] = transpose_8x8(Half::down(w[2], w[3]));
             if (u == 0) {
-              mma_16816_z<false>(ones[nt], kOnes, kOnes, kOnes, kOnes, wb[nt][0], wb[nt][1]);
+              mma_16816_z<false>(ones[nt], kOnes, kOnes, kOnes, kOnes, wb[u][nt][0], wb[u][nt][1]);
             } else {
-              mma_16816<false>(ones[nt], kOnes, kOnes, kOnes, kOnes, wb[nt][0], wb[nt][1]);
+              mma_16816<false>(ones[nt], kOnes, kOnes, kOnes, kOnes, wb[u][nt][0], wb[u][nt][1]);
             }
           }
-          // result
+        }
+        // Result.  A step's products are summed by themselves, begun with 8 times the
+        // rounded weights taken off, and added to the others in binary32: the tensor
+        // cores cut a sum off at 2^-23 of it with every product added, a bias over a
+        // long run of one warp (131071 keys that weigh 2^-26 of a first one had 1.13
+        // times the error that the rounding of weights allows).  It takes 4% of the time.
+        constexpr int kOctets = D / 64;
+        uint32_t va[2][kOctets], vb[2][kOctets], vc[2][kOctets], vd[2][kOctets];  // tokens 2t, 2t+1, 2t+8, 2t+9
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
           const uint32_t tile = data + u * kBytes;
-          constexpr int kOctets = D / 64;
-          uint32_t va[kOctets], vb[kOctets], vc[kOctets], vd[kOctets];  // tokens 2t, 2t+1, 2t+8, 2t+9
           if constexpr (D == 128) {
             const uint4 y = lds128(tile + 8 * D + 16 * lane), z = lds128(tile + 12 * D + 16 * lane);
-            va[0] = y.x, va[1] = y.y, vb[0] = y.z, vb[1] = y.w;
-            vc[0] = z.x, vc[1] = z.y, vd[0] = z.z, vd[1] = z.w;
+            va[u][0] = y.x, va[u][1] = y.y, vb[u][0] = y.z, vb[u][1] = y.w;
+            vc[u][0] = z.x, vc[u][1] = z.y, vd[u][0] = z.z, vd[u][1] = z.w;
           } else {
             const uint2 y = lds64(tile + 8 * D + 8 * lane), z = lds64(tile + 12 * D + 8 * lane);
-            va[0] = y.x, vb[0] = y.y;
-            vc[0] = z.x, vd[0] = z.y;
+            va[u][0] = y.x, vb[u][0] = y.y;
+            vc[u][0] = z.x, vd[u][0] = z.y;
           }
+        }
 #pragma unroll
-          for (int o = 0; o < kOctets; ++o)
+        for (int o = 0; o < kOctets; ++o)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < 2; ++half) {
+            float sums[NT][2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
               const uint32_t sel = half ? 0x7632 : 0x5410;
-              const uint32_t y = prmt_b32(va[o], vb[o], sel), z = prmt_b32(vc[o], vd[o], sel);
-              const uint32_t y8 = y >> 8, z8 = z >> 8;
+              const uint32_t y = prmt_b32(va[u][o], vb[u][o], sel), z = prmt_b32(vc[u][o], vd[u][o], sel);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_16816<false>(acc[nt][4 * o + 2 * half], y & 0x000f000fu, y & 0x00f000f0u,
-                                 z & 0x000f000fu, z & 0x00f000f0u, wb[nt][0], wb[nt][1]);
-                mma_16816<false>(acc[nt][4 * o + 2 * half + 1], y8 & 0x000f000fu, y8 & 0x00f000f0u,
-                                 z8 & 0x000f000fu, z8 & 0x00f000f0u, wb[nt][0], wb[nt][1]);
+              for (int odd = 0; odd < 2; ++odd) {
+                const uint32_t yo = odd ? y >> 8 : y, zo = odd ? z >> 8 : z;
+                const uint32_t c0 = yo & 0x000f000fu, c1 = yo & 0x00f000f0u;
+                const uint32_t c2 = zo & 0x000f000fu, c3 = zo & 0x00f000f0u;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  float(&to)[4] = sums[nt][odd];
+                  const uint32_t b0 = wb[u][nt][0], b1 = wb[u][nt][1];
+                  if (u == 0) {
+                    mma_16816_from(to, c0, c1, c2, c3, b0, b1, ones[nt][0] * -0x1p-21f, ones[nt][1] * -0x1p-21f,
+                                   ones[nt][0] * -0x1p-17f, ones[nt][1] * -0x1p-17f);
+                  } else {
+                    mma_16816<false>(to, c0, c1, c2, c3, b0, b1);
+                  }
+                }
               }
             }
-        }
-        // 8 times the weights off the sums, which so stay as small as the centred
-        // codes'.  Products are rounded down to 2^-24 of a sum, and over a long run of
-        // positive codes that adds up: at the end instead of here, 131072 tokens have
-        // 1.8 times the error of a result rounded once (so 1.48 times, most of it from
-        // the weights; it takes 2% of the time).
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float less = ones[nt][c] * -0x1p-21f, less_odd = ones[nt][c] * -0x1p-17f;
+              for (int odd = 0; odd < 2; ++odd)
 #pragma unroll
-            for (int y = 0; y < D / 16; ++y) acc[nt][y][c] += less, acc[nt][y][c + 2] += less_odd;
+                for (int c = 0; c < 4; ++c) acc[nt][4 * o + 2 * half + odd][c] += sums[nt][odd][c];
           }
         __syncwarp();  // the slot and the tokens' numbers are read
         if (issued < count) issue();

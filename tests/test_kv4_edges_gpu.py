@@ -83,9 +83,9 @@ def test_one_wide_row_among_narrow_ones(m, dim, new, copies):  # noqa: F811
         p.check(out)
 
 
-@pytest.mark.parametrize("new,copies", [(1, 2600), (100, 80)])
+@pytest.mark.parametrize("n,new,copies", [(32768, 1, 2600), (32768, 100, 80), (131072, 1, 2600)])
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,power", [(32768, 18), (32768, 19), (32768, 20), (32768, 21), (32768, 22), (32768, 24)])
+@pytest.mark.parametrize("power", [18, 19, 20, 21, 22, 24, 26, 31])
 def test_one_strong_key_before_many_weak_ones(m, dtype, n, power, new, copies):  # noqa: F811
     """Keys that weigh 2^-power of the first each have their part in the result too."""
     p = Problem(m, [n], [new], 1, 2, 128, 64, dtype, seed=34)
