@@ -101,6 +101,18 @@ def test_one_strong_key_before_many_weak_ones(m, dtype, n, power, new, copies): 
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,new", [(1, 1), (8, 1), (8, 3)])
+def test_fp16_results_of_few_rows_are_rounded_once(m, dim, group, new):  # noqa: F811
+    """Many keys of like weights, where each weight's rounding shows.  All but the result
+    is held to 2^-14 of it or better, so the error is next to that of one rounding."""
+    n = 60000
+    p = Problem(m, [n], [new], 2, group, dim, 64, torch.half, seed=39, sharp=0.5)
+    want, _ = R.attention(p.q, p.k, p.v, new)
+    once = (want.half().double() - want).norm()
+    assert (attend(m, p, [n], [new]).double() - want).norm() <= 1.15 * once
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 def test_keys_next_to_zero(m, dim):  # noqa: F811
     """Keys whose scale is a subnormal of the type, or of 32 bits: they weigh as zeros do."""
     lens, new = [200, 150], [1, 150]
