@@ -14,7 +14,11 @@
 //   O += P (C_v - 8)      tcgen05.mma, P from tensor memory
 //
 // As in the decode kernel the operands are codes, exact in 16 bits, so that
-// nothing is rounded but the weights.  What scales and offsets add is put into
+// nothing is rounded but the weights.  Here they are one half for either type: an
+// fp16 result of a prompt has 1.3 times the error of a result rounded once, and a
+// second product for what the rounding leaves, as the decode kernel has, would add
+// half of the step's tensor work and as many stores to tensor memory again.  What
+// scales and offsets add is put into
 // the same products as 16 more channels, in two or three 16-bit terms each
 // (2^-22 of a value): with z = offset / s_k + 8 a key's argument of the
 // exponential is s_k (S + z sum(q) + log2 s_v / s_k), so its column of S needs
@@ -99,6 +103,13 @@ constexpr int kSplitBatch = 1024;  // requests of a launch that shares out keys
 // Steps of a CTA where keys are shared out: an item costs a CTA about as much as
 // four steps before and after its own.
 constexpr int kLeastPromptSteps = 4;
+
+// The tensor cores cut a sum off at 2^-23 of it with every product added, which is
+// a bias over many keys (131071 that weigh 2^-26 of a first one had 3.7 times the
+// error that the rounding of weights allows).  After so many steps (about 900
+// products of a channel) the results so far go to the softmax warps' local memory,
+// are added to in binary32 there, and the products begin anew.
+constexpr int kFreshSteps = 128;
 
 // What the careful form of a step needs to know of its keys (the usual one
 // reads the scales alone).
@@ -612,6 +623,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) top[i] = kLowest, l[i] = off[i] = 0.f;
       int largest = -1000;  // exponent of a value scale up to here
+      // This thread's row of the result up to the last step that was a multiple of
+      // kFreshSteps: every second 16 channels, and the sums' 16 columns.
+      constexpr int kSettled = D / 32 + 1;
+      volatile float settled[16 * kSettled];
       for (int it = 0; it < steps; ++it) {
         const int buf = it & 3;
         wait_warp(c_full + 8 * buf, it >> 2);
@@ -627,7 +642,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         wait_warp(s_full + 8 * qi, it);
         if (gave_up()) break;
         tc_fence_after();
-        if (plain && it > 0 && j0 + kStep <= lo + 1 && (p.window == 0 || hi - j0 < p.window)) {
+        if (plain && it % kFreshSteps != 0 && j0 + kStep <= lo + 1 && (p.window == 0 || hi - j0 < p.window)) {
           // the step with the maximum as it is
           uint32_t weights[2][16];  // of either 16 lanes
           float mx[2] = {kLowest, kLowest};
@@ -736,7 +751,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             mx[i] = fmaxf(mx[i], other[row0 + 8 * i].y);
             moves |= mx[i] > top[i] + kMoveAt;
           }
-          if (__any_sync(0xffffffffu, moves)) {
+          if (__any_sync(0xffffffffu, moves) || it % kFreshSteps == 0) {
             float f[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -751,14 +766,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               wait_warp(spent + 8 * (it & 1), it >> 1);
               if (gave_up()) break;
               tc_fence_after();
+              if (it % kFreshSteps != 0) {
 #pragma unroll 1
-              for (int c = half; c < kN / 16; c += 2) {
-                uint32_t o[16];
-                tmem_load_16(o_at + 16 * c, o);
-                tmem_loaded(o);
+                for (int c = half; c < kN / 16; c += 2) {
+                  uint32_t o[16];
+                  tmem_load_16(o_at + 16 * c, o);
+                  tmem_loaded(o);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fl);
-                tmem_store_16(o_at + 16 * c, o);
+                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fl);
+                  tmem_store_16(o_at + 16 * c, o);
+                }
+              }
+              if (it >= kFreshSteps) {
+#pragma unroll 1
+                for (int c = 0; c < kSettled; ++c) {
+                  uint32_t o[16] = {};
+                  if (it % kFreshSteps == 0) {
+                    tmem_load_16(o_at + (c == D / 32 ? D : 32 * c + 16 * half), o);
+                    tmem_loaded(o);
+                  }
+#pragma unroll
+                  for (int i = 0; i < 16; ++i)
+                    settled[16 * c + i] =
+                        (__uint_as_float(o[i]) + (it > kFreshSteps ? settled[16 * c + i] : 0.f)) * fl;
+                }
               }
             }
           }
@@ -834,6 +865,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         tmem_loaded(o);
         sum += 4.f * (__uint_as_float(o[0]) + __uint_as_float(o[1]));
         rest += __uint_as_float(o[2]) + __uint_as_float(o[3]);
+        if (steps > kFreshSteps) {
+          const volatile float* more = settled + 16 * (D / 32);
+          sum += 4.f * (more[0] + more[1]);
+          rest += more[2] + more[3];
+        }
       }
       const float over = sum == 0.f ? 0.f : 1.f / sum;
       const bool whole = after[0] == 1, there = qi * 128 + row < after[3];
@@ -857,6 +893,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             tmem_loaded(o);
           }
           if (!there) continue;
+          if (steps > kFreshSteps) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + settled[16 * (c >> 1) + i]);
+          }
           if (!whole) {
             float4* to = reinterpret_cast<float4*>(part + c * (256 * 16));
 #pragma unroll
@@ -1104,7 +1144,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           tc_fence_after();
           const uint64_t v_desc = umma_desc_sw128_k(base + Cfg::kOffV + stage * Cfg::kV);
           const uint32_t s_at = t0 + Cfg::kColS + kStep * qi, o_at = t0 + Cfg::kColO + kN * qi;
-          warp_umma_ts<4>(o_at, s_at, v_desc, id_o, it > 0);
+          warp_umma_ts<4>(o_at, s_at, v_desc, id_o, it % kFreshSteps != 0);
           warp_umma_ts<kStep / 16 - 4>(o_at, s_at + 64, v_desc + (kN * 128 >> 4), id_o, 1);
           if (more) scores(qi, next);
         }

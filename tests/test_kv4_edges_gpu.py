@@ -83,7 +83,7 @@ def test_one_wide_row_among_narrow_ones(m, dim, new, copies):  # noqa: F811
         p.check(out)
 
 
-@pytest.mark.parametrize("n,new,copies", [(32768, 1, 2600), (32768, 100, 80), (131072, 1, 2600)])
+@pytest.mark.parametrize("n,new,copies", [(32768, 1, 2600), (131072, 1, 2600), (32768, 100, 80), (131072, 100, 80)])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("power", [18, 19, 20, 21, 22, 24, 26, 31])
 def test_one_strong_key_before_many_weak_ones(m, dtype, n, power, new, copies):  # noqa: F811
