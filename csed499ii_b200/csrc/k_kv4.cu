@@ -99,12 +99,14 @@ size_t workspace_bytes(int sms) {
 }
 
 template <class T, int D, int NT>
-int launch_decode(DecodeParams p, int64_t most, int sms, int dev, cudaStream_t stream) {
+int launch_decode(DecodeParams p, int sms, int dev, cudaStream_t stream) {
   using Cfg = DecodeCfg<D, NT>;
   const int bad = allow_smem<kv4_decode_kernel<T, D, NT>>(dev, Cfg::kSmem);
   if (bad) return bad;
   // The kernel keeps a sum per request in shared memory, and counts steps in 32
-  // bits: larger batches go in slices.
+  // bits: larger batches go in slices.  What it can meet counts here, not what the
+  // caller says of the lengths.
+  const int64_t all = static_cast<int64_t>(p.starts ? p.rows : 1) * p.group, most = all < p.most ? all : p.most;
   const int64_t steps = (static_cast<int64_t>(p.width) * p.cache.page_size / kStepTokens + 1) *
                         p.cache.heads * ((most + Cfg::kRows - 1) / Cfg::kRows);  // of a request, at most
   const int64_t fit = 0x3fffffffll / steps;
@@ -283,10 +285,9 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
   const bool vector = aligned(q, 16) && ((q_row | q_head) & 7) == 0;
   const int few_rows = group > kFewRows ? group : kFewRows;  // a single token is always few
   const int64_t most = static_cast<int64_t>(starts ? max_new : 1) * group;
-  const int64_t few_most = most < few_rows ? most : few_rows;
   const DecodeParams few{c, static_cast<const uint8_t*>(q), q_row, q_head, vector,
                          static_cast<uint8_t*>(out), block_tables, table_stride, width, lens, starts,
-                         0, batch, rows, 1, q_heads, group, window, few_rows, scale,
+                         0, batch, rows, 1, most <= few_rows, q_heads, group, window, few_rows, scale,
                          static_cast<int*>(workspace),
                          reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status};
   const PromptParams many{c, static_cast<const uint8_t*>(q), q_row, q_head, vector, static_cast<uint8_t*>(out),
@@ -296,8 +297,8 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
   return dispatch(dtype, head_dim, [&](auto type, auto dim) {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value;
-    const int bad = most <= 8 ? launch_decode<T, D, 1>(few, few_most, sms, dev, on_stream)
-                              : launch_decode<T, D, 2>(few, few_most, sms, dev, on_stream);
+    const int bad = most <= 8 ? launch_decode<T, D, 1>(few, sms, dev, on_stream)
+                              : launch_decode<T, D, 2>(few, sms, dev, on_stream);
     return bad || most <= few_rows ? bad : launch_prompt<T, D>(many, sms, dev, on_stream);
   });
 }

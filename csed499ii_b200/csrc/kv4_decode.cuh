@@ -71,6 +71,7 @@ struct DecodeParams {
   int batch;
   int rows;              // of q
   int pad;               // 1: rows past the last request are set to zero
+  int alone;             // 1: no other kernel serves the requests that are left alone
   int q_heads;
   int group;             // query heads per key/value head
   int window;            // 0: none
@@ -398,17 +399,18 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
     __syncthreads();
   }
 
-  // --- rows that see nothing ------------------------------------------------
+  // --- rows that see nothing, and rows that nobody serves ---------------------
   {
     const int64_t row_bytes = 2ll * p.q_heads * D;
 #pragma unroll 1
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
       if (pre[b] != (b ? pre[b - 1] : 0)) continue;
       const Span s = span_of<kRows>(p, b);
-      if (s.chunks == 0) continue;
+      if (s.chunks == 0 && (s.n <= 0 || !p.alone)) continue;
+      const uint32_t x = s.chunks == 0 ? 0x7fff7fffu : 0u;  // NaN in either type
 #pragma unroll 1
       for (int64_t i = 16 * threadIdx.x; i < s.n * row_bytes; i += 16 * Cfg::kThreads)
-        *reinterpret_cast<uint4*>(p.out + s.first * row_bytes + i) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(p.out + s.first * row_bytes + i) = make_uint4(x, x, x, x);
     }
     const int end = !p.starts || !p.pad ? p.rows : p.batch ? max(p.starts[p.batch], 0) : 0;
 #pragma unroll 1

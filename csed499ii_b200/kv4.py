@@ -292,7 +292,9 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
         the cache's; rows and heads may have any stride
     @block_tables: ``torch.int`` ``(batch, width)``, @lens: ``torch.int`` ``(batch,)``
     @starts: ``torch.int`` ``(batch + 1,)``; None: one row for each request
-    @max_new: no request has more rows than this (default: all of ``q``'s)
+    @max_new: no request has more rows than this (default: all of ``q``'s); it
+        picks the kernels, so give it for steps of single or few tokens: they are
+        slower without.  Rows of a request that has more can be NaN
     @scale: of the scores, default ``1 / sqrt(head_dim)``
     @out: ``(rows, heads, head_dim)``, contiguous
     @workspace: :func:`kv4_workspace`; None: one that the module keeps for the

@@ -388,8 +388,10 @@ int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_s
  * A value's scale below 2^-90 (bf16 values smaller than 2^-75) counts as 2^-90.
  *   q          element (row, head, c) at row * q_row + head * q_head + c
  *   out        [rows][q_heads][head_dim], 16-byte aligned
- *   max_new    no request has more rows than this (it picks the kernel: not
- *              more work, and no result, hangs on how close it is)
+ *   max_new    no request has more rows than this.  It picks the kernels, so
+ *              the time and a result's last bits can hang on it; the closer the
+ *              faster.  A request that has more is served all the same where the
+ *              kernels picked can, and else its rows are NaN
  *   workspace  sm100_marlin_kv4_workspace_bytes(dev) bytes, 16-byte aligned,
  *              the first 4096 zero before the first call (and left so by every
  *              one); calls that may overlap need their own

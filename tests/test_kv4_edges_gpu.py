@@ -121,3 +121,27 @@ def test_keys_next_to_zero(m, dim):  # noqa: F811
     p.k[::4] = (torch.rand(p.k[::4].shape, device=DEV) * tiny[torch.arange(88, device=DEV) % 6, None, None]).bfloat16()
     m.kv4_append(p.k, p.v, p.cache, p.slots)
     p.check(attend(m, p, lens, new))
+
+
+# ---------------------------------------------------------------------------
+# max_new
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_step_without_new_tokens(m, dim):  # noqa: F811
+    """Rows that only pad a step of fixed shape are zeros."""
+    p = Problem(m, [40, 0, 300], [0, 0, 0], 2, 4, dim, 64, torch.half, seed=40, pad=3)
+    assert not attend(m, p, [40, 0, 300], [0, 0, 0]).any()
+    none = torch.zeros(0, 1, dtype=torch.int32, device=DEV)
+    assert not m.kv4_attention(p.q, p.cache, none, ints([]), starts=ints([0]), max_new=0).any()
+
+
+def test_requests_with_more_rows_than_max_new(m):  # noqa: F811
+    """They are served, or their rows are NaN; the others' rows are what they are."""
+    lens, new = [131, 200, 90, 128, 300], [2, 1, 0, 30, 300]
+    p = Problem(m, lens, new, 2, 2, 64, 32, torch.half, seed=41, pad=2)
+    for most in (0, 1, 2, 31):
+        out = m.kv4_attention(p.q, p.cache, p.tables, ints(lens), starts=ints(p.starts), max_new=most)
+        assert torch.isnan(out[33:333]).all()
+        out[33:333] = attend(m, p, lens, new)[33:333]
+        p.check(out)
+    p.check(m.kv4_attention(p.q, p.cache, p.tables, ints(lens), starts=ints(p.starts), max_new=33))
