@@ -69,6 +69,7 @@ SIGNATURES = {
                                             _c_int, _vp, _i64, _c_int, _vp, _vp, _c_int, _c_int,
                                             _c_int, _c_int, _c_int, ctypes.c_float, _vp, _vp,
                                             _size, _c_int, _vp]),
+    "sm100_marlin_kv4_stall": (_c_int, [_c_int]),
     "sm100_marlin_kv4_workspace_bytes": (_size, [_c_int]),
 }
 

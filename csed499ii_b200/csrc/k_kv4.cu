@@ -90,6 +90,8 @@ int allow_smem(int dev, int bytes) {
 // 372 and 245.
 constexpr int kFewRows = 64;
 
+std::atomic<int> stalled_cta{-1};  // sm100_marlin_kv4_stall
+
 // Counters of the decode kernel's grid, then either kernel's parts.
 constexpr size_t kCounterBytes = 4096;
 constexpr size_t kPromptPart = 256 * (128 + 2);
@@ -289,7 +291,8 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
                          static_cast<uint8_t*>(out), block_tables, table_stride, width, lens, starts,
                          0, batch, rows, 1, most <= few_rows, q_heads, group, window, few_rows, scale,
                          static_cast<int*>(workspace),
-                         reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status};
+                         reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status,
+                         stalled_cta.load(std::memory_order_relaxed)};
   const PromptParams many{c, static_cast<const uint8_t*>(q), q_row, q_head, vector, static_cast<uint8_t*>(out),
                           block_tables, table_stride, width, lens, starts, batch, rows, q_heads,
                           group, window, few_rows, scale, 0, few.partials, status};
@@ -301,6 +304,12 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
                               : launch_decode<T, D, 2>(few, sms, dev, on_stream);
     return bad || most <= few_rows ? bad : launch_prompt<T, D>(many, sms, dev, on_stream);
   });
+}
+
+int sm100_marlin_kv4_stall(int cta) {
+  if (cta < -1) return SM100_MARLIN_ERR_ARGUMENT;
+  stalled_cta.store(cta, std::memory_order_relaxed);
+  return SM100_MARLIN_OK;
 }
 
 size_t sm100_marlin_kv4_workspace_bytes(int dev) {

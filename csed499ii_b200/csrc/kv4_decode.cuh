@@ -80,6 +80,7 @@ struct DecodeParams {
   int* counters;         // [grid], zero between launches
   float* partials;       // [grid][2] parts
   int* status;
+  int stalled;           // CTA whose first warp waits for more than comes (-1: none), for tests
 };
 
 template <int D, int NT>
@@ -357,7 +358,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
 
-  if (lane < kDepth) mbar_init(smem_addr(bars + kDepth * warp + lane), 1);
+  if (lane < kDepth)
+    mbar_init(smem_addr(bars + kDepth * warp + lane), warp == 0 && static_cast<int>(blockIdx.x) == p.stalled ? 2 : 1);
   if (lane < 2) segments[2 * warp + lane].begin = -1;
   if (threadIdx.x == 0) *abort_flag = *drain_flag = 0;
   fence_mbar_init();
@@ -832,7 +834,6 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
     }
   }
   __syncthreads();
-  if (*abort_flag) return;
 
   // --- parts of this CTA's warps, joined: a warp a row -------------------------
   using Row = Slice<D / 32>;
@@ -851,7 +852,22 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
                  : reinterpret_cast<const float*>(smem + Cfg::kOffParts) + (s >> 1) * kPart;
   };
   int open0 = -1, open1 = -1;  // segments of the items that other CTAs share: from before, into the next
-  {
+  if (*abort_flag) {
+    // The others still wait to be counted (or find their counter as it must be next
+    // time): what this CTA shares is handed on as a part that is NaN.
+    if (threadIdx.x < 2) {
+      const int at = threadIdx.x ? cta_end - 1 : cta_begin;
+      const Walk w = walk_to<kRows>(p, pre, at);
+      const int begin = at - (w.step - w.s.step0), end = begin + w.s.steps;
+      const bool shared = threadIdx.x ? begin >= cta_begin && end > cta_end : begin < cta_begin;
+      segments[threadIdx.x] = {shared ? begin : -1, end, w.b, w.head, w.chunk};
+      float* to = p.partials + (2ll * blockIdx.x + threadIdx.x) * kPart + kRows * D;
+      for (int r = 0; r < kRows; ++r) to[r] = 0.f, to[kRows + r] = CUDART_NAN_F;
+    }
+    __syncthreads();
+    if (segments[0].begin >= 0) open0 = 0;
+    if (segments[1].begin >= 0) open1 = 1;
+  } else {
     const int mine = lane < 2 * kWarps ? segments[lane].begin : -1;
     uint32_t left = __ballot_sync(0xffffffffu, mine >= 0);
     int unit = 0;

@@ -405,6 +405,12 @@ int sm100_marlin_kv4_attention(const void* q, int64_t q_row, int64_t q_head, con
                                int max_new, int window, float scale, void* out, void* workspace,
                                size_t workspace_bytes, int dev, void* stream);
 
+/* For tests: a wait for the cache of kv4_attention calls with few rows runs out in
+ * CTA `cta` (0.5 s each; -1: none, as at the start).  The call records
+ * SM100_MARLIN_STATUS_FULL_WAIT_TIMEOUT, results that the CTA has a part in are NaN
+ * or not written, and the workspace is as before any other call. */
+int sm100_marlin_kv4_stall(int cta);
+
 /* Bytes of kv4_attention's workspace on a device. */
 size_t sm100_marlin_kv4_workspace_bytes(int dev);
 

@@ -145,3 +145,33 @@ def test_requests_with_more_rows_than_max_new(m):  # noqa: F811
         out[33:333] = attend(m, p, lens, new)[33:333]
         p.check(out)
     p.check(m.kv4_attention(p.q, p.cache, p.tables, ints(lens), starts=ints(p.starts), max_new=33))
+
+
+# ---------------------------------------------------------------------------
+# a wait that runs out
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("lens,heads,group,ctas", [
+    ([30000], 1, 8, (0, 30, 58)),              # one item of all CTAs that work
+    ([30000] * 5, 1, 1, (0, 28, 144)),         # items with the same CTAs each
+    ([9000, 8000, 7000], 3, 3, (0, 1, 77, 140))])  # CTAs that share an item on either side
+def test_calls_after_a_wait_that_gave_up(m, lens, heads, group, ctas):  # noqa: F811
+    """The workspace is as it was, whichever CTA gave up, and the next calls are right."""
+    from csed499ii_b200 import _ext
+
+    lib = _ext.load()
+    assert m.device_status(0) == 0
+    p = Problem(m, lens, [1] * len(lens), heads, group, 128, 64, torch.half, seed=42)
+    space = m.kv4_workspace(DEV)
+    args = (p.q, p.cache, p.tables, ints(lens))
+    want = m.kv4_attention(*args, workspace=space)
+    p.check(want)
+    for cta in ctas:
+        assert lib.sm100_marlin_kv4_stall(cta) == 0
+        try:
+            out = m.kv4_attention(*args, workspace=space)
+        finally:
+            assert lib.sm100_marlin_kv4_stall(-1) == 0
+        assert m.device_status(0) != 0 and m.device_status(0) == 0
+        assert not torch.equal(out, want) and not space[:1024].any()
+        for _ in range(3):
+            assert torch.equal(m.kv4_attention(*args, workspace=space), want)
