@@ -256,20 +256,32 @@ _workspaces = {}
 
 
 def kv4_workspace(device="cuda"):
-    """A zeroed workspace for :func:`kv4_attention` calls that follow one another."""
+    """A workspace for :func:`kv4_attention` calls that follow one another (its
+    first 4096 bytes are zero, and left so by every call)."""
     device = torch.device(device)
     dev = device.index if device.index is not None else torch.cuda.current_device()
-    return torch.zeros(max(_ext.load().sm100_marlin_kv4_workspace_bytes(dev), 16) // 4, dtype=_INT32,
-                       device=torch.device("cuda", dev))
+    space = torch.empty(max(_ext.load().sm100_marlin_kv4_workspace_bytes(dev), 4096) // 4, dtype=_INT32,
+                        device=torch.device("cuda", dev))
+    space[:1024].zero_()
+    return space
+
+
+def _capturing(dev):
+    """Whether the current stream of ``dev`` is being captured into a graph."""
+    if dev == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def _workspace(dev, stream):
+    # A graph may be replayed beside the stream that it was captured on, and beside
+    # other graphs: it gets its own, in its own memory.  (Stream 0 cannot be captured.)
+    if stream and _capturing(dev):
+        return kv4_workspace(torch.device("cuda", dev))
     found = _workspaces.get((dev, stream))
     if found is None:
-        found = kv4_workspace(torch.device("cuda", dev))
-        # a graph's memory is the graph's own: nothing made in a capture is kept
-        if not torch.cuda.is_current_stream_capturing():
-            _workspaces[dev, stream] = found
+        found = _workspaces[dev, stream] = kv4_workspace(torch.device("cuda", dev))
     return found
 
 
@@ -298,7 +310,8 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
     @scale: of the scores, default ``1 / sqrt(head_dim)``
     @out: ``(rows, heads, head_dim)``, contiguous
     @workspace: :func:`kv4_workspace`; None: one that the module keeps for the
-        current stream
+        current stream, or in a capture one that is the graph's own.  Graphs
+        that share a memory pool share it too: do not replay them at once
     """
     fast = _ext._torch_fast if _ext._torch_fast_tried else _ext.torch_fast()
     if fast is not None and out is None and cache.is_cuda:

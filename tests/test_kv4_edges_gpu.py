@@ -175,3 +175,50 @@ def test_calls_after_a_wait_that_gave_up(m, lens, heads, group, ctas):  # noqa: 
         assert not torch.equal(out, want) and not space[:1024].any()
         for _ in range(3):
             assert torch.equal(m.kv4_attention(*args, workspace=space), want)
+
+
+# ---------------------------------------------------------------------------
+# workspaces of graphs
+# ---------------------------------------------------------------------------
+def test_a_graph_has_its_own_workspace(m):  # noqa: F811
+    """Also where calls on the captured stream came before: neither the module's
+    workspace for that stream nor that of another graph is in it."""
+    from csed499ii_b200 import kv4
+
+    p = Problem(m, [9000, 40], [1, 1], 2, 8, 128, 64, torch.half, seed=43)
+    lens = ints(p.lens)
+    want = m.kv4_attention(p.q, p.cache, p.tables, lens)
+    p.check(want)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(DEV) for _ in range(3)]
+    graphs, outs = [], []
+    with torch.cuda.stream(streams[0]):
+        m.kv4_attention(p.q, p.cache, p.tables, lens)
+        for _ in range(2):
+            streams[0].synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=streams[0]):
+                outs.append(m.kv4_attention(p.q, p.cache, p.tables, lens))
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    kept = kv4._workspaces[0, streams[0].cuda_stream]
+    kept[:1024] = 1  # counters that no call would join by
+    for graph, out in zip(graphs, outs):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    kept[:1024] = 0
+    for _ in range(20):  # both graphs and calls on the captured stream at once
+        torch.cuda.synchronize()
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        got = []
+        for _ in range(5):
+            for graph, stream in zip(graphs, streams[1:]):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            with torch.cuda.stream(streams[0]):
+                got.append(m.kv4_attention(p.q, p.cache, p.tables, lens))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x in got + outs)
