@@ -127,7 +127,7 @@ struct Place {
 
   __device__ __forceinline__ Place(const Cache& cache, int slot, int head) {
     const int page = slot / cache.page_size, place = slot - page * cache.page_size;
-    tile = cache.page_tiles<D>(page, head) + (place / kTile) * tile_bytes(D);
+    tile = cache.tile<D>(page, head, place / kTile);
     at = place % kTile;
   }
   // of channels [8 o, 8 o + 8)

@@ -492,10 +492,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
         there[warp * kDepth + slot] = (ok0 ? 1 : 0) | (ok1 ? 2 : 0);
         if (nth + 1 < per_page && ok0) {  // both tiles of one page
           mbar_arrive_expect_tx(bar, 2 * kBytes);
-          bulk_g2s(dst, p.cache.page_tiles<D>(page0, in.head) + nth * kBytes, 2 * kBytes, bar, policy);
+          bulk_g2s(dst, p.cache.tile<D>(page0, in.head, nth), 2 * kBytes, bar, policy);
         } else if (ok0 || ok1) {
           mbar_arrive_expect_tx(bar, (ok0 ? kBytes : 0) + (ok1 ? kBytes : 0));
-          if (ok0) bulk_g2s(dst, p.cache.page_tiles<D>(page0, in.head) + nth * kBytes, kBytes, bar, policy);
+          if (ok0) bulk_g2s(dst, p.cache.tile<D>(page0, in.head, nth), kBytes, bar, policy);
           if (ok1) bulk_g2s(dst + kBytes, p.cache.page_tiles<D>(page1, in.head), kBytes, bar, policy);
         } else {
           mbar_arrive(bar);

@@ -60,6 +60,11 @@ struct Cache {
     return tiles + (static_cast<int64_t>(page) * heads + head) * (page_size / kTile) *
                        static_cast<int64_t>(tile_bytes(D));
   }
+  // Tile `nth` of (page, head); a page alone can pass 2 GB.
+  template <int D>
+  __device__ __forceinline__ uint8_t* tile(int page, int head, int nth) const {
+    return page_tiles<D>(page, head) + static_cast<int64_t>(nth) * tile_bytes(D);
+  }
 };
 
 // Two floats in one register pair, for the two-wide instructions.

@@ -465,7 +465,7 @@ template <class T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     kv4_prompt_kernel(const __grid_constant__ PromptParams p) {
   using Cfg = PromptCfg<D>;
-  constexpr int kBytes = tile_bytes(D), kStep = Cfg::kStep, kTiles = Cfg::kTiles, kN = Cfg::kN;
+  constexpr int kStep = Cfg::kStep, kTiles = Cfg::kTiles, kN = Cfg::kN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -940,7 +940,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (static_cast<int64_t>(t) * kTile < len) {
           const int page = p.tables[p.table_stride * b + t / per_page];
           if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.pages))
-            at = reinterpret_cast<uint64_t>(p.cache.page_tiles<D>(page, head) + t % per_page * kBytes);
+            at = reinterpret_cast<uint64_t>(p.cache.tile<D>(page, head, t % per_page));
         }
         tiles[8 * (it & 3) + lane] = at;
       }

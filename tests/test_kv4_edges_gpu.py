@@ -222,3 +222,21 @@ def test_a_graph_has_its_own_workspace(m):  # noqa: F811
                 got.append(m.kv4_attention(p.q, p.cache, p.tables, lens))
         torch.cuda.synchronize()
         assert all(torch.equal(x, want) for x in got + outs)
+
+
+# ---------------------------------------------------------------------------
+# large pages
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("new", [1, 150])
+def test_offsets_past_32_bits_inside_a_page(m, new):  # noqa: F811
+    """One page of 2^24 tokens takes 2.3 GB; the request's tokens are its last ones."""
+    n, page, dim = 16384, 2**24, 128
+    p = Problem(m, [n], [new], 1, 4, dim, 64, torch.half, seed=44)
+    cache = torch.empty(1, 1, page // 16, 8 * dim + 64, dtype=torch.half, device=DEV)
+    slots = torch.arange(page - n, page, dtype=torch.int32, device=DEV)
+    m.kv4_append(p.k, p.v, cache, slots)
+    k, v = m.kv4_read(cache, slots)
+    assert torch.equal(k, R.values(p.k).half()) and torch.equal(v, R.values(p.v).half())
+    # the window leaves the rest of the page unseen
+    p.check(m.kv4_attention(p.q, cache, ints([[0]]), ints([page]), starts=ints(p.starts), max_new=new,
+                            window=5000), 5000)
