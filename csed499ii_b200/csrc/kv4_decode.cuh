@@ -103,6 +103,13 @@ struct DecodeCfg {
   static_assert((kWarps + kRows) * (2 * D + 8) * 4 <= kRing, "sheets do not fit the rings");
 };
 
+// Tokens of a request: what its table can hold, and few enough that a step past the
+// last one still has a 32-bit position.
+__device__ __forceinline__ int held_tokens(int len, int width, int page_size) {
+  const int64_t room = min(static_cast<int64_t>(width) * page_size, static_cast<int64_t>(0x7fffff00));
+  return max(static_cast<int>(min(static_cast<int64_t>(len), room)), 0);
+}
+
 // What a launch knows about one request.
 struct Span {
   int first, n, len;    // query rows, tokens
@@ -115,8 +122,7 @@ __device__ __forceinline__ Span span_of(const DecodeParams& p, int b) {
   Span s;
   s.first = p.starts ? min(max(p.starts[b], 0), p.rows) : p.row0 + b;
   s.n = p.starts ? min(p.starts[b + 1], p.rows) - s.first : 1;
-  const int64_t room = static_cast<int64_t>(p.width) * p.cache.page_size;
-  s.len = static_cast<int>(min(static_cast<int64_t>(p.lens[b]), room));
+  s.len = held_tokens(p.lens[b], p.width, p.cache.page_size);
   const int64_t rows = static_cast<int64_t>(s.n) * p.group;
   const bool mine = s.n > 0 && rows <= p.most;
   s.chunks = mine ? (static_cast<int>(rows) + ROWS - 1) / ROWS : 0;

@@ -440,8 +440,7 @@ __device__ __forceinline__ PromptItem prompt_item(const PromptParams& p, const i
   x.tile = item - (x.b ? pre[x.b - 1] : 0);
   x.first = min(max(p.starts[x.b], 0), p.rows);
   x.n = min(p.starts[x.b + 1], p.rows) - x.first;
-  const int64_t room = static_cast<int64_t>(p.width) * p.cache.page_size;
-  x.len = static_cast<int>(min(static_cast<int64_t>(p.lens[x.b]), room));
+  x.len = held_tokens(p.lens[x.b], p.width, p.cache.page_size);
   x.rows = min(256, x.n * p.group - x.tile * 256);
   x.before = x.len - x.n;
   const int lo = x.before + x.tile * 256 / p.group, hi = x.before + (x.tile * 256 + x.rows - 1) / p.group;

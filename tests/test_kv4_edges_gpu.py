@@ -240,3 +240,19 @@ def test_offsets_past_32_bits_inside_a_page(m, new):  # noqa: F811
     # the window leaves the rest of the page unseen
     p.check(m.kv4_attention(p.q, cache, ints([[0]]), ints([page]), starts=ints(p.starts), max_new=new,
                             window=5000), 5000)
+
+
+def test_the_longest_requests(m):  # noqa: F811
+    """A table of 128 entries that are one page of 2^24 tokens holds 2^31: the last
+    steps of such a request end at the limit of 32 bits."""
+    page, dim, new = 2**24, 64, [1, 5, 100]
+    cache = torch.zeros(1, 1, page // 16, 8 * dim + 64, dtype=torch.half, device=DEV)
+    p = Problem(m, [3000] * 3, new, 1, 2, dim, 64, torch.half, seed=45)
+    most = 2**31 - 256  # its last token is at 2^24 - 257 of the page
+    m.kv4_append(p.k[:3000], p.v[:3000], cache, torch.arange(page - 3256, page - 256, dtype=torch.int32, device=DEV))
+    p.k, p.v = p.k[:3000].repeat(3, 1, 1), p.v[:3000].repeat(3, 1, 1)
+    for lens in ([most] * 3, [2**31 - 1] * 3):
+        p.check(m.kv4_attention(p.q, cache, torch.zeros(3, 128, dtype=torch.int32, device=DEV), ints(lens),
+                                starts=ints(p.starts), max_new=100, window=700), 700)
+    assert not m.kv4_attention(p.q, cache, torch.zeros(3, 128, dtype=torch.int32, device=DEV), ints([-2**31, -5, 0]),
+                               starts=ints(p.starts), max_new=100, window=700).any()
