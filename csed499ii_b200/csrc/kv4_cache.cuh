@@ -36,9 +36,11 @@ struct ReadParams {
   int tokens;
 };
 
-// 8 channels as 4 words of two.
+// 8 channels as 4 words of two.  Not through the read-only path: this kernel has
+// begun while the one before it may still write them, and loads of that path need
+// not stay behind the wait.
 __device__ __forceinline__ uint4 load_8(const uint8_t* p, bool aligned) {
-  if (aligned) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (aligned) return *reinterpret_cast<const uint4*>(p);
   const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
   uint4 x;
   x.x = e[0] | static_cast<uint32_t>(e[1]) << 16;

@@ -256,3 +256,28 @@ def test_the_longest_requests(m):  # noqa: F811
                                 starts=ints(p.starts), max_new=100, window=700), 700)
     assert not m.kv4_attention(p.q, cache, torch.zeros(3, 128, dtype=torch.int32, device=DEV), ints([-2**31, -5, 0]),
                                starts=ints(p.starts), max_new=100, window=700).any()
+
+
+# ---------------------------------------------------------------------------
+# inputs written right before
+# ---------------------------------------------------------------------------
+def test_keys_written_by_the_call_before(m):  # noqa: F811
+    """kv4_append begins while the projection before it ends: its rows are the new ones."""
+    k, heads, dim, rows = 2048, 4, 128, 48
+    g = torch.Generator(device=DEV).manual_seed(46)
+    layer = m.Layer_2_4(k, 2 * heads * dim, groupsize=128).to(DEV)
+    w = torch.randn(k, 2 * heads * dim, generator=g, device=DEV).half() * 0.02
+    layer.pack(type("W", (), {"weight": w, "bias": None})(), (w.view(k // 128, 128, -1).abs().amax(1) / 7).half())
+    xs = [torch.randn(rows, k, generator=g, device=DEV).half() for _ in range(2)]
+    want = [R.values(layer(x).view(rows, -1, dim)).half().split(heads, 1) for x in xs]
+    workspace = torch.zeros(2 * heads * dim // 128 * 16, dtype=torch.int32, device=DEV)
+    out = torch.zeros(rows, 2 * heads * dim, dtype=torch.half, device=DEV)
+    cache = m.kv4_cache(3, heads, dim, 16, torch.half, DEV)
+    slots = ints(list(range(rows)))
+    for i in range(60):  # the same output, read by the call before, and written again
+        m.mul_2_4(xs[i % 2], layer.B, layer.meta, out, layer.s, workspace)
+        m.kv4_append(*out.view(rows, -1, dim).split(heads, 1), cache, slots)
+        got = m.kv4_read(cache, slots)
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i % 2])), i
