@@ -204,9 +204,15 @@ int sm100_marlin_kv4_schedule(const int* new_lens, const int* lens, int* block_t
         kv4_schedule_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 20 * kMaxBatch);
     if (e != cudaSuccess) return cuda_fail(e);
   }
-  // One CTA where the lengths or the count are updated in place: the others
-  // would read them while it writes.
-  const bool in_place = lens_out == lens || free_count_out == free_count;
+  // One CTA where the new lengths or the new count lie in what is read: the others
+  // would read it while it writes.
+  auto overlap = [](const int* a, int64_t n, const int* b, int64_t m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + 4 * m && y < x + 4 * n && n > 0 && m > 0;
+  };
+  bool in_place = overlap(lens_out, batch, free_count, 1) || overlap(free_count_out, 1, free_count, 1);
+  for (const int* in : {new_lens, lens})
+    in_place |= overlap(lens_out, batch, in, batch) || overlap(free_count_out, 1, in, batch);
   const int ctas = in_place ? 1 : 1 + (rows > batch ? rows : batch) / kScheduleThreads;
   return launched(launch(kv4_schedule_kernel, dim3(ctas < 148 ? ctas : 148), kScheduleThreads, smem,
                          static_cast<cudaStream_t>(stream), p));

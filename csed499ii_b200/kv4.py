@@ -129,9 +129,9 @@ def kv4_schedule(new_lens, lens, block_tables, free_pages, free_count, rows, pag
     @free_pages: ``torch.int``; pages given back are written from ``free_count`` on
     @free_count: ``torch.int`` ``(1,)``
     @rows: rows of the step, padding included (slot -1, position 0 past the last request's)
-    @lens_out, @free_count_out: tensors for the new lengths and count; ``lens``
-        and ``free_count`` themselves are allowed (a step that is replayed from
-        a CUDA graph updates them in place)
+    @lens_out, @free_count_out: tensors for the new lengths and count; they may
+        lie in ``new_lens``, ``lens`` and ``free_count`` (a step that is replayed
+        from a CUDA graph updates the last two in place)
     """
     fast = _ext._torch_fast if _ext._torch_fast_tried else _ext.torch_fast()
     if fast is not None:

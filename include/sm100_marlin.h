@@ -346,7 +346,8 @@ int sm100_marlin_set_trace_buffer(void* buf);
  * refused too.  Writes
  *   block_tables   the new entries of requests that grow
  *   free_pages     the pages given back, from entry *free_count on
- *   lens_out, free_count_out   after the step (may be lens and free_count)
+ *   lens_out, free_count_out   after the step (may lie in new_lens, lens and
+ *                  free_count; no other output may lie in an input)
  *   starts         [batch + 1] first row of each request (of all, refused too)
  *   slots, positions   [rows]; past the last request's rows -1 and 0
  *   fate           [batch], SM100_MARLIN_KV4_*

@@ -4,11 +4,13 @@ Tolerances are those that ``kv4_reference.attention`` derives; where values are
 scaled by a power of two, which is exact in every step of the format, results
 are scaled back and held to the bound of the values before.
 """
+import random
+
 import pytest
 import torch
 
 import kv4_reference as R
-from test_kv4_gpu import DEV, TYPES, Problem, ints, m  # noqa: F401  (m is the fixture)
+from test_kv4_gpu import DEV, KINDS, TYPES, Problem, ints, m, schedule_case  # noqa: F401  (m is the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -281,3 +283,32 @@ def test_keys_written_by_the_call_before(m):  # noqa: F811
         if i % 3 == 0:
             torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want[i % 2])), i
+
+
+# ---------------------------------------------------------------------------
+# scheduling into its inputs
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("where", ["new_lens", "lens, shifted", "new_lens, count in lens", "count first in lens"])
+def test_schedule_writes_into_any_input(m, where):  # noqa: F811
+    """New lengths and count that lie in what the step reads, with rows for many CTAs."""
+    rng = random.Random(47)
+    batch, page = 1300, 16
+    for _ in range(5):
+        new, lens, tables, free, count = schedule_case(rng, batch, page, 25, 300, 6000, KINDS["mixed"])
+        rows = sum(max(0, x) for x in new) + 9
+        want = R.schedule(new, lens, tables, free, count, rows, page)
+        t_new, t_tables, t_free, t_count = ints(new), ints(tables), ints(free), ints([count])
+        both = ints(lens + [0])
+        t_lens, lens_out, count_out = both[:-1], t_new, None
+        if where == "lens, shifted":
+            lens_out = both[1:]
+        elif where == "new_lens, count in lens":
+            count_out = t_lens[700:701]
+        elif where == "count first in lens":
+            lens_out, count_out = None, t_lens[:1]
+        step = m.kv4_schedule(t_new, t_lens, t_tables, t_free, t_count, rows, page, lens_out=lens_out,
+                              free_count_out=count_out)
+        for name in ("lens", "starts", "slots", "positions", "fate"):
+            assert getattr(step, name).tolist() == want[name], name
+        assert step.free_count.item() == want["free_count"]
+        assert t_tables.tolist() == want["tables"] and t_free.tolist() == want["free"]
