@@ -150,7 +150,8 @@ def kv4_schedule(new_lens, lens, block_tables, free_pages, free_count, rows, pag
             and free_pages.dtype is _INT32 and free_pages.get_device() == dev
             and free_count.dtype is _INT32 and free_count.get_device() == dev and free_count.numel() == 1
             and new_lens.is_contiguous() and lens.is_contiguous() and block_tables.is_contiguous()
-            and free_pages.is_contiguous() and rows >= 0 and 0 < page_size < 2**31):
+            and free_pages.is_contiguous() and 0 <= rows < 2**31 and 0 < page_size < 2**31
+            and free_pages.numel() < 2**31 and tables_shape[1] < 2**31):
         if dev < 0:
             raise RuntimeError("new_lens must be a CUDA tensor")
         _check_ints("new_lens", new_lens, dev)
@@ -160,8 +161,10 @@ def kv4_schedule(new_lens, lens, block_tables, free_pages, free_count, rows, pag
         _check_tables(block_tables, dev, batch)
         if batch > 8192:
             raise RuntimeError("kv4_schedule takes at most 8192 requests")
-        if rows < 0 or not 0 < page_size < 2**31:
-            raise RuntimeError("rows must not be negative, page_size must be positive")
+        if not (0 <= rows < 2**31 and 0 < page_size < 2**31):
+            raise RuntimeError("rows must not be negative, page_size must be positive, both below 2**31")
+        if free_pages.numel() >= 2**31 or tables_shape[1] >= 2**31:
+            raise RuntimeError("free_pages and the rows of block_tables must have less than 2**31 entries")
     if lens_out is None:
         lens_out = torch.empty_like(lens)
     else:
@@ -329,10 +332,13 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
     if not (q.dtype is cache.dtype and q.get_device() == dev and len(shape) == 3 and shape[2] == dim
             and at[2] == 1 and lens.dtype is _INT32 and lens.get_device() == dev and lens.is_contiguous()
             and block_tables.dtype is _INT32 and block_tables.get_device() == dev
-            and len(tables_shape) == 2 and tables_shape[0] == batch and block_tables.is_contiguous()):
+            and len(tables_shape) == 2 and tables_shape[0] == batch and block_tables.is_contiguous()
+            and max(batch, shape[0], tables_shape[1]) < 2**31 - 1):
         _check_rows("q", q, cache, None, dim, dev)
         _check_ints("lens", lens, dev)
         _check_tables(block_tables, dev, batch)
+        if max(batch, shape[0], tables_shape[1]) >= 2**31 - 1:
+            raise RuntimeError("requests, rows of q and entries of a table must be less than 2**31 - 1")
     rows, q_heads = shape[0], shape[1]
     if q_heads == 0 or q_heads % heads != 0:
         raise RuntimeError(f"q must have a multiple of {heads} heads, got {q_heads}")

@@ -312,3 +312,10 @@ def test_schedule_writes_into_any_input(m, where):  # noqa: F811
             assert getattr(step, name).tolist() == want[name], name
         assert step.free_count.item() == want["free_count"]
         assert t_tables.tolist() == want["tables"] and t_free.tolist() == want["free"]
+
+
+def test_schedule_refuses_rows_past_32_bits(m):  # noqa: F811
+    one, tables = ints([1] * 3), ints([[0, 1]] * 3)
+    for rows, page in ((2**31, 16), (2**32 + 3, 16), (3, 2**31), (3, 2**32 + 16)):
+        with pytest.raises(RuntimeError, match="2\\*\\*31"):
+            m.kv4_schedule(one, one, tables, ints([2, 3]), ints([2]), rows, page)
