@@ -118,7 +118,7 @@ int launch_decode(DecodeParams p, int sms, int dev, cudaStream_t stream) {
   do {
     const int n = batch - done < slice ? batch - done : slice;
     p.batch = n;
-    p.pad = done + n == batch;
+    p.pad = (done + n == batch ? 1 : 0) | (done == 0 ? 2 : 0);
     const cudaError_t e = launch(kv4_decode_kernel<T, D, NT>, dim3(sms), Cfg::kThreads, Cfg::kSmem, stream, p);
     if (e != cudaSuccess) return cuda_fail(e);
     p.lens += n;

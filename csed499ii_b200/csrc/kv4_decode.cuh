@@ -70,7 +70,7 @@ struct DecodeParams {
   int row0;              // row of request 0 where starts is null
   int batch;
   int rows;              // of q
-  int pad;               // 1: rows past the last request are set to zero
+  int pad;               // 1: rows past the last request are set to zero; 2: those before the first are
   int alone;             // 1: no other kernel serves the requests that are left alone
   int q_heads;
   int group;             // query heads per key/value head
@@ -420,12 +420,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
       for (int64_t i = 16 * threadIdx.x; i < s.n * row_bytes; i += 16 * Cfg::kThreads)
         *reinterpret_cast<uint4*>(p.out + s.first * row_bytes + i) = make_uint4(x, x, x, x);
     }
-    const int end = !p.starts || !p.pad ? p.rows : p.batch ? max(p.starts[p.batch], 0) : 0;
+    const int before = p.starts && p.pad & 2 ? min(max(p.batch ? p.starts[0] : 0, 0), p.rows) : 0;
+    const int end = !p.starts || !(p.pad & 1) ? p.rows : min(max(p.batch ? p.starts[p.batch] : 0, before), p.rows);
 #pragma unroll 1
-    for (int row = min(end, p.rows) + blockIdx.x; row < p.rows; row += gridDim.x)
+    for (int i = blockIdx.x; i < before + p.rows - end; i += gridDim.x) {
+      const int64_t row = i < before ? i : end + i - before;
 #pragma unroll 1
-      for (int64_t i = 16 * threadIdx.x; i < row_bytes; i += 16 * Cfg::kThreads)
-        *reinterpret_cast<uint4*>(p.out + row * row_bytes + i) = make_uint4(0, 0, 0, 0);
+      for (int64_t j = 16 * threadIdx.x; j < row_bytes; j += 16 * Cfg::kThreads)
+        *reinterpret_cast<uint4*>(p.out + row * row_bytes + j) = make_uint4(0, 0, 0, 0);
+    }
   }
 
   // --- this CTA's steps -----------------------------------------------------

@@ -302,7 +302,7 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
     Request ``b``'s rows of ``q`` are ``starts[b]:starts[b + 1]``, the last of
     its ``lens[b]`` tokens (append them first); each sees the keys up to its
     own position and, with ``window``, only that many of them.  Rows that see
-    nothing and rows past the last request are zeros.
+    nothing and rows of no request are zeros.
     @q: ``(rows, heads, head_dim)`` of the cache's type, ``heads`` a multiple of
         the cache's; rows and heads may have any stride
     @block_tables: ``torch.int`` ``(batch, width)``, @lens: ``torch.int`` ``(batch,)``

@@ -384,8 +384,9 @@ int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_s
  * starts[b + 1]) (starts NULL: row b alone, and rows == batch) and are the
  * last tokens of the lens[b] that it has in the cache: row i of n sees keys up
  * to its own position lens[b] - n + i and, with window > 0, only the last
- * `window` of those.  A row that sees nothing, and rows past the last request,
- * get zeros; entries of the table outside the cache are keys that nobody sees.
+ * `window` of those.  A row that sees nothing, and rows of no request (past
+ * the last, or before the first), get zeros; entries of the table outside the
+ * cache are keys that nobody sees.
  * A request has at most what its table holds, and 2^31 - 256 tokens.
  * A value's scale below 2^-90 (bf16 values smaller than 2^-75) counts as 2^-90.
  *   q          element (row, head, c) at row * q_row + head * q_head + c

@@ -23,7 +23,7 @@ def attend(m, p, lens, new, **kw):  # noqa: F811
 # sizes of values
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("power", [-85, -70, -50, 0, 50, 70])
+@pytest.mark.parametrize("power", [-85, -70, -50, 0, 50, 70, 120])
 def test_values_of_any_exponent(m, dim, power):  # noqa: F811
     """The same values times a power of two: the same results times it."""
     lens, new = [400, 150], [1, 150]
@@ -31,6 +31,14 @@ def test_values_of_any_exponent(m, dim, power):  # noqa: F811
     m.kv4_append(p.k, p.v * 2.0**power, p.cache, p.slots)
     # of the result; the check is of the unscaled values
     p.check((attend(m, p, lens, new).double() * 2.0**-power).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-30, -1e-9])
+def test_scales_next_to_zero(m, scale):  # noqa: F811
+    lens, new = [333, 200], [1, 200]
+    for dtype in TYPES:
+        p = Problem(m, lens, new, 2, 4, 64, 64, dtype, seed=49)
+        p.check(attend(m, p, lens, new, scale=scale), scale=scale)
 
 
 @pytest.mark.parametrize("power", [-130, -115, -100])
@@ -147,6 +155,20 @@ def test_requests_with_more_rows_than_max_new(m):  # noqa: F811
         out[33:333] = attend(m, p, lens, new)[33:333]
         p.check(out)
     p.check(m.kv4_attention(p.q, p.cache, p.tables, ints(lens), starts=ints(p.starts), max_new=33))
+
+
+@pytest.mark.parametrize("new", [[1, 2, 0], [1, 2, 300]])
+def test_rows_before_the_first_request(m, new):  # noqa: F811
+    lens = [131, 200, 300]
+    p = Problem(m, lens, new, 2, 2, 64, 32, torch.half, seed=48, pad=2)
+    q = torch.cat([torch.ones_like(p.q[:5]), p.q])
+    out = m.kv4_attention(q, p.cache, p.tables, ints(lens), starts=ints([5 + x for x in p.starts]), max_new=max(new))
+    assert not out[:5].any()
+    p.check(out[5:])
+    out = torch.full_like(q, 7.0)
+    m.kv4_attention(q, p.cache, p.tables, ints(lens), starts=ints([5 + x for x in p.starts]), max_new=max(new), out=out)
+    assert not out[:5].any()
+    p.check(out[5:])
 
 
 # ---------------------------------------------------------------------------
