@@ -10,16 +10,18 @@
 //
 // Codes 0..15 are exact in 16 bits and scale and offset stay in 32 bits
 // outside the products, so nothing is dequantised and nothing is rounded but
-// the weights w = p s.  They go into the products as halves: one for a bf16 model
-// (11 bits, where a result has 8), the sum of two for an fp16 model (22 bits; with one the
-// error of a result was 1.2 to 1.5 times that of a result rounded once, and 16 x
-// 1024 tokens of 32 heads took 25.2 us instead of 27.7).  The exponential gives w itself, its argument is the score plus log2 s, and the running
-// maximum is that of these arguments: a half then holds the weights that
-// matter whatever sizes the values have, and p is w / s in 32 bits.  sum(p) and the
-// offset term take the weights as they are, and the codes act as if centred on 8: a
-// rounding error meets at most 8 steps of its row's scale, never its offset, which
-// can be 2^15 scales (with rounded weights in the offset term one wide row among
-// 20000 narrow ones moved the result by 5 times what its rounding allows).
+// the weights w = p s.  They go into the products as halves: one for a bf16
+// model (11 bits, where a result has 8), the sum of two for an fp16 model (22
+// bits; with one the error of a result was 1.2 to 1.5 times that of a result
+// rounded once, and 16 x 1024 tokens of 32 heads took 25.2 us instead of 27.6).
+// The exponential gives w itself, its argument is the score plus log2 s, and the
+// running maximum is that of these arguments: a half then holds the weights that
+// matter whatever sizes the values have, and p is w / s in 32 bits.  sum(p) and
+// the offset term take the weights as they are, and the codes act as if centred
+// on 7.5: a rounding error meets at most 7.5 steps of its row's scale, never its
+// offset, which can be 2^15 scales (with rounded weights in the offset term one
+// wide row among 20000 narrow ones moved the result by 5 times what its rounding
+// allows).
 //
 // mma.m16n8k16 takes 16 tokens (scores) or 16 channels (result) as its rows
 // and 8 query rows as its columns; the 8 query heads of a group fill it.  Codes
@@ -256,8 +258,12 @@ __device__ __forceinline__ uint32_t key_odd(uint32_t w) {
 // log2 e: scores are kept as exponents of two.
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The middle of the codes: values are held as what they are off it and their value
+// at it, so that for values around zero neither's sum is much larger than the result.
+constexpr float kMid = 7.5f;
+
 // What the weights need to know of a row of values: its scale's logarithm and
-// reciprocal, and its value at code 8 over the scale.
+// reciprocal, and its value at code kMid over the scale.
 //
 // The sum of the weights is kept as sum(w / s), so 1 / s has to leave room for a
 // long sum in 32 bits: a scale below 2^-90 (bf16 values below 2^-75) counts as
@@ -267,7 +273,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // half: 2^-10 of the offset is below what its own value adds to the result, and
 // 2^-60 for a row of zeros is in the middle of what scales can be.
 struct ValueRow {
-  float log_s, inv_s, at_8;
+  float log_s, inv_s, at_mid;
 };
 __device__ __forceinline__ ValueRow value_row(float2 pair) {
   const float s = pair.x > 0.f ? fmaxf(fmaxf(pair.x, fabsf(pair.y) * 0x1p-30f), 0x1p-90f)
@@ -275,7 +281,7 @@ __device__ __forceinline__ ValueRow value_row(float2 pair) {
   ValueRow r;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r.log_s) : "f"(s));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inv_s) : "f"(s));
-  r.at_8 = fmaf(pair.y, r.inv_s, 8.f);
+  r.at_mid = fmaf(pair.y, r.inv_s, kMid);
   return r;
 }
 
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
     const uint32_t full = smem_addr(bars + kDepth * warp);
     // of each token of a step: key scale, key offset, log2 of the value scale
     float* tokens = reinterpret_cast<float*>(smem + Cfg::kOffTokens) + warp * 160;
-    float2* token_sums = reinterpret_cast<float2*>(tokens + 96);  // 1 / value scale, value at code 8 / scale
+    float2* token_sums = reinterpret_cast<float2*>(tokens + 96);  // 1 / value scale, value at code kMid / scale
     Walk at = walk_to<kRows>(p, pre, begin);
     // the first queries are on their way while the first pages are looked up
     {
@@ -592,14 +598,14 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
           const float2 kp = T::up(lds32(tile + off_k_pair(D, lane & 15)));
           const ValueRow v = value_row(T::up(lds32(tile + off_v_pair(D, lane & 15))));
           float4 x = make_float4(kp.x * c1, (kBf ? fmaf(kp.x, -128.f, kp.y) : kp.y) * c2, v.log_s, v.inv_s);
-          float at_8 = v.at_8;
-          if (!(fabsf(at_8) <= 3.4e38f)) x.y = CUDART_NAN_F, x.w = at_8 = 0.f;
+          float at_mid = v.at_mid;
+          if (!(fabsf(at_mid) <= 3.4e38f)) x.y = CUDART_NAN_F, x.w = at_mid = 0.f;
           if (j0 + lane >= at.s.len || !(there[warp * kDepth + slot] >> (lane >> 4) & 1))
-            x = make_float4(0.f, 0.f, -CUDART_INF_F, 0.f), at_8 = 0.f;
+            x = make_float4(0.f, 0.f, -CUDART_INF_F, 0.f), at_mid = 0.f;
           tokens[lane] = x.x;
           tokens[32 + lane] = x.y;
           tokens[64 + lane] = x.z;
-          token_sums[lane] = make_float2(x.w, at_8);
+          token_sums[lane] = make_float2(x.w, at_mid);
         }
         __syncwarp();
         // the arguments of the weights
@@ -717,7 +723,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
               const float2 r01 = Half::up(w01), r23 = Half::up(w23);
               w[0] -= r01.x, w[1] -= r01.y, w[2] -= r23.x, w[3] -= r23.y;
 #pragma unroll
-              for (int c = 0; c < 4; ++c) a1[nt][c & 1] = fmaf(-8.f, w[c], a1[nt][c & 1]);
+              for (int c = 0; c < 4; ++c) a1[nt][c & 1] = fmaf(-kMid, w[c], a1[nt][c & 1]);
               wb[u][nt][kTerms - 1][0] = transpose_8x8(Half::down(w[0], w[1]));
               wb[u][nt][kTerms - 1][1] = transpose_8x8(Half::down(w[2], w[3]));
             }
@@ -728,11 +734,12 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
             }
           }
         }
-        // Result.  A step's products are summed by themselves, begun with 8 times the
-        // rounded weights taken off, and added to the others in binary32: the tensor
+        // Result.  A step's products are summed by themselves, begun with kMid times
+        // the rounded weights taken off, and added to the others in binary32: the tensor
         // cores cut a sum off at 2^-23 of it with every product added, a bias over a
         // long run of one warp (131071 keys that weigh 2^-26 of a first one had 1.13
         // times the error that the rounding of weights allows).  It takes 4% of the time.
+        constexpr float kLess = -kMid * 0x1p-24f;
         constexpr int kOctets = D / 64;
         uint32_t va[2][kOctets], vb[2][kOctets], vc[2][kOctets], vd[2][kOctets];  // tokens 2t, 2t+1, 2t+8, 2t+9
 #pragma unroll
@@ -769,8 +776,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
                     float(&to)[4] = sums[nt][odd];
                     const uint32_t b0 = wb[u][nt][i][0], b1 = wb[u][nt][i][1];
                     if (u == 0 && i == 0) {
-                      mma_16816_from(to, c0, c1, c2, c3, b0, b1, ones[nt][0] * -0x1p-21f, ones[nt][1] * -0x1p-21f,
-                                     ones[nt][0] * -0x1p-17f, ones[nt][1] * -0x1p-17f);
+                      mma_16816_from(to, c0, c1, c2, c3, b0, b1, ones[nt][0] * kLess, ones[nt][1] * kLess,
+                                     ones[nt][0] * (16.f * kLess), ones[nt][1] * (16.f * kLess));
                     } else {
                       mma_16816<false>(to, c0, c1, c2, c3, b0, b1);
                     }

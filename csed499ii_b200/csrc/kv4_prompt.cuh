@@ -11,18 +11,18 @@
 //   S = Q (C_k - 8)^T     tcgen05.mma, Q and the codes in shared memory
 //   P                     in the softmax warps' registers, back to tensor
 //                         memory in the place of S
-//   O += P (C_v - 8)      tcgen05.mma, P from tensor memory
+//   O += P 2 (C_v - m)    tcgen05.mma, P from tensor memory; m is a row's middle code
 //
 // As in the decode kernel the operands are codes, exact in 16 bits, so that
 // nothing is rounded but the weights.  Here they are one half for either type: an
-// fp16 result of a prompt has 1.3 times the error of a result rounded once, and a
-// second product for what the rounding leaves, as the decode kernel has, would add
-// half of the step's tensor work and as many stores to tensor memory again.  What
-// scales and offsets add is put into
+// fp16 result has 1.2 to 1.45 times the error of a result rounded once (the weights'
+// roundings are as large as its own), and a second product for what the rounding
+// leaves, as the decode kernel has, would add half of the step's tensor work and as
+// many stores to tensor memory again.  What scales and offsets add is put into
 // the same products as 16 more channels, in two or three 16-bit terms each
 // (2^-22 of a value): with z = offset / s_k + 8 a key's argument of the
 // exponential is s_k (S + z sum(q) + log2 s_v / s_k), so its column of S needs
-// one multiply-add; and the columns 1 / s_v and offset / s_v + 8 next to the
+// one multiply-add; and the columns 1 / s_v and offset / s_v + m next to the
 // values' codes give sum(p) and the values' offsets with the result (the weights
 // are w = p s_v).  Without them every pair of keys costs the softmax ten
 // broadcast reads of shared memory, and those bound it (a prompt of 8192 tokens,
@@ -116,7 +116,7 @@ constexpr int kFreshSteps = 128;
 struct Numbers {
   float scale[128];  // of the key, times scale * log2 e
   float z[128];      // the key's value at code 8 over its scale
-  float log_s[128], inv_s[128], at_8[128];  // ValueRow
+  float log_s[128], inv_s[128], at_mid[128];  // of the value
 };
 
 template <int D>
@@ -134,7 +134,8 @@ struct PromptCfg {
   static constexpr int kOffKx = kOffQx + 2 * kQx;
   static constexpr int kOffNumbers = kOffKx + 2 * kKx;  // four stages
   static constexpr int kOffRows = kOffNumbers + 4 * sizeof(Numbers);  // [tile][half][row] of two numbers
-  static constexpr int kOffMisc = kOffRows + 2 * 2 * 128 * 8;
+  static constexpr int kOffMiddles = kOffRows + 2 * 2 * 128 * 8;  // [stage][key]: 1024 + twice a value's middle, a half
+  static constexpr int kOffMisc = kOffMiddles + 4 * 256;
   static constexpr int kSmem = kOffMisc + 1280 + 1024;  // and room to align
   static_assert(kSmem <= kPrefillSmemBudget && kK % 1024 == 0 && kV % 1024 == 0 && kKx % 256 == 0, "tiles");
   static constexpr uint32_t kColS = 0, kColO = 2 * kStep, kCols = 512;
@@ -304,6 +305,13 @@ __device__ __forceinline__ uint4 centred(uint32_t w) {
   return r;
 }
 
+// Twice what the codes in nibbles `at` of either half of `q` are off their rows'
+// middles (`middle` is 1024 + twice those).
+__device__ __forceinline__ half2 twice_off(uint32_t q, int at, half2 middle) {
+  const uint32_t x = lop3<kLutAndOr>(at ? q >> (4 * at - 1) : q << 1, 0x001e001eu, 0x64006400u);  // 1024 + 2 c
+  return __hsub2(*reinterpret_cast<const half2*>(&x), middle);
+}
+
 template <int N>
 __device__ __forceinline__ void take_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -393,9 +401,26 @@ template <class T>
 __device__ __forceinline__ bool terms_hold(float z, float log) {
   return T::kBf16 ? fabsf(z) < 1e30f && fabsf(log) < 1e30f : fabsf(z) < 60000.f && fabsf(log) < 1e9f;
 }
+// A value's row with the code nearest to its zero as the middle, in halves of a code:
+// what codes are off it sums up to the result itself, and its own value is at most a
+// quarter of the scale (more where a row does not reach zero).  With one middle for
+// all rows, codes and middles of values that are not symmetric about zero have sums
+// that cancel, and what the tensor cores cut off either stays: 30 times the error of
+// a result rounded once for exponentially distributed values less their mean, 20000 keys
+// of like weight.
+struct MiddleRow : ValueRow {
+  float twice;  // the middle, 0..30
+};
+__device__ __forceinline__ MiddleRow middle_row(float2 pair) {
+  MiddleRow r;
+  static_cast<ValueRow&>(r) = value_row(pair);
+  r.twice = rintf(fminf(fmaxf(-2.f * pair.y * r.inv_s, 0.f), 30.f));
+  r.at_mid = fmaf(pair.y, r.inv_s, 0.5f * r.twice);
+  return r;
+}
 // The values' two numbers go into halves, a quarter of inv_s in 2^-9..2^15.
 __device__ __forceinline__ bool sums_hold(const ValueRow& v) {
-  return v.inv_s >= 0x1p-7f && v.inv_s <= 0x1p17f && fabsf(v.at_8) < 60000.f;
+  return v.inv_s >= 0x1p-7f && v.inv_s <= 0x1p17f && fabsf(v.at_mid) < 60000.f;
 }
 
 // Inclusive prefix sums of the requests' items in `pre`, and their total.
@@ -826,7 +851,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const float rest = (z ? w1 : w0) - (bit(in_v, at + z) ? z ? w.y : w.x : 0.f);
                 if ((z ? x1 : x0) != -CUDART_INF_F) {
                   l[r] = fmaf(rest, k.inv_s[at + z], l[r]);
-                  off[r] = fmaf(rest, k.at_8[at + z], off[r]);
+                  off[r] = fmaf(rest, k.at_mid[at + z], off[r]);
                 }
               }
             }
@@ -871,6 +896,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       }
       const float over = sum == 0.f ? 0.f : 1.f / sum;
+      auto value = [&](uint32_t x) { return fmaf(0.5f, __uint_as_float(x), rest) * over; };  // codes were twice
       const bool whole = after[0] == 1, there = qi * 128 + row < after[3];
       const int at = after[2] + qi * 128 + row, at_token = at / p.group;
       uint8_t* dst = p.out + 2 * ((static_cast<int64_t>(after[1] + at_token) * p.q_heads + head * p.group + at -
@@ -902,9 +928,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             for (int i = 0; i < 4; ++i) {
               float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
               if (sum != 0.f)
-                y = make_float4((__uint_as_float(o[4 * i]) + rest) * over, (__uint_as_float(o[4 * i + 1]) + rest) * over,
-                                (__uint_as_float(o[4 * i + 2]) + rest) * over,
-                                (__uint_as_float(o[4 * i + 3]) + rest) * over);
+                y = make_float4(value(o[4 * i]), value(o[4 * i + 1]), value(o[4 * i + 2]), value(o[4 * i + 3]));
               to[i] = y;
             }
             continue;
@@ -912,9 +936,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            w[i] = sum == 0.f ? 0u
-                              : T::down((__uint_as_float(o[2 * i]) + rest) * over,
-                                        (__uint_as_float(o[2 * i + 1]) + rest) * over);
+            w[i] = sum == 0.f ? 0u : T::down(value(o[2 * i]), value(o[2 * i + 1]));
           *reinterpret_cast<uint4*>(dst + 32 * c) = make_uint4(w[0], w[1], w[2], w[3]);
           *reinterpret_cast<uint4*>(dst + 32 * c + 16) = make_uint4(w[4], w[5], w[6], w[7]);
         }
@@ -978,7 +1000,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const float2 ks = T::up(kp);
           const float s = ks.x > 0.f ? ks.x : fmaxf(fabsf(ks.y) * 0x1p-10f, 0x1p-10f);
           const float z = __fdividef(ks.y, s) + 8.f, scale = s * c2;
-          const ValueRow v = value_row(T::up(vp));
+          const MiddleRow v = middle_row(T::up(vp));
           const float log = __fdividef(v.log_s, scale);
           const bool held = here && terms_hold<T>(z, log);
           Numbers& k = numbers[buf];
@@ -986,7 +1008,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           k.z[id] = z;
           k.log_s[id] = v.log_s;
           k.inv_s[id] = v.inv_s;
-          k.at_8[id] = v.at_8;
+          k.at_mid[id] = v.at_mid;
+          reinterpret_cast<uint16_t*>(smem + Cfg::kOffMiddles + buf * 256)[id] =
+              static_cast<uint16_t>(Half::down(1024.f + v.twice, 0.f));
           const uint32_t mask = __ballot_sync(0xffffffffu, here);
           const uint32_t mask_k = __ballot_sync(0xffffffffu, held);
           const uint32_t mask_v = __ballot_sync(0xffffffffu, here && sums_hold(v));
@@ -1066,9 +1090,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (it >= 2) wait_warp(spent + 8 * (stage ^ 1), (it - 1) >> 1);
         const uint32_t dst = smem_addr(smem) + Cfg::kOffV + stage * Cfg::kV;
         if (id < kStep) {
-          const ValueRow v = value_row(T::up(vp));
+          const MiddleRow v = middle_row(T::up(vp));
           const bool held = here && sums_hold(v);
-          const float inv = held ? 0.25f * v.inv_s : 0.f, z = held ? v.at_8 : 0.f;
+          const float inv = held ? 0.25f * v.inv_s : 0.f, z = held ? v.at_mid : 0.f;
           const float h = rounded<Half>(inv), zh = rounded<Half>(z);
           const uint32_t x = Half::down(h, inv - h), y = Half::down(zh, z - zh);
           const uint32_t at = dst + (id >> 6) * (kN * 128) + 2 * (id & 7);
@@ -1080,6 +1104,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                          : "memory");
           }
         }
+        wait_warp(c_full + 8 * (it & 3), it >> 2);  // the middles are there
+        half2 middle[4];                            // of tokens 2t and 2t + 1
+        {
+          const uint4 x = lds128(smem_addr(smem) + Cfg::kOffMiddles + (it & 3) * 256 + 16 * half);
+          const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int t = 0; t < 4; ++t) middle[t] = *reinterpret_cast<const half2*>(&y[t]);
+        }
         if (serves)
 #pragma unroll
         for (int o = 0; o < kWordsV; ++o) {
@@ -1089,7 +1121,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {  // tokens 2t and 2t + 1
               const uint32_t y = prmt(w[2 * t * kWordsV + o], w[(2 * t + 1) * kWordsV + o], part < 2 ? 0x5410 : 0x7632);
-              dequant_pair(y >> (8 * (part & 1)), even[t], odd[t]);
+              even[t] = twice_off(y, 2 * (part & 1), middle[t]);
+              odd[t] = twice_off(y, 2 * (part & 1) + 1, middle[t]);
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {

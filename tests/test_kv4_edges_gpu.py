@@ -122,6 +122,26 @@ def test_fp16_results_of_few_rows_are_rounded_once(m, dim, group, new):  # noqa:
     assert (attend(m, p, [n], [new]).double() - want).norm() <= 1.15 * once
 
 
+@pytest.mark.parametrize("skewed", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,new,copies,most", [
+    (20000, 1, 2600, 1.15), (20000, 100, 80, 1.55), (4000, 300, 80, 1.55), (60000, 100, 1, 1.55)])
+def test_fp16_results_of_values_around_zero(m, dim, n, new, copies, most, skewed):  # noqa: F811
+    """Keys of like weight, so that values average out and what sums lose shows.
+
+    Few rows have the error of one rounding.  In the prompt kernel each weight is rounded as
+    the result is, which adds as much again: the root of two, and a little for all else."""
+    p = Problem(m, [n], [new], 1, 4, dim, 64, torch.half, seed=46, sharp=0.3)
+    if skewed:  # exponential less the mean: a row's zero is near its lowest codes
+        g = torch.Generator(device=DEV).manual_seed(47)
+        p.v = (-torch.log(torch.rand(p.v.shape, generator=g, device=DEV).clamp(min=1e-6)) - 1).half()
+        m.kv4_append(p.k, p.v, p.cache, p.slots)
+    want, _ = R.attention(p.q, p.k, p.v, new)
+    once = (want.half().double() - want).norm()
+    for out in attend_many(m, p, n, new, copies):
+        assert (out.double() - want).norm() <= most * once
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_keys_next_to_zero(m, dim):  # noqa: F811
     """Keys whose scale is a subnormal of the type, or of 32 bits: they weigh as zeros do."""
