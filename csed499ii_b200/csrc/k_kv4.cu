@@ -85,9 +85,9 @@ int allow_smem(int dev, int bytes) {
 }
 
 // Requests with at most this many query rows for a key/value head go to the
-// decode kernel, others to the prompt kernel.  At 64 requests, 8 heads of 128: 64
-// rows over 4096 tokens take 374 us here and 411 there, 128 rows over 2048 tokens
-// 372 and 245.
+// decode kernel, others to the prompt kernel.  At 64 requests, 8 heads of 128, over
+// 4096 tokens: 48 rows take 348 us here and 409 there, 64 rows 451 and 410 (bf16: 391
+// and 420); 128 rows over 2048 tokens 453 and 242.
 constexpr int kFewRows = 64;
 
 std::atomic<int> stalled_cta{-1};  // sm100_marlin_kv4_stall
@@ -145,7 +145,7 @@ int launch_prompt(PromptParams p, int sms, int dev, cudaStream_t stream) {
     if (items > 0) {
       // Items that leave half of the GPU idle share out their keys, if they can have
       // enough of them (a last launch joins them): 256 rows of each of 8 heads over 16384
-      // tokens take 90 us instead of 392.
+      // tokens take 87 us instead of 392.
       const int64_t keys = static_cast<int64_t>(p.width) * p.cache.page_size;
       p.split = batch <= kSplitBatch && 2 * items * heads <= sms && keys >= 2 * kLeastPromptSteps * PromptCfg<D>::kStep
                     ? sms / heads

@@ -5,10 +5,11 @@
 // other.  Eight lanes own one token and head, its key and its value row: a lane
 // holds D/64 pieces of 8 channels of both, 64 channels apart; the rows' ranges
 // are shuffle reductions, and the 8 codes of a piece are one 32-bit word of the
-// tile.  8192 tokens of 8 heads of 128: written in 11.3 us (42.5 MB, 3.8 TB/s; 62% of
-// issue slots are taken, the integer and the float pipe two fifths of the time each), read
-// in 8.0 us (5.3 TB/s of 6.55 measured for a copy).  With a lane for 8 channels of
-// a row the row's own numbers cost twice as much: 15.1 and 9.4 us.
+// tile.  8192 tokens of 8 heads of 128, one call after another: written in 13.0 us
+// (42.5 MB, 3.3 TB/s; 62% of issue slots are taken, the integer and the float pipe two
+// fifths of the time each), read in 9.1 us (4.7 TB/s of 6.55 measured for a copy).
+// With a lane for 8 channels of a row the row's own numbers cost twice as much, a
+// third and a sixth more time.
 #pragma once
 
 #include <math_constants.h>

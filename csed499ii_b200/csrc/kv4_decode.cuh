@@ -38,12 +38,14 @@
 // finishes last, in CTA order, so results do not depend on timing.
 //
 // Measured at 8 key/value heads of 128 and 8 query heads each: one request of
-// 131072 tokens (142.8 MB) in 45 us, 64 of up to 8192 (256 MB, bf16) in 80 us, 3.2
-// TB/s of 6.55 measured for a copy.  Instructions bound it: 290 a warp and tile, half
-// of them on the integer pipe (each takes a scheduler two cycles there) to turn
-// codes into operands, which is 120 cycles a tile and SM at the 52% of issue slots
-// that 16 warps of 128 registers fill.  Launch, first bytes, and joins in the CTA
-// and over CTAs are 16 us of the 45.
+// 131072 tokens (142.8 MB, fp16) in 50.6 us, 64 of up to 8192 (256 MB, bf16) in 82 us,
+// 2.8 and 3.1 TB/s of 6.55 measured for a copy.  Instructions bound it: 372 a warp and
+// tile in the first (its start and joins among them), two fifths of the time on the
+// integer pipe to turn codes into operands, at the 51% of issue slots that 16 warps of
+// 128 registers fill.  Those registers are not quite enough: D = 128 with one column
+// tile spills 88 bytes for fp16 models and 76 for bf16, D = 64 with two 448 and 256
+// (8 warps of 255 do not spill there: from 5% less time to 15% more).  Launch, first
+// bytes, and joins in the CTA and over CTAs are about 16 us of the 50.
 #pragma once
 
 #include <math_constants.h>
@@ -440,7 +442,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, 1)
   // --- this CTA's steps -----------------------------------------------------
   // Joining an item over CTAs costs about as much as kRoundSteps steps of one.
   // Where all items are as long, a CTA's share is rounded up to whole ones if
-  // that takes no more, or else every item gets the same CTAs to itself.
+  // that takes no more, or else every item gets the same CTAs to itself.  (16
+  // requests of 32 heads: 27.6 us at 1024 tokens each, 28.1 at 1000 to 1015.)
   const int ctas = gridDim.x, cta = blockIdx.x;
   int quota = (total + ctas - 1) / ctas, per_item = 0;  // CTAs that an item has to itself
   const bool even = longest == shortest;

@@ -103,7 +103,10 @@ def kv4_cache(pages, kv_heads, head_dim, page_size=64, dtype=torch.half, device=
 
 
 class KV4Step(NamedTuple):
-    """What :func:`kv4_schedule` returns; every field is an int32 tensor."""
+    """What :func:`kv4_schedule` returns; every field is an int32 tensor.
+
+    ``starts``, ``slots``, ``positions`` and ``fate`` can share one allocation: who
+    keeps one of them for long, or saves it, clones it."""
 
     lens: torch.Tensor        # (batch,) tokens in the cache after the step
     free_count: torch.Tensor  # (1,) free pages after the step
@@ -235,7 +238,8 @@ def kv4_append(k, v, cache, slots):
 
 def kv4_read(cache, slots):
     """Keys and values at ``slots``, each ``(tokens, kv_heads, head_dim)`` in the
-    cache's type; zeros where a slot is outside the cache."""
+    cache's type; zeros where a slot is outside the cache.  The two can share one
+    allocation."""
     fast = _ext._torch_fast if _ext._torch_fast_tried else _ext.torch_fast()
     if fast is not None:
         done = fast.kv4_read(cache, slots)
@@ -302,7 +306,9 @@ def kv4_attention(q, cache, block_tables, lens, starts=None, max_new=None, windo
     Request ``b``'s rows of ``q`` are ``starts[b]:starts[b + 1]``, the last of
     its ``lens[b]`` tokens (append them first); each sees the keys up to its
     own position and, with ``window``, only that many of them.  Rows that see
-    nothing and rows of no request are zeros.
+    nothing and rows of no request are zeros.  Sums are in 32 bits; the weights of
+    the values have 11 bits, or 22 for ``torch.half`` with at most 64 rows of a
+    request for a key/value head.
     @q: ``(rows, heads, head_dim)`` of the cache's type, ``heads`` a multiple of
         the cache's; rows and heads may have any stride
     @block_tables: ``torch.int`` ``(batch, width)``, @lens: ``torch.int`` ``(batch,)``

@@ -387,6 +387,9 @@ int sm100_marlin_kv4_read(const void* cache, int pages, int kv_heads, int page_s
  * `window` of those.  A row that sees nothing, and rows of no request (past
  * the last, or before the first), get zeros; entries of the table outside the
  * cache are keys that nobody sees.
+ * Sums are in binary32.  The weights of the values have 11 bits, or 22 for fp16
+ * where a request has at most 64 rows for a key/value head: an fp16 result of more
+ * rows has 1.2 to 1.45 times the error of one that is rounded once.
  * A request has at most what its table holds, and 2^31 - 256 tokens.
  * A value's scale below 2^-90 (bf16 values smaller than 2^-75) counts as 2^-90.
  *   q          element (row, head, c) at row * q_row + head * q_head + c
